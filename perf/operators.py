@@ -248,7 +248,7 @@ def _plain_codes(x):
     """(codes, scales, minima) of [tokens, heads, dim]: groups of 32 channels."""
     x = x.float().unflatten(-1, (-1, 32))
     lo, hi = x.amin(-1), x.amax(-1)
-    scale = ((hi - lo) / 15).half()
+    scale = ((hi - lo) / torch.full_like(hi, 15)).half()  # by a tensor: a division, not a product with 1/15
     wide = scale.float()[..., None]
     codes = torch.where(wide > 0, (x - lo[..., None]) / wide, 0.0).round().clamp(0, 15)
     return codes.to(torch.uint8), scale, lo.half()

@@ -248,7 +248,9 @@ def _plain_codes(x):
     """(codes, scales, minima) of [tokens, heads, dim]: groups of 32 channels."""
     x = x.float().unflatten(-1, (-1, 32))
     lo, hi = x.amin(-1), x.amax(-1)
-    scale = ((hi - lo) / torch.full_like(hi, 15)).half()  # by a tensor: a division, not a product with 1/15
+    step = (hi - lo) / torch.full_like(hi, 15)  # by a tensor: a division, not a product with 1/15
+    scale = step.half()  # rounded down, so that scale * 15 + lo is never beyond the type's range
+    scale = (scale.view(torch.int16) - (scale.float() > step).short()).view(torch.float16)
     wide = scale.float()[..., None]
     codes = torch.where(wide > 0, (x - lo[..., None]) / wide, 0.0).round().clamp(0, 15)
     return codes.to(torch.uint8), scale, lo.half()
@@ -393,7 +395,9 @@ def _exact_quantised(x):
     """The values that the 4-bit codes of x stand for."""
     d = x.double().reshape(*x.shape[:-1], x.shape[-1] // 32, 32)
     low = d.min(-1, keepdim=True).values
-    step = ((d.max(-1, keepdim=True).values - low) / 15).half().double()
+    wide = (d.max(-1, keepdim=True).values - low) / 15
+    step = wide.half()
+    step = torch.where(step.double() > wide, (step.view(torch.int16) - 1).view(torch.float16), step).double()
     n = torch.where(step > 0, torch.round((d - low) / step), torch.zeros_like(d))
     return (n.clamp(max=15) * step + low).reshape(x.shape)
 

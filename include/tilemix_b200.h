@@ -284,6 +284,99 @@ int tm_silu_mul(const void* gate, const void* up, void* out, int64_t n, void* st
  * squared-mean extension and the tail of PrefillRMSNorm (:718-771). */
 int tm_rms_norm(const void* x, const void* weight, void* out, int64_t rows, int cols, float eps, void* stream);
 
+/*
+ * Paged 4-bit key/value cache (no reference counterpart: its decode runs the
+ * model's own attention on a 16-bit cache).
+ *
+ * The pool is uint8 [num_pages, heads_k, page_size / 16 * 20 * head_dim],
+ * 16-byte aligned: every value costs 5 bits (4-bit codes, an fp16 scale s and an
+ * fp16 minimum m for each 32 channels of a token's head; value = s * code + m;
+ * byte order in csrc/kv4_layout.cuh). head_dim 64 or 128, page_size a multiple
+ * of 16. Slot = page * page_size + position in the page; a request's pages are
+ * the entries of its block-table row.
+ *
+ * What only the device can see is reported through error_flag (optional device
+ * int, first writer wins): 11 free pages, table columns, slots or max_kv_len
+ * exceeded, or a length negative; 12 a page number outside the pool (its keys are
+ * left out); 13 a slot outside the pool (skipped).
+ */
+
+/* Arguments of tm_build_block_tables. */
+typedef struct tm_block_tables_params {
+  const int32_t* cached_lens; /* [batch] tokens cached so far */
+  const int32_t* new_lens;    /* [batch] tokens to add */
+  int32_t* block_table;       /* [batch, cols]: new pages are entered in place */
+  int64_t table_stride;       /* elements from row to row */
+  int cols;
+  const int32_t* free_pages;  /* ring of page numbers, [capacity] */
+  int64_t capacity;
+  const int64_t* free_span;   /* [2]: free are the ring's entries [span[0], span[1]) modulo capacity */
+  int batch, page_size;
+  int64_t n_slots;            /* rows of the packed new tokens; those behind the last request get slot -1 */
+  int64_t* slots;             /* out [n_slots] */
+  int32_t* positions;         /* out [n_slots]: position in the request, 0 where there is no token */
+  int32_t* cu_seqlens;        /* out [batch + 1]: row offsets of the new tokens */
+  int32_t* kv_lens;           /* out [batch]: cached + new; not an input's buffer */
+  int64_t* free_span_out;     /* out [2]; not free_span's buffer */
+  int* error_flag;
+} tm_block_tables_params;
+
+/* Pages, slots, positions and offsets of the next tokens of a batch, from their
+ * lengths alone and on the device: pages are taken from the ring in request
+ * order. If pages, columns or slots do not suffice, or a length is negative,
+ * nothing is allocated: every slot is -1, kv_lens = cached_lens, cu_seqlens 0,
+ * free_span_out = free_span, and the error word is set. batch <= 8192. */
+int tm_build_block_tables(const tm_block_tables_params* params, void* stream);
+
+/* Return the pages of finished requests (done[b] != 0) to the ring's end, in
+ * request order: lens[b] becomes 0, its table entries -1, free_span[1] grows. */
+int tm_release_pages(int32_t* lens, const uint8_t* done, int32_t* block_table, int64_t table_stride, int cols,
+                     int32_t* free_pages, int64_t capacity, int64_t* free_span, int batch, int page_size,
+                     int* error_flag, void* stream);
+
+/* Quantise fp16 k / v [n_tokens, heads, head_dim] (element strides, head_dim
+ * contiguous, 16-byte rows) and store token i at slots[i] (int64; -1: skipped).
+ * A slot may appear once in a call. */
+int tm_kv4_append(const void* k, int64_t k_stride_tok, int64_t k_stride_head, const void* v, int64_t v_stride_tok,
+                  int64_t v_stride_head, int64_t n_tokens, const int64_t* slots, void* pool, int64_t num_pages,
+                  int heads, int head_dim, int page_size, int* error_flag, void* stream);
+
+/* Read slots back as fp16 k / v [n_tokens, heads, head_dim] (contiguous); slot -1 gives zeros. */
+int tm_kv4_read(const void* pool, int64_t num_pages, int heads, int head_dim, int page_size, const int64_t* slots,
+                int64_t n_tokens, void* k, void* v, int* error_flag, void* stream);
+
+/* Arguments of tm_kv4_attn. */
+typedef struct tm_kv4_attn_params {
+  const void* q; /* fp16 [q_tokens, heads_q, head_dim] */
+  int64_t q_stride_tok, q_stride_head;
+  void* out; /* fp16, shape of q; rows behind the last request are left as they are */
+  int64_t o_stride_tok, o_stride_head;
+  int64_t q_tokens;
+  const void* pool;
+  int64_t num_pages;
+  const int32_t* block_table; /* [batch, cols] */
+  int64_t table_stride;
+  int cols;
+  int page_size;
+  const int32_t* kv_lens;      /* [batch] keys in the cache, the new tokens' among them */
+  const int32_t* cu_seqlens_q; /* [batch + 1], or NULL: one query token a request */
+  const uint8_t* key_mask;     /* optional [batch, mask_cols]: 0 excludes a key, as does a column past the end */
+  int64_t mask_stride;
+  int mask_cols;
+  int batch, heads_q, heads_k, head_dim;
+  int max_seqlen_q, max_kv_len; /* host bounds of the query and cache lengths */
+  int causal; /* query i of n sees the keys before position kv_len - n + i + 1; else all keys */
+  float sm_scale;
+  int* error_flag;
+} tm_kv4_attn_params;
+
+/* Attention of a few query tokens a request over its cached keys. A row without
+ * a key gives 0. The split of the key axis (from the host bounds alone) needs
+ * `workspace` (16-byte aligned, tm_kv4_attn_workspace bytes, contents free); calls
+ * that may overlap need one each. */
+int tm_kv4_attn_workspace(const tm_kv4_attn_params* params, int64_t* bytes);
+int tm_kv4_attn(const tm_kv4_attn_params* params, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Human-readable text for a TM_* status code. */
 const char* tm_status_string(int status);
 

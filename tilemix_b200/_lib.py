@@ -5,6 +5,7 @@ be loaded, :func:`lib` raises. Build it with ``python -m tilemix_b200.build``.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -89,6 +90,33 @@ class TmMapParams(ctypes.Structure):
     ]
 
 
+class TmBlockTablesParams(ctypes.Structure):
+    """Mirror of ``tm_block_tables_params`` (include/tilemix_b200.h)."""
+
+    _fields_ = [
+        ("cached_lens", c_void_p), ("new_lens", c_void_p), ("block_table", c_void_p), ("table_stride", c_i64),
+        ("cols", c_int), ("free_pages", c_void_p), ("capacity", c_i64), ("free_span", c_void_p),
+        ("batch", c_int), ("page_size", c_int), ("n_slots", c_i64), ("slots", c_void_p), ("positions", c_void_p),
+        ("cu_seqlens", c_void_p), ("kv_lens", c_void_p), ("free_span_out", c_void_p), ("error_flag", c_void_p),
+    ]
+
+
+class TmKv4AttnParams(ctypes.Structure):
+    """Mirror of ``tm_kv4_attn_params`` (include/tilemix_b200.h)."""
+
+    _fields_ = [
+        ("q", c_void_p), ("q_stride_tok", c_i64), ("q_stride_head", c_i64),
+        ("out", c_void_p), ("o_stride_tok", c_i64), ("o_stride_head", c_i64), ("q_tokens", c_i64),
+        ("pool", c_void_p), ("num_pages", c_i64),
+        ("block_table", c_void_p), ("table_stride", c_i64), ("cols", c_int), ("page_size", c_int),
+        ("kv_lens", c_void_p), ("cu_seqlens_q", c_void_p),
+        ("key_mask", c_void_p), ("mask_stride", c_i64), ("mask_cols", c_int),
+        ("batch", c_int), ("heads_q", c_int), ("heads_k", c_int), ("head_dim", c_int),
+        ("max_seqlen_q", c_int), ("max_kv_len", c_int), ("causal", c_int),
+        ("sm_scale", ctypes.c_float), ("error_flag", c_void_p),
+    ]
+
+
 # (name, restype, argtypes) of every exported entry point.
 SIGNATURES = {
     "tm_quant_per_block_int8": (c_int, [c_void_p, c_i64, c_i64, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
@@ -110,10 +138,20 @@ SIGNATURES = {
                                       c_int, c_void_p]),
     "tm_silu_mul": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_void_p]),
     "tm_rms_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_int, ctypes.c_float, c_void_p]),
+    "tm_build_block_tables": (c_int, [ctypes.POINTER(TmBlockTablesParams), c_void_p]),
+    "tm_release_pages": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_int, c_void_p, c_i64, c_void_p, c_int, c_int,
+                                 c_void_p, c_void_p]),
+    "tm_kv4_append": (c_int, [c_void_p, c_i64, c_i64, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_void_p, c_i64,
+                              c_int, c_int, c_int, c_void_p, c_void_p]),
+    "tm_kv4_read": (c_int, [c_void_p, c_i64, c_int, c_int, c_int, c_void_p, c_i64, c_void_p, c_void_p, c_void_p,
+                            c_void_p]),
+    "tm_kv4_attn_workspace": (c_int, [ctypes.POINTER(TmKv4AttnParams), ctypes.POINTER(c_i64)]),
+    "tm_kv4_attn": (c_int, [ctypes.POINTER(TmKv4AttnParams), c_void_p, c_i64, c_void_p]),
     "tm_status_string": (ctypes.c_char_p, [c_int]),
 }
 
 _LIB = None
+_NO_SWITCH = contextlib.nullcontext()
 
 
 def lib() -> ctypes.CDLL:
@@ -134,6 +172,14 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _LIB = handle
     return _LIB
+
+
+def on_device(device):
+    """Context in which a kernel of ``device`` (a CUDA ``torch.device`` with an index) is launched:
+    nothing to do when it is the current one, as it almost always is."""
+    import torch
+
+    return _NO_SWITCH if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def check(status: int, what: str) -> None:

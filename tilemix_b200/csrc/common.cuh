@@ -31,6 +31,9 @@ enum : int {
   kErrTimeoutDrain = 7,     // final drain of in-flight work timed out
   kErrTimeoutQFree = 9,     // Q producer waited too long for the previous work item's last S
   kErrTimeoutOFree = 10,    // MMA warp waited too long for the previous work item's O to be read
+  kErrCachePlan = 11,       // block tables: free pages, table columns or slots run out, or a length is negative
+  kErrCachePage = 12,       // a page number outside the pool where a key's page is looked up
+  kErrCacheSlot = 13,       // a slot outside the pool
 };
 
 constexpr unsigned long long kWaitTimeoutNs = 2000000000ull;  // 2 s

@@ -377,6 +377,27 @@ typedef struct tm_kv4_attn_params {
 int tm_kv4_attn_workspace(const tm_kv4_attn_params* params, int64_t* bytes);
 int tm_kv4_attn(const tm_kv4_attn_params* params, void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * Linear layer in 8-bit integers (no reference counterpart).
+ *
+ * tm_quant_per_token_int8 quantises the rows of x [rows, cols] (fp16 or bf16,
+ * columns contiguous): scale = amax / 127 (fp32), code = 127 x / amax rounded half
+ * away from zero; a row of zeros gets scale 0 and codes 0, a row with an infinity
+ * or a NaN that scale and codes 0.
+ * tm_int8_matmul: out[t, n] = (sum_k x8[t, k] w8[n, k]) x_scale[t] w_scale[n] +
+ * bias[n] in out_dtype, the bias (optional) too. Both operands have contiguous
+ * columns, 16-byte aligned rows (strides in elements, multiples of 16;
+ * in_features itself may be any number up to 131071); out_stride in elements.
+ */
+#define TM_DTYPE_FP16 0
+#define TM_DTYPE_BF16 1
+#define TM_DTYPE_FP32 2
+int tm_quant_per_token_int8(const void* x, int dtype, int64_t x_stride, int64_t rows, int cols, int8_t* out,
+                            int64_t out_stride, float* scale, void* stream);
+int tm_int8_matmul(const int8_t* x8, int64_t x_stride, const float* x_scale, const int8_t* w8, int64_t w_stride,
+                   const float* w_scale, const void* bias, void* out, int64_t out_stride, int out_dtype,
+                   int64_t tokens, int out_features, int in_features, int* error_flag, void* stream);
+
 /* Human-readable text for a TM_* status code. */
 const char* tm_status_string(int status);
 

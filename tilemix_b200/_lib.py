@@ -16,6 +16,7 @@ LIB_PATH = Path(os.environ.get("TILEMIX_B200_LIB", _PKG / "libtilemix_b200.so"))
 TM_OK = 0
 TM_ROUTE_MIXED, TM_ROUTE_FP16, TM_ROUTE_INT8 = 0, 1, 2
 TM_NUMERICS_GPU, TM_NUMERICS_EXACT = 0, 1
+TM_DTYPE_FP16, TM_DTYPE_BF16, TM_DTYPE_FP32 = 0, 1, 2
 
 
 def numerics_mode() -> str:
@@ -147,6 +148,9 @@ SIGNATURES = {
                             c_void_p]),
     "tm_kv4_attn_workspace": (c_int, [ctypes.POINTER(TmKv4AttnParams), ctypes.POINTER(c_i64)]),
     "tm_kv4_attn": (c_int, [ctypes.POINTER(TmKv4AttnParams), c_void_p, c_i64, c_void_p]),
+    "tm_quant_per_token_int8": (c_int, [c_void_p, c_int, c_i64, c_i64, c_int, c_void_p, c_i64, c_void_p, c_void_p]),
+    "tm_int8_matmul": (c_int, [c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_i64, c_int,
+                               c_i64, c_int, c_int, c_void_p, c_void_p]),
     "tm_status_string": (ctypes.c_char_p, [c_int]),
 }
 

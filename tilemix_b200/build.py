@@ -21,7 +21,8 @@ LIB_NAME = "libtilemix_b200.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 
 SOURCES = ["attn_api.cu", "attn_fwd_general.cu", "attn_fwd_paired.cu", "quant.cu", "precision_map.cu",
-           "attn_noalloc.cu", "prefill.cu", "cache_tables.cu", "kv4_cache.cu", "kv4_attn.cu"]
+           "attn_noalloc.cu", "prefill.cu", "cache_tables.cu", "kv4_cache.cu", "kv4_attn.cu",
+           "int8_linear.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

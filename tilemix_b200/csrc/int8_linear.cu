@@ -1,0 +1,613 @@
+// Linear layer in 8-bit integers: per-token quantiser and the integer matrix
+// product with a scale for each token and each output channel.
+//
+//   s_t = max_k |x_tk| / 127,  x8_tk = round_half_away(127 x_tk / max_k |x_tk|)
+//   y_tn = (sum_k x8_tk w8_nk) s_t w_n + b_n
+//
+// The sum is exact (int32: up to 133,000 terms of 127 * 127), so its order, the
+// split of K and the tile do not change the result; scales and bias are applied
+// in fp32 and y is rounded once.
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math_constants.h>
+
+#include "common.cuh"
+#include "kv4_layout.cuh"
+#include "tilemix_b200.h"
+
+namespace tilemix {
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn();  // attn_api.cu
+
+namespace linear {
+
+using kv4::aligned;
+
+// ----------------------------------------------------------------------------
+// Quantiser
+// ----------------------------------------------------------------------------
+constexpr int kQuantThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w));
+}
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+struct RowScale {
+  float k, amax, r;  // codes are round(k x / amax), r = 1 / amax (correctly rounded)
+  bool ok;
+};
+
+// k x = 127 x (times a power of two) is exact in fp32 (x has at most 11 significant bits), and the quotient is formed from the correctly
+// rounded reciprocal with one residual correction (Markstein), so a quotient half way between two codes is
+// exact and the others are too far from one (2^-19 relative) for their rounding to matter: the code is
+// that of exact arithmetic. |x| <= amax, so |q| <= 127.
+__device__ __forceinline__ uint32_t code_of(float x, const RowScale& s) {
+  const float y = x * s.k;
+  const float q0 = __fmul_rn(y, s.r);
+  const float q = __fmaf_rn(__fmaf_rn(-q0, s.amax, y), s.r, q0);
+  return static_cast<uint32_t>(__float2int_rz(q + copysignf(0.5f, q))) & 0xffu;
+}
+
+__device__ __forceinline__ RowScale row_scale(float amax) {
+  // bf16 rows reach from 1e-40 to 3e38: a power of two on both sides of the quotient keeps the product, the
+  // reciprocal and the residual normal.
+  const float p = amax < 5.421010862e-20f ? 1.844674407e19f : amax > 1.844674407e19f ? 5.421010862e-20f : 1.f;  // 2^+-64
+  RowScale s;
+  s.k = 127.f * p;
+  s.amax = amax * p;
+  s.ok = amax > 0.f && amax <= 3.4028235e38f;
+  s.r = s.ok ? __frcp_rn(s.amax) : 0.f;
+  return s;
+}
+
+template <typename T>
+__device__ __forceinline__ uint2 codes8(const uint4& v, const RowScale& s) {
+  const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+  uint32_t c[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2<T>(in[i]);
+    c[2 * i] = code_of(f.x, s);
+    c[2 * i + 1] = code_of(f.y, s);
+  }
+  return make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+}
+
+__device__ __forceinline__ float block_max(float m) {
+  __shared__ float red[kQuantThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = red[0];
+#pragma unroll
+  for (int i = 1; i < kQuantThreads / 32; ++i) m = max_nan(m, red[i]);
+  return m;
+}
+
+// One CTA a row, the row held in registers between the two uses (kVec 16-byte pieces a thread; 0: any length,
+// read twice). A row with an infinity or a NaN gets that scale and codes 0, so that its outputs are NaN.
+template <typename T, int kVec>
+__global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const T* x, int64_t x_stride, int cols, int8_t* out,
+                                                                  int64_t out_stride, float* scale) {
+  const T* row = x + blockIdx.x * x_stride;
+  int8_t* dst = out + blockIdx.x * out_stride;
+  float m = 0.f;
+  if constexpr (kVec > 0) {
+    uint4 v[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int c = (i * kQuantThreads + threadIdx.x) * 8;
+      v[i] = c < cols ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack2<T>(w[e]);
+        m = max_nan(m, max_nan(fabsf(f.x), fabsf(f.y)));
+      }
+    }
+    m = block_max(m);
+    const RowScale s = row_scale(m);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int c = (i * kQuantThreads + threadIdx.x) * 8;
+      if (c < cols) *reinterpret_cast<uint2*>(dst + c) = s.ok ? codes8<T>(v[i], s) : make_uint2(0, 0);
+    }
+  } else {
+    for (int c = threadIdx.x; c < cols; c += kQuantThreads) m = max_nan(m, fabsf(to_float(row[c])));
+    m = block_max(m);
+    const RowScale s = row_scale(m);
+    for (int c = threadIdx.x; c < cols; c += kQuantThreads)
+      dst[c] = s.ok ? static_cast<int8_t>(code_of(to_float(row[c]), s)) : int8_t(0);
+  }
+  if (threadIdx.x == 0) scale[blockIdx.x] = __fdiv_rn(m, 127.f);
+}
+
+template <typename T>
+static void launch_quant(const void* x, int64_t xs, int64_t rows, int cols, int8_t* out, int64_t os, float* scale,
+                         cudaStream_t st) {
+  const T* p = static_cast<const T*>(x);
+  const unsigned g = static_cast<unsigned>(rows);
+  const int pieces = (cols + kQuantThreads * 8 - 1) / (kQuantThreads * 8);
+  const bool vec = cols % 8 == 0 && aligned(x, 16) && xs % 8 == 0 && aligned(out, 8) && os % 8 == 0;
+  if (!vec || pieces > 8)
+    quant_rows_kernel<T, 0><<<g, kQuantThreads, 0, st>>>(p, xs, cols, out, os, scale);
+  else if (pieces <= 1)
+    quant_rows_kernel<T, 1><<<g, kQuantThreads, 0, st>>>(p, xs, cols, out, os, scale);
+  else if (pieces <= 2)
+    quant_rows_kernel<T, 2><<<g, kQuantThreads, 0, st>>>(p, xs, cols, out, os, scale);
+  else if (pieces <= 4)
+    quant_rows_kernel<T, 4><<<g, kQuantThreads, 0, st>>>(p, xs, cols, out, os, scale);
+  else
+    quant_rows_kernel<T, 8><<<g, kQuantThreads, 0, st>>>(p, xs, cols, out, os, scale);
+}
+
+// ----------------------------------------------------------------------------
+// Matrix product
+// ----------------------------------------------------------------------------
+// D[128 x BN] = A[128 x K] B[BN x K]^T on tcgen05 kind::i8, both operands K-major in 128-byte swizzled tiles
+// that TMA brings (it fills rows and columns past the ends with zeros), int32 accumulators in TMEM, two of
+// them, so that one tile's epilogue runs under the next tile's products. With many tokens they are the A side
+// (a lane of TMEM is a token); with few, the weights are, and the tokens are the N side, as narrow as they
+// are (a lane is a channel): the tensor core then never works on padding rows and the weights stream through.
+// A split of K is a cluster of CTAs, one part each, whose int32 partial tiles are added through distributed
+// shared memory: exact, so without an effect on the result, and without a workspace.
+constexpr int kBM = 128, kBK = 128;
+constexpr int kGemmThreads = 256;
+constexpr int kMaxSplit = 8;
+constexpr int kSms = 148;
+
+struct GemmArgs {
+  int rows_a, rows_b;
+  int k_tiles, split;
+  int tiles_a, tiles_b;
+  const float* scale_a;  // of the lanes' rows
+  const float* scale_b;  // of the columns' rows
+  const void* bias;      // optional, of the channels, in the output's type
+  void* out;             // [tokens, channels], row stride ldo
+  int64_t ldo;
+  int vec;  // rows of `out` take 16-byte stores
+  int* err;
+};
+
+__device__ __forceinline__ void tma_load_2d_e(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ int32_t ld_cluster(uint32_t saddr, uint32_t rank) {
+  int32_t v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %1, %2;\n\t"
+      "ld.shared::cluster.b32 %0, [a];\n\t}"
+      : "=r"(v)
+      : "r"(saddr), "r"(rank)
+      : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void store_one(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store_one(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
+__device__ __forceinline__ float load_one(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float load_one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float load_one(const float* p) { return *p; }
+__device__ __forceinline__ uint32_t pack2(const __half*, float a, float b) { return pack_half2_rn(a, b); }
+__device__ __forceinline__ uint32_t pack2(const __nv_bfloat16*, float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int BN>
+struct GemmShape {
+  static constexpr int kStageBytes = (kBM + BN) * kBK;
+  // Wide tiles: as many stages as fit. Narrow ones: two CTAs an SM, so that a split's CTAs are all resident.
+  static constexpr int kStages = BN >= 256 ? 4 : BN >= 128 ? 6 : BN >= 64 ? 4 : 5;
+  static constexpr int kSmem = kStages * kStageBytes + 1024;
+  static constexpr int kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
+};
+
+// Scales, bias and store of kCols consecutive columns of this lane's row.
+template <int kCols, bool kTokenLanes, typename OutT>
+__device__ __forceinline__ void emit(const uint32_t* acc, const GemmArgs& g, int a, int b0) {
+  if (a >= g.rows_a) return;
+  OutT* out = static_cast<OutT*>(g.out);
+  const OutT* bias = static_cast<const OutT*>(g.bias);
+  const float sa = __ldg(g.scale_a + a);
+  if constexpr (kTokenLanes) {
+    OutT* row = out + a * g.ldo;
+    float v[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const int b = min(b0 + c, g.rows_b - 1);
+      v[c] = static_cast<float>(static_cast<int32_t>(acc[c])) * sa * __ldg(g.scale_b + b);
+      if (bias != nullptr) v[c] += load_one(bias + b);
+    }
+    if constexpr (sizeof(OutT) == 2) {
+      if (g.vec && b0 + kCols <= g.rows_b) {
+#pragma unroll
+        for (int c = 0; c + 8 <= kCols; c += 8)
+          *reinterpret_cast<uint4*>(row + b0 + c) =
+              make_uint4(pack2(out, v[c], v[c + 1]), pack2(out, v[c + 2], v[c + 3]), pack2(out, v[c + 4], v[c + 5]),
+                         pack2(out, v[c + 6], v[c + 7]));
+        if constexpr (kCols % 8 != 0) {
+#pragma unroll
+          for (int c = kCols / 8 * 8; c < kCols; ++c) store_one(row + b0 + c, v[c]);
+        }
+        return;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+      if (b0 + c < g.rows_b) store_one(row + b0 + c, v[c]);
+  } else {
+    const float bv = bias != nullptr ? load_one(bias + a) : 0.f;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const int b = b0 + c;
+      if (b < g.rows_b) {
+        // the token's scale first, as with the tokens on the lanes
+        float v = static_cast<float>(static_cast<int32_t>(acc[c])) * __ldg(g.scale_b + b) * sa;
+        if (bias != nullptr) v += bv;
+        store_one(out + b * g.ldo + a, v);
+      }
+    }
+  }
+}
+
+template <int BN, bool kTokenLanes, typename OutT>
+__global__ void __launch_bounds__(kGemmThreads) gemm_kernel(const __grid_constant__ CUtensorMap map_a,
+                                                           const __grid_constant__ CUtensorMap map_b,
+                                                           const GemmArgs g) {
+  using S = GemmShape<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_base;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = g.split > 1 ? blockIdx.x % g.split : 0;
+  const int first_tile = g.split > 1 ? blockIdx.x / g.split : blockIdx.x;
+  const int tile_step = g.split > 1 ? g.tiles_a * g.tiles_b : gridDim.x;
+  const int tiles = g.tiles_a * g.tiles_b;
+  const int k0 = static_cast<int>(static_cast<int64_t>(g.k_tiles) * rank / g.split);
+  const int k1 = static_cast<int>(static_cast<int64_t>(g.k_tiles) * (rank + 1) / g.split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 4);
+    }
+    fence_mbarrier_init();
+    prefetch_tmap(&map_a);
+    prefetch_tmap(&map_b);
+  }
+  if (warp == 2) {
+    tmem_alloc(&tmem_base, S::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+
+  // Tiles in groups of 16 A tiles, A fastest: a group's A tiles and the B tiles in work stay in L2.
+  auto tile_at = [&](int t, int* ta, int* tb) {
+    const int group = t / (16 * g.tiles_b), first = group * 16;
+    const int wide = min(16, g.tiles_a - first), r = t - group * 16 * g.tiles_b;
+    *ta = first + r % wide;
+    *tb = r / wide;
+  };
+
+  bool ok = true;
+  if (warp == 0) {
+    int s = 0, used = 0;
+    uint32_t phase = 0;
+    for (int t = first_tile; t < tiles && ok; t += tile_step) {
+      int ta, tb;
+      tile_at(t, &ta, &tb);
+      for (int k = k0; k < k1; ++k) {
+        if (!mbar_wait_spin(&empty[s], phase ^ 1, g.err, kErrTimeoutEmpty)) {
+          ok = false;
+          break;
+        }
+        uint8_t* st = smem + s * S::kStageBytes;
+        mbar_arrive_expect_tx_e(&full[s], S::kStageBytes);
+        tma_load_2d_e(st, &map_a, &full[s], k * kBK, ta * kBM);
+        tma_load_2d_e(st + kBM * kBK, &map_b, &full[s], k * kBK, tb * BN);
+        ++used;
+        if (++s == S::kStages) s = 0, phase ^= 1;
+      }
+    }
+    if (!ok) {  // the copies in flight land before the shared memory is given up
+      for (int i = 0; i < S::kStages && used > i; ++i) {
+        const int last = (used - 1 - i) / S::kStages;
+        mbar_wait(&full[i], last & 1, g.err, kErrTimeoutDrain);
+      }
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = make_idesc(2, 1, 0, 0, kBM, BN);
+    int s = 0, n = 0;
+    uint32_t phase = 0;
+    for (int t = first_tile; t < tiles && ok; t += tile_step, ++n) {
+      const int acc = n & 1;
+      if (!mbar_wait_spin(&acc_empty[acc], ((n >> 1) & 1) ^ 1, g.err, kErrTimeoutOFree)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d = tmem + acc * BN;
+      for (int k = k0; k < k1; ++k) {
+        if (!mbar_wait_spin(&full[s], phase, g.err, kErrTimeoutFull)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t st = smem_u32(smem + s * S::kStageBytes);
+        const uint64_t da = make_sdesc(st, 16, 1024, 2), db = make_sdesc(st + kBM * kBK, 16, 1024, 2);
+#pragma unroll
+        for (int i = 0; i < kBK / 32; ++i)
+          mma_i8_ss_e(d, da + 2 * i, db + 2 * i, idesc, (k > k0 || i > 0) ? 1u : 0u);
+        tc_commit_e(&empty[s]);
+        if (++s == S::kStages) s = 0, phase ^= 1;
+      }
+      if (ok) tc_commit_e(&acc_full[acc]);
+    }
+    if (!ok) {  // products in flight end before TMEM is given up: a barrier of this warp's own
+      __shared__ __align__(8) uint64_t drain;
+      if (lane == 0) {
+        mbar_init(&drain, 1);
+        fence_mbarrier_init();
+      }
+      __syncwarp();
+      tc_commit_e(&drain);
+      mbar_wait(&drain, 0, g.err, kErrTimeoutDrain);
+    }
+  } else if (warp >= 4) {
+    const int quad = warp & 3;
+    int n = 0;
+    for (int t = first_tile; t < tiles; t += tile_step, ++n) {
+      const int acc = n & 1;
+      if (!mbar_wait_spin(&acc_full[acc], (n >> 1) & 1, g.err, kErrTimeoutScores)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d = tmem + acc * BN + (static_cast<uint32_t>(quad * 32) << 16);
+      int ta, tb;
+      tile_at(t, &ta, &tb);
+      const int a = ta * kBM + quad * 32 + lane;
+      if (g.split == 1) {
+        if constexpr (BN >= 32) {
+#pragma unroll 1
+          for (int c = 0; c < BN; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(d + c, r);
+            tmem_wait_ld();
+            emit<32, kTokenLanes, OutT>(r, g, a, tb * BN + c);
+          }
+        } else {
+          uint32_t r[16];
+          tmem_ld16(d, r);
+          tmem_wait_ld();
+          emit<16, kTokenLanes, OutT>(r, g, a, tb * BN);
+        }
+      } else {
+        // this part's partial tile, column by column (a warp's 32 lanes are 128 consecutive bytes); every
+        // copy has landed and every product has read its stage, so the ring is free
+        int32_t* red = reinterpret_cast<int32_t*>(smem) + quad * 32 + lane;
+#pragma unroll 1
+        for (int c = 0; c < BN; c += 16) {
+          uint32_t r[16];
+          tmem_ld16(d + c, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) red[(c + i) * kBM] = static_cast<int32_t>(r[i]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[acc]);
+    }
+  }
+
+  if (g.split > 1) {  // a cluster has one tile; the barriers are reached whatever happened above
+    __syncwarp();
+    cluster_sync();
+    if (warp >= 4 && ok) {
+      int ta, tb;
+      tile_at(first_tile, &ta, &tb);
+      const int quad = warp & 3, cols = BN / g.split;
+      const int a = ta * kBM + quad * 32 + lane;
+      const uint32_t base = smem_u32(smem) + (quad * 32 + lane) * 4;
+      for (int c = rank * cols; c < (rank + 1) * cols; c += 2) {
+        int32_t sum[2] = {0, 0};
+        for (int p = 0; p < g.split; ++p) {
+          sum[0] += ld_cluster(base + c * (kBM * 4), p);
+          sum[1] += ld_cluster(base + (c + 1) * (kBM * 4), p);
+        }
+        const uint32_t u[2] = {static_cast<uint32_t>(sum[0]), static_cast<uint32_t>(sum[1])};
+        emit<2, kTokenLanes, OutT>(u, g, a, tb * BN + c);
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // nobody leaves while its partial tile is read
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) tmem_dealloc(tmem, S::kTmemCols);
+}
+
+struct Plan {
+  bool token_lanes;
+  int bn, split;
+};
+
+// Which side is the lanes', how wide a tile is and into how many parts K is cut, by sizes alone.
+static Plan plan_of(int64_t m, int n, int k_tiles) {
+  Plan p{};
+  p.token_lanes = m > 128;
+  if (!p.token_lanes)
+    p.bn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+  else
+    p.bn = 256;
+  auto tiles = [&]() {
+    const int64_t a = p.token_lanes ? m : n, b = p.token_lanes ? n : m;
+    return ((a + kBM - 1) / kBM) * ((b + p.bn - 1) / p.bn);
+  };
+  if (p.token_lanes)
+    while (p.bn > 64 && tiles() < kSms / 2) p.bn /= 2;
+  p.split = 1;
+  if (p.bn <= 128)
+    while (p.split < kMaxSplit && tiles() * p.split * 2 <= 2 * kSms && k_tiles / (p.split * 2) >= 4) p.split *= 2;
+  return p;
+}
+
+static int make_map(CUtensorMap* m, const void* base, int64_t rows, int k, int64_t stride, int box_rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return TM_ERR_LAUNCH;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(kBK), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1u, 1u};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TM_OK : TM_ERR_TMAP;
+}
+
+template <int BN, bool kTokenLanes, typename OutT>
+static int launch(const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& g, cudaStream_t st) {
+  using S = GemmShape<BN>;
+  auto kernel = gemm_kernel<BN, kTokenLanes, OutT>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess)
+    return TM_ERR_LAUNCH;
+  const int64_t tiles = static_cast<int64_t>(g.tiles_a) * g.tiles_b;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(g.split > 1 ? tiles * g.split : tiles < kSms ? tiles : kSms));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = static_cast<unsigned>(g.split);
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = g.split > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, a, b, g) == cudaSuccess ? TM_OK : TM_ERR_LAUNCH;
+}
+
+template <typename OutT>
+static int dispatch(const Plan& p, const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& g, cudaStream_t st) {
+  if (p.token_lanes) {
+    if (p.bn == 256) return launch<256, true, OutT>(a, b, g, st);
+    if (p.bn == 128) return launch<128, true, OutT>(a, b, g, st);
+    return launch<64, true, OutT>(a, b, g, st);
+  }
+  if (p.bn == 128) return launch<128, false, OutT>(a, b, g, st);
+  if (p.bn == 64) return launch<64, false, OutT>(a, b, g, st);
+  if (p.bn == 32) return launch<32, false, OutT>(a, b, g, st);
+  return launch<16, false, OutT>(a, b, g, st);
+}
+
+}  // namespace linear
+}  // namespace tilemix
+
+extern "C" int tm_quant_per_token_int8(const void* x, int dtype, int64_t x_stride, int64_t rows, int cols, int8_t* out,
+                                       int64_t out_stride, float* scale, void* stream) {
+  using namespace tilemix::linear;
+  if (rows < 0 || cols <= 0) return TM_ERR_SHAPE;
+  if (dtype != TM_DTYPE_FP16 && dtype != TM_DTYPE_BF16) return TM_ERR_UNSUPPORTED;
+  if (rows > 0x7fffffffll) return TM_ERR_SHAPE;
+  if (rows == 0) return TM_OK;
+  if (!x || !out || !scale) return TM_ERR_NULL;
+  if (!aligned(x, 2) || !aligned(scale, 4)) return TM_ERR_ALIGN;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == TM_DTYPE_FP16)
+    launch_quant<__half>(x, x_stride, rows, cols, out, out_stride, scale, st);
+  else
+    launch_quant<__nv_bfloat16>(x, x_stride, rows, cols, out, out_stride, scale, st);
+  return cudaGetLastError() == cudaSuccess ? TM_OK : TM_ERR_LAUNCH;
+}
+
+extern "C" int tm_int8_matmul(const int8_t* x8, int64_t x_stride, const float* x_scale, const int8_t* w8,
+                              int64_t w_stride, const float* w_scale, const void* bias, void* out, int64_t out_stride,
+                              int out_dtype, int64_t tokens, int out_features, int in_features, int* error_flag,
+                              void* stream) {
+  using namespace tilemix::linear;
+  if (tokens < 0 || out_features <= 0 || in_features <= 0) return TM_ERR_SHAPE;
+  if (out_dtype < TM_DTYPE_FP16 || out_dtype > TM_DTYPE_FP32) return TM_ERR_UNSUPPORTED;
+  // int32 sums of in_features products of at most 127 * 127 (128 * 128, should a caller bring -128)
+  if (in_features > 131071 || tokens > 0x7fffff00ll || out_features > 0x7fffff00) return TM_ERR_UNSUPPORTED;
+  if (tokens == 0) return TM_OK;
+  if (!x8 || !x_scale || !w8 || !w_scale || !out) return TM_ERR_NULL;
+  const int es = out_dtype == TM_DTYPE_FP32 ? 4 : 2;
+  if (!aligned(x8, 16) || !aligned(w8, 16) || x_stride % 16 || w_stride % 16) return TM_ERR_ALIGN;
+  if (!aligned(out, es) || !aligned(x_scale, 4) || !aligned(w_scale, 4) || (bias && !aligned(bias, es)))
+    return TM_ERR_ALIGN;
+  if (x_stride < 0 || w_stride < 0 || (tokens > 1 && x_stride < in_features) ||
+      (out_features > 1 && w_stride < in_features))
+    return TM_ERR_SHAPE;
+  const int64_t round_k = (static_cast<int64_t>(in_features) + 15) / 16 * 16;
+  if (tokens == 1 && x_stride < round_k) x_stride = round_k;  // one row: its stride is never used
+  if (out_features == 1 && w_stride < round_k) w_stride = round_k;
+  const int k_tiles = (in_features + kBK - 1) / kBK;
+  const Plan p = plan_of(tokens, out_features, k_tiles);
+  GemmArgs g{};
+  g.rows_a = static_cast<int>(p.token_lanes ? tokens : out_features);
+  g.rows_b = static_cast<int>(p.token_lanes ? out_features : tokens);
+  g.k_tiles = k_tiles;
+  g.split = p.split;
+  g.tiles_a = (g.rows_a + kBM - 1) / kBM;
+  g.tiles_b = (g.rows_b + p.bn - 1) / p.bn;
+  if (static_cast<int64_t>(g.tiles_a) * g.tiles_b * p.split > 0x7fffffffll - 1024) return TM_ERR_UNSUPPORTED;
+  g.scale_a = p.token_lanes ? x_scale : w_scale;
+  g.scale_b = p.token_lanes ? w_scale : x_scale;
+  g.bias = bias;
+  g.out = out;
+  g.ldo = out_stride;
+  g.vec = es == 2 && aligned(out, 16) && out_stride % 8 == 0;
+  g.err = error_flag;
+  CUtensorMap mx, mw;
+  int rc = make_map(&mx, x8, tokens, in_features, x_stride, p.token_lanes ? kBM : p.bn);
+  if (rc != TM_OK) return rc;
+  rc = make_map(&mw, w8, out_features, in_features, w_stride, p.token_lanes ? p.bn : kBM);
+  if (rc != TM_OK) return rc;
+  const CUtensorMap& ma = p.token_lanes ? mx : mw;
+  const CUtensorMap& mb = p.token_lanes ? mw : mx;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (out_dtype == TM_DTYPE_FP16) return dispatch<__half>(p, ma, mb, g, st);
+  if (out_dtype == TM_DTYPE_BF16) return dispatch<__nv_bfloat16>(p, ma, mb, g, st);
+  return dispatch<float>(p, ma, mb, g, st);
+}

@@ -366,14 +366,15 @@ typedef struct tm_kv4_attn_params {
   int batch, heads_q, heads_k, head_dim;
   int max_seqlen_q, max_kv_len; /* host bounds of the query and cache lengths */
   int causal; /* query i of n sees the keys before position kv_len - n + i + 1; else all keys */
-  float sm_scale;
+  float sm_scale; /* > 0 */
   int* error_flag;
 } tm_kv4_attn_params;
 
 /* Attention of a few query tokens a request over its cached keys. A row without
- * a key gives 0. The split of the key axis (from the host bounds alone) needs
- * `workspace` (16-byte aligned, tm_kv4_attn_workspace bytes, contents free); calls
- * that may overlap need one each. */
+ * a key gives 0. The work is split over the keys on the device, from the lengths;
+ * the parts' states go through `workspace` (16-byte aligned, tm_kv4_attn_workspace
+ * bytes, contents free); calls that may overlap need one each. Keys beyond
+ * max_kv_len are left out and reported. */
 int tm_kv4_attn_workspace(const tm_kv4_attn_params* params, int64_t* bytes);
 int tm_kv4_attn(const tm_kv4_attn_params* params, void* workspace, int64_t workspace_bytes, void* stream);
 

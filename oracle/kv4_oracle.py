@@ -112,9 +112,12 @@ def attention(q, keys, values, kv_len, sm_scale, causal, key_mask=None):
     """64-bit attention of one request's n query tokens [n, heads_q, dim] over keys / values [kv_len, heads_k, dim],
     and a bound on what fp16 operands may change.
 
-    Bound: rounding k to fp16 (2^-11 relative) moves a score by at most d = scale 2^-11 sum |q| |k|, so a weight by the
-    factor e^(2 d) (numerator and sum); v and p are rounded to fp16 (2^-11 each, a p under 2^-14 by at most 2^-25 of
-    the largest weight), the result once more; 2^-18 covers the fp32 sums and exponentials.
+    Bound: scores come from the codes, as sums of q (1024 + n) that start at -1024 sum q: products of two fp16 numbers
+    are exact, their fp32 sum is rounded (or cut) three times a group of 32 channels, at 2^-22 of at most 1039 sum |q|
+    each; times the group's scale s (its range / 15) that is under 2^-10 s sum |q|. The fp32 steps that follow add
+    2^-21 sum |q| |k|. With d the sum of both, times sm_scale, a weight changes by the factor e^(2 d) (numerator and
+    sum). v and p are rounded to fp16 (2^-11 each; a p under 2^-14 by at most 2^-25 of the largest weight), the result
+    once more; 2^-18 covers the fp32 sums and exponentials.
     """
     n, heads_q, dim = q.shape
     group = heads_q // keys.shape[1]
@@ -133,7 +136,10 @@ def attention(q, keys, values, kv_len, sm_scale, causal, key_mask=None):
             k, v = keys[seen, h // group], values[seen, h // group]
             s = k @ q[i, h] * sm_scale
             p = np.exp(s - s.max())
-            d = 2.0 ** -11 * sm_scale * (np.abs(k) @ np.abs(q[i, h])).max()
+            groups = k.reshape(len(k), -1, GROUP)
+            step = (groups.max(-1) - groups.min(-1)) / 15
+            d = sm_scale * (2.0 ** -10 * step @ np.abs(q[i, h]).reshape(-1, GROUP).sum(-1)
+                            + 2.0 ** -21 * np.abs(k) @ np.abs(q[i, h])).max()
             total = p.sum()
             out[i, h] = p @ v / total
             near = p @ np.abs(v) / total

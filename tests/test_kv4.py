@@ -112,7 +112,9 @@ ATTN = dict(q=lambda: _Fake((3, 4, 64)), pool=_pool, block_table=lambda: _i32(3,
     (dict(cu_seqlens_q=_i32(3)), ValueError, "batch \\+ 1"),
     (dict(key_mask=_i32(3, 9)), TypeError, "bool"),
     (dict(key_mask=_i32(2, 9, dtype=torch.bool)), ValueError, "row for each"),
-    (dict(out=_Fake((3, 4, 128))), ValueError, "match q"),
+    (dict(out=_Fake((3, 4, 128)), sm_scale=1.0), ValueError, "match q"),
+    (dict(out=_Fake((3, 4, 64)), sm_scale=0.0), ValueError, "sm_scale"),
+    (dict(out=_Fake((3, 4, 64)), sm_scale=float("nan")), ValueError, "sm_scale"),
 ])
 def test_attention_refusals(change, exc, text):
     from tilemix_b200.attention.kv4 import kv4_attention
@@ -196,7 +198,7 @@ def test_c_abi_refusals_need_no_gpu():
         p.q_stride_head = p.o_stride_head = 128
         p.q_tokens = p.batch = 4
         p.num_pages, p.table_stride, p.cols, p.page_size = 16, 4, 4, 32
-        p.heads_q, p.heads_k, p.head_dim, p.max_seqlen_q, p.max_kv_len, p.causal = 8, 2, 128, 1, 128, 1
+        p.heads_q, p.heads_k, p.head_dim, p.max_seqlen_q, p.max_kv_len, p.causal, p.sm_scale = 8, 2, 128, 1, 128, 1, 0.1
         for k, v in over.items():
             setattr(p, k, v)
         return lib().tm_kv4_attn_workspace(ctypes.byref(p), ctypes.byref(need)), p
@@ -206,10 +208,11 @@ def test_c_abi_refusals_need_no_gpu():
                          (-2, dict(page_size=24)), (-2, dict(page_size=0)), (-4, dict(head_dim=96)),
                          (-4, dict(batch=65536)), (-2, dict(max_seqlen_q=2)), (-3, dict(q=fake + 8)),
                          (-3, dict(q_stride_head=132)), (-3, dict(pool=fake + 8)), (-4, dict(max_kv_len=2**30 + 1)),
-                         (-2, dict(q_tokens=3))):
+                         (-2, dict(q_tokens=3)), (-2, dict(sm_scale=0.0)), (-2, dict(sm_scale=float("inf")))):
         assert attn(**over)[0] == status, over
     assert lib().tm_kv4_attn_workspace(None, ctypes.byref(need)) == -1
-    # a split key axis needs its workspace
+    assert attn(q_tokens=2**31, max_seqlen_q=65535, cu_seqlens_q=fake, max_kv_len=2**30, cols=2**25)[0] == -4
+    # the parts of a split key axis need their workspace
     rc, p = attn(batch=1, q_tokens=1, max_kv_len=1 << 20, cols=1 << 15)
     assert rc == 0 and need.value > 0
     assert lib().tm_kv4_attn(ctypes.byref(p), None, 0, None) == -1

@@ -258,6 +258,9 @@ def kv4_attention(q: Tensor, pool: Tensor, block_table: Tensor, kv_lens: Tensor,
         out = torch.empty((rows, heads, d), dtype=torch.float16, device=device)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or (rows and out.stride(2) != 1):
         raise ValueError("out must match q")
+    scale = d ** -0.5 if sm_scale is None else float(sm_scale)
+    if not 0 < scale < float("inf"):
+        raise ValueError("sm_scale must be positive and finite")
     capacity = cols * page_size
     bound = capacity if max_kv_len is None else min(int(max_kv_len), capacity)
     p = TmKv4AttnParams(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), rows,
@@ -267,7 +270,7 @@ def kv4_attention(q: Tensor, pool: Tensor, block_table: Tensor, kv_lens: Tensor,
                         0 if key_mask is None else key_mask.stride(0),
                         0 if key_mask is None else key_mask.shape[1],
                         batch, heads, heads_k, d, max_seqlen_q, bound, bool(causal),
-                        d ** -0.5 if sm_scale is None else sm_scale, _error_word(device).data_ptr())
+                        scale, _error_word(device).data_ptr())
     need = ctypes.c_int64()
     check(lib().tm_kv4_attn_workspace(ctypes.byref(p), ctypes.byref(need)), "tm_kv4_attn")
     # From the allocator on the call's own stream: two streams or graphs never share it.

@@ -27,6 +27,8 @@
 #include <cuda_fp16.h>
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kv4_layout.cuh"
 #include "tilemix_b200.h"
@@ -39,8 +41,11 @@ constexpr int kAttnThreads = 32 * kAttnWarps;
 constexpr int kStages = 3;
 constexpr int kStepBlocks = 2;                        // 16-key blocks a step
 constexpr int kStepKeys = kStepBlocks * kBlockTokens;
-constexpr int kChunkKeys = kStepKeys * kAttnWarps;    // keys of one step of every warp
+constexpr int kChunkKeys = kStepKeys * kAttnWarps;    // keys of one step of every warp: the unit of work
 constexpr int kSms = 148;
+
+// CTAs an SM of the kernel with NT row tiles, by registers and shared memory.
+constexpr int resident(int nt) { return nt == 1 ? 3 : 2; }
 
 struct AttnArgs {
   const __half* q;
@@ -61,16 +66,41 @@ struct AttnArgs {
   __half* out;
   int64_t o_st, o_sh;
   int64_t q_tokens;
-  int heads_q, heads_k, group, row_tiles;  // row_tiles: CTAs along the rows of a (request, KV head)
+  int batch, heads_q, heads_k, group;
   int max_q;
+  int64_t max_kv;  // most keys a request may have: its bound and its table row's
   int causal;
   float scale_log2;
-  int chunk;   // keys a split
-  int splits;  // splits of the longest request
-  float* part_o;   // [splits][q_tokens][heads_q][D]
-  float2* part_ml; // [splits][q_tokens][heads_q] (max in log2 units, sum)
+  int ctas;            // CTAs that share the work
+  long long* starts;   // [batch + 1] first chunk of each request, written by CTA 0 for the join
+  float* part_o;       // [2 ctas][rows of a tile][D]
+  float2* part_ml;     // [2 ctas][rows of a tile] (max in log2 units, sum)
   int* err;
 };
+
+// A request's share of the work.
+struct Request {
+  int q0, n_q;   // its query tokens
+  int kv;        // its keys
+  int tiles;     // row tiles a KV head
+  int chunks;    // chunks of kChunkKeys keys of one (KV head, row tile), at least 1
+};
+
+template <int NT>
+__device__ __forceinline__ Request request_of(const AttnArgs& a, int b) {
+  Request r;
+  r.q0 = b;
+  r.n_q = 1;
+  if (a.cu != nullptr) {
+    r.q0 = a.cu[b];
+    r.n_q = min(a.cu[b + 1] - r.q0, a.max_q);
+  }
+  if (r.q0 < 0 || r.n_q < 0 || r.q0 + static_cast<int64_t>(r.n_q) > a.q_tokens) r.n_q = 0;
+  r.kv = static_cast<int>(min(static_cast<int64_t>(max(a.kv_lens[b], 0)), a.max_kv));
+  r.tiles = (r.n_q * a.group + 8 * NT - 1) / (8 * NT);
+  r.chunks = max(1, (r.kv + kChunkKeys - 1) / kChunkKeys);
+  return r;
+}
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -81,15 +111,32 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// D = A B + C
+__device__ __forceinline__ void mma16816_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
+// D = A[16 x 8] B[8 x 8]
+__device__ __forceinline__ void mma1688(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm(
+      "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
+}
+
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
@@ -102,19 +149,24 @@ __device__ __forceinline__ uint32_t lop_and_or(uint32_t x, uint32_t m, uint32_t 
 __device__ __forceinline__ __half2 as_h2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-// Eight codes of a word as four fp16 pairs of values: pair i holds nibbles i and i + 4, value = s n + m.
+// Codes of a word in the mantissa of 1024: pair i holds nibbles i and i + 4, even pairs as 1024 + n, odd
+// ones as 1024 + 16 n.
+__device__ __forceinline__ void spread8(uint32_t w, uint32_t (&o)[4]) {
+  const uint32_t magic = 0x64006400u, w8 = w >> 8;
+  o[0] = lop_and_or(w, 0x000F000Fu, magic);
+  o[1] = lop_and_or(w, 0x00F000F0u, magic);
+  o[2] = lop_and_or(w8, 0x000F000Fu, magic);
+  o[3] = lop_and_or(w8, 0x00F000F0u, magic);
+}
+
+// The values s n + m of a word's codes as fp16 pairs (s, m of the pair's two halves).
 __device__ __forceinline__ void unpack8(uint32_t w, __half2 s, __half2 m, uint32_t (&o)[4]) {
-  const uint32_t magic = 0x64006400u;
   const __half2 k1024 = as_h2(0x64006400u), r16 = as_h2(0x2C002C00u), k64 = as_h2(0xD400D400u);  // 1024, 1/16, -64
-  const uint32_t w8 = w >> 8;
-  const __half2 n0 = __hsub2(as_h2(lop_and_or(w, 0x000F000Fu, magic)), k1024);
-  const __half2 n1 = __hfma2(as_h2(lop_and_or(w, 0x00F000F0u, magic)), r16, k64);
-  const __half2 n2 = __hsub2(as_h2(lop_and_or(w8, 0x000F000Fu, magic)), k1024);
-  const __half2 n3 = __hfma2(as_h2(lop_and_or(w8, 0x00F000F0u, magic)), r16, k64);
-  o[0] = as_u32(__hfma2(n0, s, m));
-  o[1] = as_u32(__hfma2(n1, s, m));
-  o[2] = as_u32(__hfma2(n2, s, m));
-  o[3] = as_u32(__hfma2(n3, s, m));
+  spread8(w, o);
+  o[0] = as_u32(__hfma2(__hsub2(as_h2(o[0]), k1024), s, m));
+  o[1] = as_u32(__hfma2(__hfma2(as_h2(o[1]), r16, k64), s, m));
+  o[2] = as_u32(__hfma2(__hsub2(as_h2(o[2]), k1024), s, m));
+  o[3] = as_u32(__hfma2(__hfma2(as_h2(o[3]), r16, k64), s, m));
 }
 
 template <int N>
@@ -137,38 +189,26 @@ __device__ __forceinline__ Words<N> load_words(const uint8_t* p) {
   return r;
 }
 
-// One CTA: one (request, KV head, tile of 8 NT rows, split of the keys).
+// The work of a call is the list of all chunks: by request, then KV head, then row tile, then key. CTA c takes
+// chunks [c per, (c + 1) per), whatever requests they belong to, so ragged lengths leave no CTA behind; a
+// (KV head, row tile) that several CTAs share leaves partial states for the join, one that a CTA has whole is
+// written at once. A CTA's first run of chunks may continue another's (slot 2 c), its last may be continued
+// (slot 2 c + 1).
 template <int D, int NT>
-__global__ void __launch_bounds__(kAttnThreads) attn_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, resident(NT)) attn_kernel(const AttnArgs a) {
   using L = Layout<D>;
   constexpr int G = L::kGroups;
   constexpr int kRows = 8 * NT;
   constexpr int kStageBytes = kStepBlocks * L::kBlockBytes;
-  constexpr int kRingBytes = kAttnWarps * kStages * kStageBytes;
-  static_assert(kAttnWarps * kRows * D * 4 <= kRingBytes, "the merge reuses the ring");
+  constexpr int kState = NT * (8 * G + 4);  // floats of a lane's state (o, m, l)
   extern __shared__ __align__(128) uint8_t smem[];
+  float* sh_state = reinterpret_cast<float*>(smem + kAttnWarps * kStages * kStageBytes);  // [2][kState][32]
   __shared__ __align__(8) uint64_t bars[kAttnWarps][kStages];
-  __shared__ float sh_m[kAttnWarps][kRows], sh_l[kAttnWarps][kRows];
-
-  const int b = blockIdx.y, split = blockIdx.z;
-  const int hk = blockIdx.x / a.row_tiles, row0 = (blockIdx.x % a.row_tiles) * kRows;
-  int q0 = b, n_q = 1;
-  if (a.cu != nullptr) {
-    q0 = a.cu[b];
-    n_q = min(a.cu[b + 1] - q0, a.max_q);
-  }
-  if (q0 < 0 || n_q <= 0 || q0 + static_cast<int64_t>(n_q) > a.q_tokens) return;
-  const int n_rows = n_q * a.group;
-  if (row0 >= n_rows) return;
-  const int64_t cap = static_cast<int64_t>(a.cols) * a.page_blocks * kBlockTokens;
-  const int kv = static_cast<int>(min(static_cast<int64_t>(max(a.kv_lens[b], 0)),
-                                      min(cap, static_cast<int64_t>(a.chunk) * a.splits)));
-  const int parts = max(1, (kv + a.chunk - 1) / a.chunk);
-  if (split >= parts) return;
-  if (kv < a.kv_lens[b] && threadIdx.x == 0) record_error(a.err, kErrCachePlan);  // longer than the table or max_kv_len
-  const int key0 = split * a.chunk, key1 = min(kv, key0 + a.chunk);  // this CTA's keys
+  __shared__ long long sh_part[kAttnWarps], sh_start;
+  __shared__ int sh_b;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up; it waits for our end
 
   uint8_t* ring = smem + warp * kStages * kStageBytes;
   uint64_t* bar = bars[warp];
@@ -176,397 +216,585 @@ __global__ void __launch_bounds__(kAttnThreads) attn_kernel(const AttnArgs a) {
     for (int s = 0; s < kStages; ++s) mbar_init(&bar[s], 1);
     fence_mbarrier_init();
   }
-  __syncwarp();
 
-  // The warp's steps: blocks key0 / 16 + 2 (warp + kAttnWarps i).
-  const int blk0 = key0 / kBlockTokens, blk1 = (key1 + kBlockTokens - 1) / kBlockTokens;
-  const int all_steps = (blk1 - blk0 + kStepBlocks - 1) / kStepBlocks;
-  const int steps = all_steps > warp ? (all_steps - warp + kAttnWarps - 1) / kAttnWarps : 0;
+  // Where this CTA's chunks begin: a scan over the requests, a run of them a thread.
+  const int run = (a.batch + kAttnThreads - 1) / kAttnThreads;
+  const int rb0 = min(tid * run, a.batch), rb1 = min(rb0 + run, a.batch);
+  long long mine = 0;
+  for (int b = rb0; b < rb1; ++b) {
+    const Request r = request_of<NT>(a, b);
+    mine += static_cast<long long>(r.tiles) * a.heads_k * r.chunks;
+    if (blockIdx.x == 0 && r.kv < a.kv_lens[b]) record_error(a.err, kErrCachePlan);  // longer than it may be
+  }
+  long long inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) sh_part[warp] = inc;
+  __syncthreads();
+  long long total = 0, before = inc - mine;
+#pragma unroll
+  for (int w = 0; w < kAttnWarps; ++w) {
+    if (w < warp) before += sh_part[w];
+    total += sh_part[w];
+  }
+  const long long per = (total + a.ctas - 1) / a.ctas;
+  long long pos = per * blockIdx.x;
+  const long long end = min(total, pos + per);
+  if (blockIdx.x == 0) {
+    long long at = before;
+    for (int b = rb0; b < rb1; ++b) {
+      a.starts[b] = at;
+      const Request r = request_of<NT>(a, b);
+      at += static_cast<long long>(r.tiles) * a.heads_k * r.chunks;
+    }
+    if (tid == 0) a.starts[a.batch] = total;
+  }
+  if (pos >= end) return;
+  if (before <= pos && pos < before + mine) {
+    long long at = before;
+    for (int b = rb0; b < rb1; ++b) {
+      const Request r = request_of<NT>(a, b);
+      const long long n = static_cast<long long>(r.tiles) * a.heads_k * r.chunks;
+      if (pos < at + n) {
+        sh_b = b;
+        sh_start = at;
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  int b = sh_b;
+  long long b_start = sh_start;
+  Request rq = request_of<NT>(a, b);
 
-  // Page numbers of 32 steps at a time, one step a lane.
-  const int32_t* row = a.table + b * a.table_stride;
-  const uint8_t* head_base = a.pool + static_cast<int64_t>(hk) * a.page_bytes;
-  int32_t pid[kStepBlocks];
-  int issued = 0;
-  uint32_t stage_bad = 0;  // bit (kStepBlocks stage + block): the block's page is outside the pool
+  // The current run of chunks: one (request, KV head, row tile), keys [key0, key1).
+  int hk, row0, chunk0, n_chunks, key0, blk1, steps;
+  auto locate = [&]() {
+    const int off = static_cast<int>(pos - b_start);
+    const int unit = off / rq.chunks;
+    chunk0 = off - unit * rq.chunks;
+    n_chunks = static_cast<int>(min(static_cast<long long>(rq.chunks - chunk0), end - pos));
+    hk = unit / rq.tiles;
+    row0 = (unit - hk * rq.tiles) * kRows;
+    key0 = chunk0 * kChunkKeys;
+    const int key1 = min(rq.kv, key0 + n_chunks * kChunkKeys);
+    blk1 = (key1 + kBlockTokens - 1) / kBlockTokens;
+    const int all_steps = (blk1 - key0 / kBlockTokens + kStepBlocks - 1) / kStepBlocks;
+    steps = all_steps > warp ? (all_steps - warp + kAttnWarps - 1) / kAttnWarps : 0;
+  };
+  locate();
+
+  // Bulk copies of the warp's steps: blocks key0 / 16 + 2 (warp + kAttnWarps i). Each lane looks up one step of
+  // the next 32 (its pages, the addresses of its blocks) and issues that step's copies itself when its turn
+  // comes, so a step costs a few instructions. Steps of all runs count on through the ring's stages.
+  const uint8_t* src[kStepBlocks];  // the lane's step; NULL: past the run's end, or its page is outside the pool
+  uint32_t absent[kStepBlocks];     // bit i: step i of the 32 lacks the block
+  int issued = 0;                   // steps of the current run whose copies are under way
+  int in_stage = 0;                 // stage of the next step to issue
+  uint32_t stage_bad = 0;           // bit (kStepBlocks stage + block): not in the stage
+  int all_issued = 0;
   auto issue = [&]() {
     if ((issued & 31) == 0) {
+      const int32_t* row = a.table + b * a.table_stride;
 #pragma unroll
       for (int u = 0; u < kStepBlocks; ++u) {
-        const int blk = blk0 + kStepBlocks * (warp + kAttnWarps * (issued + lane)) + u;
-        pid[u] = blk < blk1 ? row[blk / a.page_blocks] : 0;
-        if (blk < blk1 && (pid[u] < 0 || pid[u] >= a.pages)) {
-          record_error(a.err, kErrCachePage);
-          pid[u] = -1;
+        const int blk = key0 / kBlockTokens + kStepBlocks * (warp + kAttnWarps * (issued + lane)) + u;
+        src[u] = nullptr;
+        if (blk < blk1) {
+          const int col = blk / a.page_blocks;
+          const int64_t page = row[col];
+          if (page >= 0 && page < a.pages)
+            src[u] = a.pool + page * a.page_stride + static_cast<int64_t>(hk) * a.page_bytes +
+                     static_cast<int64_t>(blk - col * a.page_blocks) * L::kBlockBytes;
+          else
+            record_error(a.err, kErrCachePage);
         }
+        absent[u] = __ballot_sync(0xffffffffu, src[u] == nullptr);
       }
     }
-    const int s = issued % kStages;
-    const int first = blk0 + kStepBlocks * (warp + kAttnWarps * issued);
-    int page[kStepBlocks];
-    uint32_t bytes = 0;
+    uint32_t bad = 0;
 #pragma unroll
-    for (int u = 0; u < kStepBlocks; ++u) {
-      page[u] = __shfl_sync(0xffffffffu, pid[u], issued & 31);
-      const uint32_t bit = 1u << (kStepBlocks * s + u);
-      const bool have = first + u < blk1;
-      if (have && page[u] >= 0) {
-        bytes += L::kBlockBytes;
-        stage_bad &= ~bit;
-      } else {
-        page[u] = -1;
-        stage_bad |= bit;
-      }
-    }
-    if (lane == 0) {
-      mbar_arrive_expect_tx(&bar[s], bytes);
+    for (int u = 0; u < kStepBlocks; ++u) bad |= ((absent[u] >> (issued & 31)) & 1u) << u;
+    stage_bad = (stage_bad & ~(((1u << kStepBlocks) - 1) << (kStepBlocks * in_stage))) | bad << (kStepBlocks * in_stage);
+    if (lane == (issued & 31)) {
+      uint8_t* dst = ring + in_stage * kStageBytes;
+      uint64_t* full = &bar[in_stage];
+      mbar_arrive_expect_tx(full, (kStepBlocks - __popc(bad)) * L::kBlockBytes);
 #pragma unroll
       for (int u = 0; u < kStepBlocks; ++u)
-        if (page[u] >= 0)
-          bulk_load(ring + s * kStageBytes + u * L::kBlockBytes,
-                    head_base + page[u] * a.page_stride +
-                        static_cast<int64_t>((first + u) % a.page_blocks) * L::kBlockBytes,
-                    L::kBlockBytes, &bar[s]);
+        if (src[u] != nullptr) bulk_load(dst + u * L::kBlockBytes, src[u], L::kBlockBytes, full);
     }
     ++issued;
+    ++all_issued;
+    in_stage = in_stage == kStages - 1 ? 0 : in_stage + 1;
   };
-  for (int s = 0; s < kStages && issued < steps; ++s) issue();
-
-  // Queries as the B operand: tile x, column g = row row0 + 8 x + g; the K order of a lane's channels.
-  // Padding rows are 0 and see what the last row sees.
-  uint32_t qf[NT][2 * G][2];
-  int lim[NT][2];  // keys [0, lim) visible to the rows of columns 2 t and 2 t + 1
-  int lim_lo = 0x7fffffff, lim_hi = 0;
-#pragma unroll
-  for (int x = 0; x < NT; ++x) {
-    const int r = row0 + 8 * x + g;
-    const __half* qr = a.q + static_cast<int64_t>(q0 + r / a.group) * a.q_st +
-                       static_cast<int64_t>(hk * a.group + r % a.group) * a.q_sh;
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < n_rows) v = __ldg(reinterpret_cast<const uint4*>(qr + 32 * j + 8 * t));
-      // channel i with channel i + 4, as a word's nibbles unpack
-      qf[x][2 * j][0] = __byte_perm(v.x, v.z, 0x5410);
-      qf[x][2 * j][1] = __byte_perm(v.x, v.z, 0x7632);
-      qf[x][2 * j + 1][0] = __byte_perm(v.y, v.w, 0x5410);
-      qf[x][2 * j + 1][1] = __byte_perm(v.y, v.w, 0x7632);
-    }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int rc = min(row0 + 8 * x + 2 * t + c, n_rows - 1);
-      lim[x][c] = a.causal ? min(kv, kv - n_q + rc / a.group + 1) : kv;
-    }
-  }
-  {
-    const int first_row = row0, last_row = min(row0 + kRows, n_rows) - 1;
-    lim_lo = a.causal ? min(kv, kv - n_q + first_row / a.group + 1) : kv;
-    lim_hi = a.causal ? min(kv, kv - n_q + last_row / a.group + 1) : kv;
-  }
-  const uint8_t* mask = a.mask != nullptr ? a.mask + b * a.mask_stride : nullptr;
-
-  float o[NT][2 * G][4];
-  float m[NT][2], l[NT][2];
-#pragma unroll
-  for (int x = 0; x < NT; ++x) {
-#pragma unroll
-    for (int i = 0; i < 2 * G; ++i)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[x][i][c] = 0.f;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) m[x][c] = -CUDART_INF_F, l[x][c] = 0.f;
-  }
+  __syncwarp();
+  while (issued < steps && issued < kStages) issue();
 
   // Operand rows of the mma <-> tokens of a block: rows 2 i, 2 i + 1 (+ 8) are tokens i, i + 4 (+ 8), so
   // that the four keys of a lane's V operand are t, t + 4, t + 8, t + 12 and a quad reads whole rows.
   const int tok_g = (g >> 1) + (g & 1) * 4;
+  int s = 0;           // stage of the next step to consume, and its phase
+  uint32_t phase = 0;
   bool ok = true;
-  for (int i = 0; i < steps; ++i) {
-    const int s = i % kStages;
-    const int key = key0 + kStepKeys * (warp + kAttnWarps * i);
-    const uint32_t bad = (stage_bad >> (kStepBlocks * s)) & ((1u << kStepBlocks) - 1);
-    // Which of the step's keys count for any row: bit `token` of block u.
-    const bool plain = bad == 0 && mask == nullptr && key + kStepKeys <= lim_lo;
-    uint32_t live[kStepBlocks];
-    if (!plain) {
-#pragma unroll
-      for (int u = 0; u < kStepBlocks; ++u) {
-        const int kk = key + kBlockTokens * u + lane;
-        bool on = lane < kBlockTokens && !((bad >> u) & 1) && kk < lim_hi;
-        if (on && mask != nullptr) on = kk < a.mask_cols && mask[kk] != 0;
-        live[u] = __ballot_sync(0xffffffffu, on);
-      }
-    }
-    if (!mbar_wait_spin(&bar[s], (i / kStages) & 1, a.err, kErrTimeoutFull)) {
-      ok = false;
-      break;
-    }
-    const uint8_t* st = ring + s * kStageBytes;
 
-    float sc[kStepBlocks][NT][4];
+  while (true) {
+    // Queries as the B operand: tile x, column g = row row0 + 8 x + g, the K order of a lane's channels.
+    // Scores are formed from the codes themselves, spread into the mantissa of 1024 (two instructions a
+    // pair): q' . (1024 + n) in fp32 starting at -1024 sum q', then times the group's scale, plus its minimum
+    // times sum q' (an mma with the sum as two fp16 numbers). Channels on odd nibbles, 16 n, have q' / 16. q'
+    // is q times a power of two that brings the row's largest magnitude to [2^8, 2^9): q' / 16 keeps its bits,
+    // sums stay in fp16's range. Padding rows are 0.
+    uint32_t qf[NT][2 * G][2], qsum[NT];
+    float no[NT][G][4];  // -1024 sum q' of columns 2 t and 2 t + 1, twice: an accumulator to start from
+    float cs[NT][2];     // log2 units a score unit of those columns
+    int lim[NT][2];                 // keys [0, lim) visible to them; padding rows see what the last row sees
+    const int n_rows = rq.n_q * a.group;
 #pragma unroll
-    for (int u = 0; u < kStepBlocks; ++u) {
-      const uint8_t* blk = st + u * L::kBlockBytes;
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) sc[u][x][c] = 0.f;
-      const Words<G> ka = load_words<G>(blk + tok_g * L::kRowBytes + t * (4 * G));
-      const Words<G> kb = load_words<G>(blk + (tok_g + 8) * L::kRowBytes + t * (4 * G));
-      const Words<G> sa = load_words<G>(blk + L::kOffKScale + tok_g * L::kScaleBytes);
-      const Words<G> sb = load_words<G>(blk + L::kOffKScale + (tok_g + 8) * L::kScaleBytes);
+    for (int x = 0; x < NT; ++x) {
+      const int r = row0 + 8 * x + g;
+      const __half* qr = a.q + static_cast<int64_t>(rq.q0 + r / a.group) * a.q_st +
+                         static_cast<int64_t>(hk * a.group + r % a.group) * a.q_sh;
+      uint4 v[G];
+      float top = 0.f;
 #pragma unroll
       for (int j = 0; j < G; ++j) {
-        uint32_t pa[4], pb[4];
-        unpack8(ka.w[j], __low2half2(as_h2(sa.w[j])), __high2half2(as_h2(sa.w[j])), pa);
-        unpack8(kb.w[j], __low2half2(as_h2(sb.w[j])), __high2half2(as_h2(sb.w[j])), pb);
+        v[j] = make_uint4(0, 0, 0, 0);
+        if (r < n_rows) v[j] = __ldg(reinterpret_cast<const uint4*>(qr + 32 * j + 8 * t));
+        const __half2 m2 = __hmax2(__hmax2(__habs2(as_h2(v[j].x)), __habs2(as_h2(v[j].y))),
+                                   __hmax2(__habs2(as_h2(v[j].z)), __habs2(as_h2(v[j].w))));
+        top = fmaxf(top, fmaxf(__low2float(m2), __high2float(m2)));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^(8 - floor(log2 top)) by its exponent bits
+      const uint32_t ex = __float_as_uint(top) >> 23;
+      const bool norm = top > 0.f && top <= 65504.f;
+      const float up = norm ? __uint_as_float((262u - ex) << 23) : 1.f;
+      const float down = norm ? __uint_as_float((ex - 8u) << 23) : 1.f;
+      float sum_j = 0.f, off[G];
 #pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          mma16816(sc[u][x], pa[0], pb[0], pa[1], pb[1], qf[x][2 * j][0], qf[x][2 * j][1]);
-          mma16816(sc[u][x], pa[2], pb[2], pa[3], pb[3], qf[x][2 * j + 1][0], qf[x][2 * j + 1][1]);
+      for (int j = 0; j < G; ++j) {
+        const float2 c01 = __half22float2(as_h2(v[j].x)), c23 = __half22float2(as_h2(v[j].y));
+        const float2 c45 = __half22float2(as_h2(v[j].z)), c67 = __half22float2(as_h2(v[j].w));
+        const float u16 = up * 0.0625f;
+        const __half2 p0 = __floats2half2_rn(c01.x * up, c45.x * up), p1 = __floats2half2_rn(c01.y * u16, c45.y * u16);
+        const __half2 p2 = __floats2half2_rn(c23.x * up, c67.x * up), p3 = __floats2half2_rn(c23.y * u16, c67.y * u16);
+        qf[x][2 * j][0] = as_u32(p0);
+        qf[x][2 * j][1] = as_u32(p1);
+        qf[x][2 * j + 1][0] = as_u32(p2);
+        qf[x][2 * j + 1][1] = as_u32(p3);
+        const float2 f0 = __half22float2(p0), f1 = __half22float2(p1), f2 = __half22float2(p2), f3 = __half22float2(p3);
+        const float lo = f0.x + f0.y + f2.x + f2.y, hi = f1.x + f1.y + f3.x + f3.y;
+        float both = lo + hi, sum = lo + 16.f * hi;
+#pragma unroll
+        for (int d = 1; d <= 2; d <<= 1) {
+          both += __shfl_xor_sync(0xffffffffu, both, d);
+          sum += __shfl_xor_sync(0xffffffffu, sum, d);
         }
+        off[j] = -1024.f * both;
+        if (t == j) sum_j = sum;
+      }
+      const __half sum_hi = __float2half_rn(sum_j);
+      qsum[x] = as_u32(__halves2half2(sum_hi, __float2half_rn(sum_j - __half2float(sum_hi))));
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int src = (2 * t + c) * 4;
+#pragma unroll
+        for (int j = 0; j < G; ++j) no[x][j][c] = no[x][j][c + 2] = __shfl_sync(0xffffffffu, off[j], src);
+        cs[x][c] = fmaxf(a.scale_log2 * __shfl_sync(0xffffffffu, down, src), 1.17549435e-38f);  // > 0: -inf stays -inf
+        const int rc = min(row0 + 8 * x + 2 * t + c, n_rows - 1);
+        lim[x][c] = a.causal ? min(rq.kv, rq.kv - rq.n_q + rc / a.group + 1) : rq.kv;
       }
     }
+    int lim_lo = rq.kv, lim_hi = rq.kv;
+    if (a.causal) {
+      lim_lo = min(rq.kv, rq.kv - rq.n_q + row0 / a.group + 1);
+      lim_hi = min(rq.kv, rq.kv - rq.n_q + (min(row0 + kRows, n_rows) - 1) / a.group + 1);
+    }
+    const uint8_t* mask = a.mask != nullptr ? a.mask + b * a.mask_stride : nullptr;
 
-    // Scores in log2 units, the excluded ones -inf.
+    float o[NT][2 * G][4];
+    // Running maximum in units of the scores, the same in log2 units (0 while there is none), running sum.
+    float m[NT][2], mc[NT][2], l[NT][2];
 #pragma unroll
-    for (int u = 0; u < kStepBlocks; ++u)
+    for (int x = 0; x < NT; ++x) {
+#pragma unroll
+      for (int i = 0; i < 2 * G; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[x][i][c] = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) m[x][c] = -CUDART_INF_F, mc[x][c] = 0.f, l[x][c] = 0.f;
+    }
+
+    // One step: 32 keys from stage s. With kPlain every key counts for every row.
+    auto step = [&](auto plain_tag, const int key, const uint32_t live) {
+      constexpr bool kPlain = decltype(plain_tag)::value;
+      const uint8_t* st = ring + s * kStageBytes;
+
+      float sc[kStepBlocks][NT][4];
+#pragma unroll
+      for (int u = 0; u < kStepBlocks; ++u) {
+        const uint8_t* blk = st + u * L::kBlockBytes;
+        const uint8_t* ks = blk + L::kOffKScale + tok_g * L::kScaleBytes;
+        const Words<G> ka = load_words<G>(blk + tok_g * L::kRowBytes + t * (4 * G));
+        const Words<G> kb = load_words<G>(blk + (tok_g + 8) * L::kRowBytes + t * (4 * G));
+        const Words<G> sa = load_words<G>(ks), sb = load_words<G>(ks + 8 * L::kScaleBytes);
+        const uint32_t ma = *reinterpret_cast<const uint32_t*>(ks + t % G * 4);
+        const uint32_t mb = *reinterpret_cast<const uint32_t*>(ks + 8 * L::kScaleBytes + t % G * 4);
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+          mma1688(sc[u][x], __byte_perm(ma, ma, 0x3232), __byte_perm(mb, mb, 0x3232), qsum[x]);
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          uint32_t pa[4], pb[4];
+          spread8(ka.w[j], pa);
+          spread8(kb.w[j], pb);
+          const float fa = __low2float(as_h2(sa.w[j])), fb = __low2float(as_h2(sb.w[j]));
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            float acc[4];
+            mma16816_from(acc, pa[0], pb[0], pa[1], pb[1], qf[x][2 * j][0], qf[x][2 * j][1],
+                          no[x][j]);
+            mma16816(acc, pa[2], pb[2], pa[3], pb[3], qf[x][2 * j + 1][0], qf[x][2 * j + 1][1]);
+            sc[u][x][0] = fmaf(fa, acc[0], sc[u][x][0]);
+            sc[u][x][1] = fmaf(fa, acc[1], sc[u][x][1]);
+            sc[u][x][2] = fmaf(fb, acc[2], sc[u][x][2]);
+            sc[u][x][3] = fmaf(fb, acc[3], sc[u][x][3]);
+          }
+        }
+      }
+
+      if constexpr (!kPlain) {
+#pragma unroll
+        for (int u = 0; u < kStepBlocks; ++u)
+#pragma unroll
+          for (int x = 0; x < NT; ++x)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int at = kBlockTokens * u + tok_g + (c >> 1) * 8;
+              if (!((live >> at) & 1) || key + at >= lim[x][c & 1]) sc[u][x][c] = -CUDART_INF_F;
+            }
+      }
+      float base[NT][2];
+      bool moved = false;
 #pragma unroll
       for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v = sc[u][x][c] * a.scale_log2;
-          if (!plain) {
-            const int tok = tok_g + (c >> 1) * 8;
-            if (!((live[u] >> tok) & 1) || key + kBlockTokens * u + tok >= lim[x][c & 1]) v = -CUDART_INF_F;
-          }
-          sc[u][x][c] = v;
+        for (int c = 0; c < 2; ++c) {
+          float top = fmaxf(sc[0][x][c], sc[0][x][c + 2]);
+#pragma unroll
+          for (int u = 1; u < kStepBlocks; ++u) top = fmaxf(top, fmaxf(sc[u][x][c], sc[u][x][c + 2]));
+          base[x][c] = top;
+          moved |= top > m[x][c];
         }
-    float base[NT][2];
+      // The maxima are joined across the lanes only when some lane's own exceeds the running one.
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          float f[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float top = base[x][c];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            top = fmaxf(m[x][c], top);
+            // m = -inf: nothing summed yet, and 0 stays 0
+            f[c] = m[x][c] == top ? 1.f : ex2_approx((m[x][c] - top) * cs[x][c]);
+            m[x][c] = top;
+            mc[x][c] = top == -CUDART_INF_F ? 0.f : top * cs[x][c];
+            l[x][c] *= f[c];
+          }
+#pragma unroll
+          for (int k = 0; k < 2 * G; ++k) {
+            o[x][k][0] *= f[0];
+            o[x][k][1] *= f[1];
+            o[x][k][2] *= f[0];
+            o[x][k][3] *= f[1];
+          }
+        }
+      }
+
+#pragma unroll
+      for (int u = 0; u < kStepBlocks; ++u) {
+        const uint8_t* blk = st + u * L::kBlockBytes + L::kOffV;
+        uint32_t pf[NT][2];
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          float p[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            p[c] = ex2_approx(fmaf(sc[u][x][c], cs[x][c & 1], -mc[x][c & 1]));
+            l[x][c & 1] += p[c];
+          }
+          pf[x][0] = transpose8x8(pack_half2_rn(p[0], p[1]));
+          pf[x][1] = transpose8x8(pack_half2_rn(p[2], p[3]));
+        }
+        constexpr int W = G / 2;  // words of a lane's share of a V row: two groups a word
+        Words<W> v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = load_words<W>(blk + (t + 4 * k) * L::kRowBytes + g * (2 * G));
+        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+        if constexpr (!kPlain) {
+          const uint32_t on = live >> (kBlockTokens * u + t);
+          keep0 = ((on & 1u) ? 0xffffu : 0u) | ((on & 0x10u) ? 0xffff0000u : 0u);
+          keep1 = ((on & 0x100u) ? 0xffffu : 0u) | ((on & 0x1000u) ? 0xffff0000u : 0u);
+        }
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          Words<4> vs = load_words<4>(blk + 16 * L::kRowBytes + (j * 4 + t) * 16);
+          if constexpr (!kPlain) {
+            vs.w[0] &= keep0;
+            vs.w[1] &= keep1;
+            vs.w[2] &= keep0;
+            vs.w[3] &= keep1;
+          }
+          const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+          uint32_t e[4], f[4];
+          unpack8(__byte_perm(v[0].w[j / 2], v[1].w[j / 2], sel), as_h2(vs.w[0]), as_h2(vs.w[2]), e);
+          unpack8(__byte_perm(v[2].w[j / 2], v[3].w[j / 2], sel), as_h2(vs.w[1]), as_h2(vs.w[3]), f);
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            mma16816(o[x][2 * j], e[0], e[1], f[0], f[1], pf[x][0], pf[x][1]);
+            mma16816(o[x][2 * j + 1], e[2], e[3], f[2], f[3], pf[x][0], pf[x][1]);
+          }
+        }
+      }
+    };
+
+    // The key mask is read a step ahead: one key of the step a lane.
+    auto mask_of = [&](int i) {
+      const int key = key0 + kStepKeys * (warp + kAttnWarps * i) + lane;
+      return i < steps && key < min(lim_hi, a.mask_cols) && mask[key] != 0;
+    };
+    bool mask_on = mask != nullptr && mask_of(0);
+    for (int i = 0; i < steps; ++i) {
+      const int key = key0 + kStepKeys * (warp + kAttnWarps * i);
+      const uint32_t bad = (stage_bad >> (kStepBlocks * s)) & ((1u << kStepBlocks) - 1);
+      // Which of the step's keys count for any row: bit `token` of block u.
+      const bool plain = bad == 0 && mask == nullptr && key + kStepKeys <= lim_lo;
+      uint32_t live = 0xffffffffu;  // bit: key of the step
+      if (!plain) {
+        live = __ballot_sync(0xffffffffu, !((bad >> (lane / kBlockTokens)) & 1) && key + lane < lim_hi &&
+                                              (mask == nullptr || mask_on));
+        if (mask != nullptr) mask_on = mask_of(i + 1);
+      }
+      if (!mbar_wait_spin(&bar[s], phase, a.err, kErrTimeoutFull)) {
+        ok = false;
+        break;
+      }
+      if (plain)
+        step(std::true_type{}, key, live);
+      else
+        step(std::false_type{}, key, live);
+      __syncwarp();  // every lane has read the stage
+      if (++s == kStages) s = 0, phase ^= 1;
+      if (issued < steps) issue();
+    }
+    if (!ok) {  // a copy did not arrive: wait (bounded) for what is in flight
+      for (int k = 0; k < kStages; ++k)
+        if (all_issued > k) mbar_wait(&bar[k], ((all_issued - 1 - k) / kStages) & 1, a.err, kErrTimeoutDrain);
+    }
+    ok = !__syncthreads_or(!ok);
+    if (!ok) return;  // the whole CTA, with the error word set
+
+    // The next run's copies start before this run's states are merged and written.
+    const int o_b_q0 = rq.q0, o_row0 = row0, o_hk = hk, o_chunk0 = chunk0;
+    const bool whole = chunk0 == 0 && n_chunks == rq.chunks;
+    pos += n_chunks;
+    const bool more = pos < end;
+    if (more) {
+      while (pos >= b_start + static_cast<long long>(rq.tiles) * a.heads_k * rq.chunks) {
+        b_start += static_cast<long long>(rq.tiles) * a.heads_k * rq.chunks;
+        rq = request_of<NT>(a, ++b);
+      }
+      locate();
+      issued = 0;
+      while (issued < steps && issued < kStages) issue();
+    }
+
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float top = fmaxf(sc[0][x][c], sc[0][x][c + 2]);
+      for (int c = 0; c < 2; ++c) m[x][c] *= cs[x][c];  // log2 units from here on
+    // Merge the warps' states: 2 and 3 into 0 and 1, then 1 into 0.
 #pragma unroll
-        for (int u = 1; u < kStepBlocks; ++u) top = fmaxf(top, fmaxf(sc[u][x][c], sc[u][x][c + 2]));
+    for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        base[x][c] = fmaxf(m[x][c], top);
-      }
-    bool moved = false;
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int x = 0; x < NT; ++x) moved |= base[x][0] > m[x][0] || base[x][1] > m[x][1];
-    if (__any_sync(0xffffffffu, moved)) {
+        for (int d = 4; d < 32; d <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], d);
 #pragma unroll
-      for (int x = 0; x < NT; ++x) {
-        // m = -inf: nothing summed yet (0 times anything below); base = -inf then stays so
-        const float f0 = m[x][0] == base[x][0] ? 1.f : ex2_approx(m[x][0] - base[x][0]);
-        const float f1 = m[x][1] == base[x][1] ? 1.f : ex2_approx(m[x][1] - base[x][1]);
-        l[x][0] *= f0;
-        l[x][1] *= f1;
-#pragma unroll
-        for (int k = 0; k < 2 * G; ++k) {
-          o[x][k][0] *= f0;
-          o[x][k][1] *= f1;
-          o[x][k][2] *= f0;
-          o[x][k][3] *= f1;
-        }
-        m[x][0] = base[x][0];
-        m[x][1] = base[x][1];
-      }
-    }
-
-#pragma unroll
-    for (int u = 0; u < kStepBlocks; ++u) {
-      const uint8_t* blk = st + u * L::kBlockBytes + L::kOffV;
-      uint32_t pf[NT][2];
-#pragma unroll
-      for (int x = 0; x < NT; ++x) {
-        float p[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float mx = m[x][c & 1];
-          p[c] = ex2_approx(sc[u][x][c] - (mx == -CUDART_INF_F ? 0.f : mx));
-          l[x][c & 1] += p[c];
-        }
-        pf[x][0] = transpose8x8(pack_half2_rn(p[0], p[1]));
-        pf[x][1] = transpose8x8(pack_half2_rn(p[2], p[3]));
-      }
-      constexpr int W = G / 2;  // words of a lane's share of a V row: two groups a word
-      Words<W> v[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = load_words<W>(blk + (t + 4 * k) * L::kRowBytes + g * (2 * G));
-      uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-      if (!plain) {
-        const uint32_t on = live[u] >> t;
-        keep0 = ((on & 1u) ? 0xffffu : 0u) | ((on & 0x10u) ? 0xffff0000u : 0u);
-        keep1 = ((on & 0x100u) ? 0xffffu : 0u) | ((on & 0x1000u) ? 0xffff0000u : 0u);
-      }
-#pragma unroll
-      for (int j = 0; j < G; ++j) {
-        Words<4> vs = load_words<4>(blk + 16 * L::kRowBytes + (j * 4 + t) * 16);
-        if (!plain) {
-          vs.w[0] &= keep0;
-          vs.w[1] &= keep1;
-          vs.w[2] &= keep0;
-          vs.w[3] &= keep1;
-        }
-        const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-        uint32_t e[4], f[4];
-        unpack8(__byte_perm(v[0].w[j / 2], v[1].w[j / 2], sel), as_h2(vs.w[0]), as_h2(vs.w[2]), e);
-        unpack8(__byte_perm(v[2].w[j / 2], v[3].w[j / 2], sel), as_h2(vs.w[1]), as_h2(vs.w[3]), f);
+    for (int half = kAttnWarps / 2; half > 0; half >>= 1) {
+      if (warp >= half && warp < 2 * half) {
+        float* to = sh_state + (warp - half) * kState * 32 + lane;
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-          mma16816(o[x][2 * j], e[0], e[1], f[0], f[1], pf[x][0], pf[x][1]);
-          mma16816(o[x][2 * j + 1], e[2], e[3], f[2], f[3], pf[x][0], pf[x][1]);
+#pragma unroll
+          for (int k = 0; k < 2 * G; ++k)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) to[(x * 8 * G + 4 * k + c) * 32] = o[x][k][c];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            to[(NT * 8 * G + 4 * x + c) * 32] = m[x][c];
+            to[(NT * 8 * G + 4 * x + 2 + c) * 32] = l[x][c];
+          }
         }
       }
-    }
-    __syncwarp();  // every lane has read the stage
-    if (issued < steps) issue();
-  }
-  if (!ok) {  // a copy did not arrive: wait (bounded) for what is in flight; the other warps still meet below
-    for (int s = 0; s < kStages; ++s) {
-      const int last = (issued - 1 - s) / kStages;
-      if (issued > s) mbar_wait(&bar[s], last & 1, a.err, kErrTimeoutDrain);
-    }
-  }
-
-  // Merge the warps' states.
+      __syncthreads();
+      if (warp < half) {
+        const float* from = sh_state + warp * kState * 32 + lane;
 #pragma unroll
-  for (int x = 0; x < NT; ++x)
+        for (int x = 0; x < NT; ++x) {
+          float f[2], h[2];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 2; ++c) {
+            const float other = from[(NT * 8 * G + 4 * x + c) * 32];
+            const float top = fmaxf(m[x][c], other);
+            const float ref = top == -CUDART_INF_F ? 0.f : top;
+            f[c] = ex2_approx(m[x][c] - ref);
+            h[c] = ex2_approx(other - ref);
+            l[x][c] = f[c] * l[x][c] + h[c] * from[(NT * 8 * G + 4 * x + 2 + c) * 32];
+            m[x][c] = top;
+          }
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], d);
-      if (g == 0) {
-        sh_m[warp][8 * x + 2 * t + c] = m[x][c];
-        sh_l[warp][8 * x + 2 * t + c] = l[x][c];
+          for (int k = 0; k < 2 * G; ++k)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              o[x][k][c] = f[c & 1] * o[x][k][c] + h[c & 1] * from[(x * 8 * G + 4 * k + c) * 32];
+        }
       }
+      __syncthreads();
     }
-  __syncthreads();  // also: no warp's copies are in flight any more, the rings are free
-  float* so = reinterpret_cast<float*>(smem);
+    if (warp == 0) {
 #pragma unroll
-  for (int x = 0; x < NT; ++x)
+      for (int x = 0; x < NT; ++x)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float* dst = so + (warp * kRows + 8 * x + 2 * t + c) * D + 4 * g;
+        for (int c = 0; c < 2; ++c) {
+          const int r = 8 * x + 2 * t + c;
+          if (o_row0 + r >= n_rows) continue;
+          if (whole) {
+            const float sum = l[x][c];
+            const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // NaN stays
+            __half* dst = a.out + static_cast<int64_t>(o_b_q0 + (o_row0 + r) / a.group) * a.o_st +
+                          static_cast<int64_t>(o_hk * a.group + (o_row0 + r) % a.group) * a.o_sh + 4 * g;
 #pragma unroll
-      for (int j = 0; j < G; ++j)
-        *reinterpret_cast<float4*>(dst + 32 * j) = make_float4(o[x][2 * j][c], o[x][2 * j][c + 2],
-                                                               o[x][2 * j + 1][c], o[x][2 * j + 1][c + 2]);
+            for (int j = 0; j < G; ++j)
+              *reinterpret_cast<uint2*>(dst + 32 * j) =
+                  make_uint2(pack_half2_rn(o[x][2 * j][c] * inv, o[x][2 * j][c + 2] * inv),
+                             pack_half2_rn(o[x][2 * j + 1][c] * inv, o[x][2 * j + 1][c + 2] * inv));
+          } else {
+            const int64_t at = (2 * static_cast<int64_t>(blockIdx.x) + (o_chunk0 == 0 ? 1 : 0)) * kRows + r;
+            float* dst = a.part_o + at * D + 4 * g;
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+              *reinterpret_cast<float4*>(dst + 32 * j) = make_float4(o[x][2 * j][c], o[x][2 * j][c + 2],
+                                                                     o[x][2 * j + 1][c], o[x][2 * j + 1][c + 2]);
+            if (g == 0) a.part_ml[at] = make_float2(m[x][c], l[x][c]);
+          }
+        }
     }
-  __syncthreads();
-  for (int i = tid; i < kRows * (D / 4); i += kAttnThreads) {
-    const int r = i / (D / 4), d = i % (D / 4) * 4;
-    if (row0 + r >= n_rows) break;
-    float top = sh_m[0][r];
-#pragma unroll
-    for (int w = 1; w < kAttnWarps; ++w) top = fmaxf(top, sh_m[w][r]);
-    const float ref = top == -CUDART_INF_F ? 0.f : top;
-    float sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kAttnWarps; ++w) {
-      const float f = ex2_approx(sh_m[w][r] - ref);
-      const float4 v = *reinterpret_cast<const float4*>(so + (w * kRows + r) * D + d);
-      sum += f * sh_l[w][r];
-      acc.x += f * v.x;
-      acc.y += f * v.y;
-      acc.z += f * v.z;
-      acc.w += f * v.w;
-    }
-    const int64_t token = q0 + (row0 + r) / a.group;
-    const int hq = hk * a.group + (row0 + r) % a.group;
-    if (parts == 1) {
-      const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // NaN stays
-      *reinterpret_cast<uint2*>(a.out + token * a.o_st + hq * a.o_sh + d) =
-          make_uint2(pack_half2_rn(acc.x * inv, acc.y * inv), pack_half2_rn(acc.z * inv, acc.w * inv));
-    } else {
-      const int64_t at = (static_cast<int64_t>(split) * a.q_tokens + token) * a.heads_q + hq;
-      *reinterpret_cast<float4*>(a.part_o + at * D + d) = acc;
-      if (d == 0) a.part_ml[at] = make_float2(top, sum);
-    }
+    if (!more) return;
   }
 }
 
-// Joins the splits of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. One warp a row.
-template <int D>
+// Joins the partial states of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. One CTA a row, the parts
+// dealt to its warps, so that a long request's parts (one from every CTA of the machine) are read in a few
+// round trips.
+template <int D, int NT>
 __global__ void __launch_bounds__(kAttnThreads) join_kernel(const AttnArgs a) {
-  const int b = blockIdx.y, lane = threadIdx.x & 31;
-  int q0 = b, n_q = 1;
-  if (a.cu != nullptr) {
-    q0 = a.cu[b];
-    n_q = min(a.cu[b + 1] - q0, a.max_q);
-  }
-  if (q0 < 0 || n_q <= 0 || q0 + static_cast<int64_t>(n_q) > a.q_tokens) return;
-  const int i = blockIdx.x * kAttnWarps + (threadIdx.x >> 5);
-  if (i >= n_q * a.heads_q) return;
-  const int64_t cap = static_cast<int64_t>(a.cols) * a.page_blocks * kBlockTokens;
-  const int kv = static_cast<int>(min(static_cast<int64_t>(max(a.kv_lens[b], 0)),
-                                      min(cap, static_cast<int64_t>(a.chunk) * a.splits)));
-  const int parts = max(1, (kv + a.chunk - 1) / a.chunk);
-  if (parts == 1) return;  // written by its only CTA
-  const int64_t token = q0 + i / a.heads_q;
-  const int hq = i % a.heads_q;
-  const int64_t row = token * a.heads_q + hq, step = a.q_tokens * a.heads_q;
-  float top = -CUDART_INF_F;
-  for (int s = lane; s < parts; s += 32) top = fmaxf(top, a.part_ml[row + s * step].x);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  const float ref = top == -CUDART_INF_F ? 0.f : top;
   constexpr int V = D / 32;  // channels a lane
-  float acc[V] = {}, sum = 0.f;
-  for (int s = 0; s < parts; ++s) {
-    const float2 ml = a.part_ml[row + s * step];
-    const float f = ex2_approx(ml.x - ref);
-    sum += f * ml.y;
-    const float* o = a.part_o + (row + s * step) * D + lane * V;
-    if constexpr (V == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(o);
-      acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(o);
-      acc[0] += f * v.x, acc[1] += f * v.y;
+  __shared__ float sh_o[kAttnWarps][D], sh_m[kAttnWarps], sh_l[kAttnWarps];
+  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Request rq = request_of<NT>(a, b);
+  const int i = blockIdx.x;
+  if (i >= rq.n_q * a.heads_q) return;
+  const int token = i / a.heads_q, hq = i - token * a.heads_q;
+  const int hk = hq / a.group, row = token * a.group + hq - hk * a.group;
+  const int tile = row / (8 * NT), r = row - tile * (8 * NT);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the attention kernel has ended, its writes are visible
+  const long long total = a.starts[a.batch], per = (total + a.ctas - 1) / a.ctas;
+  const long long first = a.starts[b] + (static_cast<long long>(hk) * rq.tiles + tile) * rq.chunks;
+  const int c0 = static_cast<int>(first / per), c1 = static_cast<int>((first + rq.chunks - 1) / per);
+  if (c0 == c1) return;  // one CTA had it whole and wrote it
+  auto slot = [&](int c) { return (2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * (8 * NT) + r; };
+  // Each warp with a running maximum of its own, four parts in flight.
+  float acc[V] = {}, sum = 0.f, top = -CUDART_INF_F;
+  for (int c = c0 + warp; c <= c1; c += 4 * kAttnWarps) {
+    float2 ml[4];
+    float v[4][V];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t at = slot(min(c + k * kAttnWarps, c1));
+      ml[k] = a.part_ml[at];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[k][e] = a.part_o[at * D + lane * V + e];
+      if (c + k * kAttnWarps > c1) ml[k] = make_float2(-CUDART_INF_F, 0.f);
     }
+    float now = top;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) now = fmaxf(now, ml[k].x);
+    const float ref = now == -CUDART_INF_F ? 0.f : now;
+    const float keep = ex2_approx(top - ref);
+    sum *= keep;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] *= keep;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (c + k * kAttnWarps > c1) break;
+      const float f = ex2_approx(ml[k].x - ref);
+      sum += f * ml[k].y;
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += f * v[k][e];
+    }
+    top = now;
   }
-  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-  __half* dst = a.out + token * a.o_st + hq * a.o_sh + lane * V;
-  if constexpr (V == 4)
-    *reinterpret_cast<uint2*>(dst) =
-        make_uint2(pack_half2_rn(acc[0] * inv, acc[1] * inv), pack_half2_rn(acc[2] * inv, acc[3] * inv));
-  else
-    *reinterpret_cast<uint32_t*>(dst) = pack_half2_rn(acc[0] * inv, acc[1] * inv);
+#pragma unroll
+  for (int e = 0; e < V; ++e) sh_o[warp][lane * V + e] = acc[e];
+  if (lane == 0) sh_m[warp] = top, sh_l[warp] = sum;
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= D) return;
+  top = sh_m[0];
+#pragma unroll
+  for (int w = 1; w < kAttnWarps; ++w) top = fmaxf(top, sh_m[w]);
+  const float ref = top == -CUDART_INF_F ? 0.f : top;
+  float o = 0.f;
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kAttnWarps; ++w) {
+    const float f = ex2_approx(sh_m[w] - ref);
+    sum += f * sh_l[w];
+    o += f * sh_o[w][d];
+  }
+  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // NaN stays
+  a.out[static_cast<int64_t>(rq.q0 + token) * a.o_st + static_cast<int64_t>(hq) * a.o_sh + d] = __float2half_rn(o * inv);
 }
 
 struct Plan {
-  int nt, row_tiles, chunk, splits;
-  int64_t part_o_bytes, part_ml_bytes;
+  int nt, ctas;
+  int64_t starts_bytes, part_o_bytes, part_ml_bytes;
+  int64_t bytes() const { return starts_bytes + part_o_bytes + part_ml_bytes; }
 };
 
-// Shape of the launch, from host-known sizes alone. Two row tiles a CTA where more than 8 rows share a KV
-// head (the unpacking is shared; four would spill). The key axis is cut so that about `kWaves` CTAs fall on
-// every slot of the machine, but not into pieces under 256 keys, whose start and join would cost more than
-// they save.
+// Two row tiles a CTA where more than 8 rows share a KV head (the unpacking is shared; four would spill). As
+// many CTAs as are resident at once, or as there can be chunks.
 static Plan plan_of(const tm_kv4_attn_params* p) {
   Plan r{};
-  const int rows = p->max_seqlen_q * (p->heads_q / p->heads_k);
+  const int64_t rows = static_cast<int64_t>(p->max_seqlen_q) * (p->heads_q / p->heads_k);
   r.nt = rows > 8 ? 2 : 1;
-  r.row_tiles = (rows + 8 * r.nt - 1) / (8 * r.nt);
-  const int64_t units = static_cast<int64_t>(p->batch) * p->heads_k * r.row_tiles;
-  constexpr int64_t kSlots = kSms * 3, kWaves = 3;
-  const int64_t keys = p->max_kv_len > 0 ? p->max_kv_len : 1;
-  int64_t chunk = (keys * units + kSlots * kWaves - 1) / (kSlots * kWaves);
-  if (chunk < 256) chunk = 256;
-  chunk = (chunk + kChunkKeys - 1) / kChunkKeys * kChunkKeys;
-  r.splits = static_cast<int>((keys + chunk - 1) / chunk);
-  r.chunk = static_cast<int>(chunk);
-  if (r.splits > 1) {
-    const int64_t n = static_cast<int64_t>(r.splits) * p->q_tokens * p->heads_q;
-    r.part_o_bytes = n * p->head_dim * 4;
-    r.part_ml_bytes = n * 8;
-  }
+  const int64_t tiles = (rows + 8 * r.nt - 1) / (8 * r.nt);
+  const int64_t chunks = p->max_kv_len / kChunkKeys + 1;
+  const int64_t most = static_cast<int64_t>(p->batch) * p->heads_k * tiles;
+  const int64_t slots = kSms * resident(r.nt);
+  r.ctas = static_cast<int>(most >= slots || chunks >= slots || most * chunks >= slots ? slots : most * chunks);
+  r.starts_bytes = (static_cast<int64_t>(p->batch) + 2) / 2 * 16;
+  r.part_o_bytes = 2ll * r.ctas * 8 * r.nt * p->head_dim * 4;
+  r.part_ml_bytes = 2ll * r.ctas * 8 * r.nt * 8;
   return r;
 }
 
@@ -587,23 +815,34 @@ static int check(const tm_kv4_attn_params* p) {
   if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->pool, 16)) return TM_ERR_ALIGN;
   if (p->q_stride_tok % 8 || p->q_stride_head % 8 || p->o_stride_tok % 8 || p->o_stride_head % 8) return TM_ERR_ALIGN;
   if (p->key_mask != nullptr && p->mask_cols < 0) return TM_ERR_SHAPE;
-  const Plan r = plan_of(p);
-  if (r.splits > 65535) return TM_ERR_UNSUPPORTED;
+  if (!(p->sm_scale > 0.f) || p->sm_scale > 3.4028235e38f) return TM_ERR_SHAPE;  // maxima are taken before scaling
+  // a request's chunks are counted in 32 bits
+  const double rows = static_cast<double>(p->max_seqlen_q) * p->heads_q;
+  if ((rows / 8 + p->heads_k) * (p->max_kv_len / kChunkKeys + 1.0) > 2147483647.0) return TM_ERR_UNSUPPORTED;
   return TM_OK;
 }
 
 template <int D, int NT>
-static cudaError_t launch(const AttnArgs& a, int batch, cudaStream_t st) {
-  constexpr int smem = kAttnWarps * kStages * kStepBlocks * Layout<D>::kBlockBytes;
+static cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
+  constexpr int smem = kAttnWarps * kStages * kStepBlocks * Layout<D>::kBlockBytes +
+                       kAttnWarps / 2 * NT * (8 * Layout<D>::kGroups + 4) * 32 * 4;
   cudaError_t e = cudaFuncSetAttribute(attn_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid(a.heads_k * a.row_tiles, batch, a.splits);
-  attn_kernel<D, NT><<<grid, kAttnThreads, smem, st>>>(a);
-  if (a.splits > 1) {
-    const dim3 jg((a.max_q * a.heads_q + kAttnWarps - 1) / kAttnWarps, batch);
-    join_kernel<D><<<jg, kAttnThreads, 0, st>>>(a);
-  }
-  return cudaGetLastError();
+  attn_kernel<D, NT><<<a.ctas, kAttnThreads, smem, st>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  // The join is set up while the attention runs (programmatic dependent launch) and waits for its end.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(a.max_q) * a.heads_q),
+                     static_cast<unsigned>(a.batch));
+  cfg.blockDim = dim3(kAttnThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel<D, NT>, a);
 }
 
 }  // namespace kv4
@@ -615,8 +854,7 @@ extern "C" int tm_kv4_attn_workspace(const tm_kv4_attn_params* p, int64_t* bytes
   *bytes = 0;
   const int rc = check(p);
   if (rc != TM_OK || p->batch == 0 || p->q_tokens == 0 || p->max_seqlen_q == 0) return rc;
-  const Plan r = plan_of(p);
-  *bytes = r.part_o_bytes + r.part_ml_bytes;
+  *bytes = plan_of(p).bytes();
   return TM_OK;
 }
 
@@ -625,10 +863,9 @@ extern "C" int tm_kv4_attn(const tm_kv4_attn_params* p, void* workspace, int64_t
   const int rc = check(p);
   if (rc != TM_OK || p->batch == 0 || p->q_tokens == 0 || p->max_seqlen_q == 0) return rc;
   const Plan r = plan_of(p);
-  const int64_t need = r.part_o_bytes + r.part_ml_bytes;
-  if (need > 0 && workspace == nullptr) return TM_ERR_NULL;
-  if (workspace_bytes < need) return TM_ERR_SHAPE;
-  if (need > 0 && !aligned(workspace, 16)) return TM_ERR_ALIGN;
+  if (workspace == nullptr) return TM_ERR_NULL;
+  if (workspace_bytes < r.bytes()) return TM_ERR_SHAPE;
+  if (!aligned(workspace, 16)) return TM_ERR_ALIGN;
   AttnArgs a{};
   a.q = static_cast<const __half*>(p->q);
   a.q_st = p->q_stride_tok;
@@ -653,20 +890,23 @@ extern "C" int tm_kv4_attn(const tm_kv4_attn_params* p, void* workspace, int64_t
   a.heads_q = p->heads_q;
   a.heads_k = p->heads_k;
   a.group = p->heads_q / p->heads_k;
-  a.row_tiles = r.row_tiles;
+  a.batch = p->batch;
   a.max_q = p->max_seqlen_q;
+  const int64_t room = static_cast<int64_t>(p->cols) * p->page_size;
+  a.max_kv = p->max_kv_len < room ? p->max_kv_len : room;
   a.causal = p->causal;
   a.scale_log2 = p->sm_scale * 1.4426950408889634f;
-  a.chunk = r.chunk;
-  a.splits = r.splits;
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + r.part_o_bytes);
+  a.ctas = r.ctas;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.starts = reinterpret_cast<long long*>(ws);
+  a.part_o = reinterpret_cast<float*>(ws + r.starts_bytes);
+  a.part_ml = reinterpret_cast<float2*>(ws + r.starts_bytes + r.part_o_bytes);
   a.err = p->error_flag;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (p->head_dim == 128)
-    e = r.nt == 2 ? launch<128, 2>(a, p->batch, st) : launch<128, 1>(a, p->batch, st);
+    e = r.nt == 2 ? launch<128, 2>(a, st) : launch<128, 1>(a, st);
   else
-    e = r.nt == 2 ? launch<64, 2>(a, p->batch, st) : launch<64, 1>(a, p->batch, st);
+    e = r.nt == 2 ? launch<64, 2>(a, st) : launch<64, 1>(a, st);
   return e == cudaSuccess ? TM_OK : TM_ERR_LAUNCH;
 }

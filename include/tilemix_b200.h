@@ -318,7 +318,6 @@ typedef struct tm_block_tables_params {
   int32_t* cu_seqlens;        /* out [batch + 1]: row offsets of the new tokens */
   int32_t* kv_lens;           /* out [batch]: cached + new; not an input's buffer */
   int64_t* free_span_out;     /* out [2]; not free_span's buffer */
-  int* error_flag;
 } tm_block_tables_params;
 
 /* Pages, slots, positions and offsets of the next tokens of a batch, from their
@@ -326,7 +325,7 @@ typedef struct tm_block_tables_params {
  * order. If pages, columns or slots do not suffice, or a length is negative,
  * nothing is allocated: every slot is -1, kv_lens = cached_lens, cu_seqlens 0,
  * free_span_out = free_span, and the error word is set. batch <= 8192. */
-int tm_build_block_tables(const tm_block_tables_params* params, void* stream);
+int tm_build_block_tables(const tm_block_tables_params* params, int* error_flag, void* stream);
 
 /* Return the pages of finished requests (done[b] != 0) to the ring's end, in
  * request order: lens[b] becomes 0, its table entries -1, free_span[1] grows. */
@@ -367,7 +366,6 @@ typedef struct tm_kv4_attn_params {
   int max_seqlen_q, max_kv_len; /* host bounds of the query and cache lengths */
   int causal; /* query i of n sees the keys before position kv_len - n + i + 1; else all keys */
   float sm_scale; /* > 0 */
-  int* error_flag;
 } tm_kv4_attn_params;
 
 /* Attention of a few query tokens a request over its cached keys. A row without
@@ -376,7 +374,8 @@ typedef struct tm_kv4_attn_params {
  * bytes, contents free); calls that may overlap need one each. Keys beyond
  * max_kv_len are left out and reported. */
 int tm_kv4_attn_workspace(const tm_kv4_attn_params* params, int64_t* bytes);
-int tm_kv4_attn(const tm_kv4_attn_params* params, void* workspace, int64_t workspace_bytes, void* stream);
+int tm_kv4_attn(const tm_kv4_attn_params* params, void* workspace, int64_t workspace_bytes, int* error_flag,
+                void* stream);
 
 /*
  * Linear layer in 8-bit integers (no reference counterpart).
@@ -394,10 +393,16 @@ int tm_kv4_attn(const tm_kv4_attn_params* params, void* workspace, int64_t works
 #define TM_DTYPE_BF16 1
 #define TM_DTYPE_FP32 2
 int tm_quant_per_token_int8(const void* x, int dtype, int64_t x_stride, int64_t rows, int cols, int8_t* out,
-                            int64_t out_stride, float* scale, void* stream);
+                            int64_t out_stride, float* scale, int* error_flag, void* stream);
 int tm_int8_matmul(const int8_t* x8, int64_t x_stride, const float* x_scale, const int8_t* w8, int64_t w_stride,
                    const float* w_scale, const void* bias, void* out, int64_t out_stride, int out_dtype,
                    int64_t tokens, int out_features, int in_features, int* error_flag, void* stream);
+/* tm_quant_per_token_int8 of x [tokens, in_features] (TM_DTYPE_FP16 or _BF16) into x8 (row stride x8_stride) and
+ * x_scale, then tm_int8_matmul of them: out and bias in x's type. x8 and x_scale are the caller's scratch. */
+int tm_int8_linear(const void* x, int dtype, int64_t x_stride, int8_t* x8, int64_t x8_stride, float* x_scale,
+                   const int8_t* w8, int64_t w_stride, const float* w_scale, const void* bias, void* out,
+                   int64_t out_stride, int64_t tokens, int out_features, int in_features, int* error_flag,
+                   void* stream);
 
 /* Human-readable text for a TM_* status code. */
 const char* tm_status_string(int status);

@@ -201,7 +201,7 @@ def test_c_abi_refusals_need_no_gpu():
         p.heads_q, p.heads_k, p.head_dim, p.max_seqlen_q, p.max_kv_len, p.causal, p.sm_scale = 8, 2, 128, 1, 128, 1, 0.1
         for k, v in over.items():
             setattr(p, k, v)
-        return lib().tm_kv4_attn_workspace(ctypes.byref(p), ctypes.byref(need)), p
+        return lib().tm_kv4_attn_workspace(ctypes.addressof(p), ctypes.byref(need)), p
 
     assert attn()[0] == 0
     for status, over in ((-1, dict(q=None)), (-1, dict(kv_lens=None)), (-1, dict(pool=None)), (-2, dict(heads_q=7)),
@@ -215,9 +215,9 @@ def test_c_abi_refusals_need_no_gpu():
     # the parts of a split key axis need their workspace
     rc, p = attn(batch=1, q_tokens=1, max_kv_len=1 << 20, cols=1 << 15)
     assert rc == 0 and need.value > 0
-    assert lib().tm_kv4_attn(ctypes.byref(p), None, 0, None) == -1
-    assert lib().tm_kv4_attn(ctypes.byref(p), fake, need.value - 1, None) == -2
-    assert lib().tm_kv4_attn(ctypes.byref(p), fake + 4, need.value, None) == -3
+    assert lib().tm_kv4_attn(ctypes.addressof(p), None, 0, None, None) == -1
+    assert lib().tm_kv4_attn(ctypes.addressof(p), fake, need.value - 1, None, None) == -2
+    assert lib().tm_kv4_attn(ctypes.addressof(p), fake + 4, need.value, None, None) == -3
 
     args = [fake, 256, 128, fake, 256, 128, 4, fake, fake, 8, 2, 128, 32, None, None]
     for at, value, status in ((0, None, -1), (7, None, -1), (8, None, -1), (0, fake + 2, -3), (1, 260, -3),
@@ -239,7 +239,7 @@ def test_c_abi_refusals_need_no_gpu():
         p.table_stride, p.cols, p.capacity, p.batch, p.page_size, p.n_slots = 4, 4, 8, 3, 16, 5
         for k, v in over.items():
             setattr(p, k, v)
-        return lib().tm_build_block_tables(ctypes.byref(p), None)
+        return lib().tm_build_block_tables(ctypes.addressof(p), None, None)
 
     for status, over in ((-1, dict(free_span=None)), (-1, dict(slots=None)), (-1, dict(kv_lens=None)),
                          (-2, dict(page_size=8)), (-2, dict(n_slots=-1)), (-4, dict(batch=8193)),

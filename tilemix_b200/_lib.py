@@ -5,9 +5,9 @@ be loaded, :func:`lib` raises. Build it with ``python -m tilemix_b200.build``.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
@@ -98,7 +98,7 @@ class TmBlockTablesParams(ctypes.Structure):
         ("cached_lens", c_void_p), ("new_lens", c_void_p), ("block_table", c_void_p), ("table_stride", c_i64),
         ("cols", c_int), ("free_pages", c_void_p), ("capacity", c_i64), ("free_span", c_void_p),
         ("batch", c_int), ("page_size", c_int), ("n_slots", c_i64), ("slots", c_void_p), ("positions", c_void_p),
-        ("cu_seqlens", c_void_p), ("kv_lens", c_void_p), ("free_span_out", c_void_p), ("error_flag", c_void_p),
+        ("cu_seqlens", c_void_p), ("kv_lens", c_void_p), ("free_span_out", c_void_p),
     ]
 
 
@@ -114,7 +114,7 @@ class TmKv4AttnParams(ctypes.Structure):
         ("key_mask", c_void_p), ("mask_stride", c_i64), ("mask_cols", c_int),
         ("batch", c_int), ("heads_q", c_int), ("heads_k", c_int), ("head_dim", c_int),
         ("max_seqlen_q", c_int), ("max_kv_len", c_int), ("causal", c_int),
-        ("sm_scale", ctypes.c_float), ("error_flag", c_void_p),
+        ("sm_scale", ctypes.c_float),
     ]
 
 
@@ -139,23 +139,25 @@ SIGNATURES = {
                                       c_int, c_void_p]),
     "tm_silu_mul": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_void_p]),
     "tm_rms_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_int, ctypes.c_float, c_void_p]),
-    "tm_build_block_tables": (c_int, [ctypes.POINTER(TmBlockTablesParams), c_void_p]),
+    "tm_build_block_tables": (c_int, [c_void_p, c_void_p, c_void_p]),
     "tm_release_pages": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_int, c_void_p, c_i64, c_void_p, c_int, c_int,
                                  c_void_p, c_void_p]),
     "tm_kv4_append": (c_int, [c_void_p, c_i64, c_i64, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_void_p, c_i64,
                               c_int, c_int, c_int, c_void_p, c_void_p]),
     "tm_kv4_read": (c_int, [c_void_p, c_i64, c_int, c_int, c_int, c_void_p, c_i64, c_void_p, c_void_p, c_void_p,
                             c_void_p]),
-    "tm_kv4_attn_workspace": (c_int, [ctypes.POINTER(TmKv4AttnParams), ctypes.POINTER(c_i64)]),
-    "tm_kv4_attn": (c_int, [ctypes.POINTER(TmKv4AttnParams), c_void_p, c_i64, c_void_p]),
-    "tm_quant_per_token_int8": (c_int, [c_void_p, c_int, c_i64, c_i64, c_int, c_void_p, c_i64, c_void_p, c_void_p]),
+    "tm_kv4_attn_workspace": (c_int, [c_void_p, ctypes.POINTER(c_i64)]),
+    "tm_kv4_attn": (c_int, [c_void_p, c_void_p, c_i64, c_void_p, c_void_p]),
+    "tm_quant_per_token_int8": (c_int, [c_void_p, c_int, c_i64, c_i64, c_int, c_void_p, c_i64, c_void_p, c_void_p,
+                                        c_void_p]),
     "tm_int8_matmul": (c_int, [c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_i64, c_int,
                                c_i64, c_int, c_int, c_void_p, c_void_p]),
+    "tm_int8_linear": (c_int, [c_void_p, c_int, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_void_p, c_void_p,
+                               c_void_p, c_i64, c_i64, c_int, c_int, c_void_p, c_void_p]),
     "tm_status_string": (ctypes.c_char_p, [c_int]),
 }
 
 _LIB = None
-_NO_SWITCH = contextlib.nullcontext()
 
 
 def lib() -> ctypes.CDLL:
@@ -178,12 +180,47 @@ def lib() -> ctypes.CDLL:
     return _LIB
 
 
-def on_device(device):
-    """Context in which a kernel of ``device`` (a CUDA ``torch.device`` with an index) is launched:
-    nothing to do when it is the current one, as it almost always is."""
+def launch(name: str, device, *args) -> None:
+    """Call an entry point that ends in (error word, stream) on ``device`` (a CUDA ``torch.device``
+    with an index) and the stream that is current there; raises what the status says. Calls of a
+    few microseconds are made through here, so it looks things up once and switches the device
+    only if it has to."""
     import torch
 
-    return _NO_SWITCH if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    index = device.index
+    args += (error_word_ptr(index), torch._C._cuda_getCurrentRawStream(index))
+    fn = getattr(_LIB or lib(), name)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args)
+    if rc:
+        check(rc, name)
+
+
+_ERROR_WORD_PTRS: dict[int, int] = {}
+
+
+def error_word_ptr(index: int) -> int:
+    """Address of the device error word (``tilemix_b200.attention.tilemix.device_error_code`` reads it)."""
+    ptr = _ERROR_WORD_PTRS.get(index)
+    if ptr is None:
+        import torch
+
+        from tilemix_b200.attention.tilemix import _error_word
+
+        ptr = _ERROR_WORD_PTRS[index] = _error_word(torch.device("cuda", index)).data_ptr()
+    return ptr
+
+
+def packer(cls):
+    """``pack(*field values)``: the bytes of a C structure mirrored by ``cls``, several times faster than
+    filling a ctypes instance. Native alignment is the C compiler's."""
+    codes = {c_void_p: "P", c_i64: "q", c_int: "i", ctypes.c_float: "f"}
+    form = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_) + "0q")
+    assert form.size == ctypes.sizeof(cls)
+    return form.pack
 
 
 def check(status: int, what: str) -> None:

@@ -19,18 +19,20 @@ word (``tilemix_b200.attention.tilemix.device_error_code``: 11, 12, 13), never i
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
 from torch import Tensor
 
-from tilemix_b200._lib import TmBlockTablesParams, TmKv4AttnParams, check, lib, on_device
-from tilemix_b200.attention.tilemix import _error_word, _raise_first
+from tilemix_b200._lib import TmBlockTablesParams, TmKv4AttnParams, check, launch, lib, packer
 
 __all__ = ["BlockTables", "build_block_tables", "release_pages", "kv4_pool", "kv4_append", "kv4_read",
            "kv4_attention"]
 
 _HEAD_DIMS = (64, 128)
+_pack_tables = packer(TmBlockTablesParams)
+_pack_attn = packer(TmKv4AttnParams)
 
 
 class BlockTables(NamedTuple):
@@ -41,10 +43,6 @@ class BlockTables(NamedTuple):
     cu_seqlens_q: Tensor   # int32 [batch + 1]: row offsets of the requests' new tokens
     kv_lens: Tensor        # int32 [batch]: tokens in the cache once the new ones are stored
     free_span: Tensor      # int64 [2]: the ring's free entries after this call
-
-
-def _stream(t: Tensor) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
 def _check_page_size(page_size: int) -> None:
@@ -98,14 +96,11 @@ def build_block_tables(cached_lens: Tensor, new_lens: Tensor, block_table: Tenso
     cu = torch.empty(batch + 1, dtype=torch.int32, device=device)
     kv_lens = torch.empty(batch, dtype=torch.int32, device=device)
     span = torch.empty(2, dtype=torch.int64, device=device)
-    p = TmBlockTablesParams(cached_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
-                            block_table.stride(0), block_table.shape[1], free_pages.data_ptr(), free_pages.numel(),
-                            free_span.data_ptr(), batch, page_size, max_new_tokens, slots.data_ptr(),
-                            positions.data_ptr(), cu.data_ptr(), kv_lens.data_ptr(), span.data_ptr(),
-                            _error_word(device).data_ptr())
-    with on_device(device):
-        rc = lib().tm_build_block_tables(ctypes.byref(p), _stream(cached_lens))
-    check(rc, "tm_build_block_tables")
+    launch("tm_build_block_tables", device,
+           _pack_tables(cached_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+                        block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_span.data_ptr(), batch,
+                        page_size, max_new_tokens, slots.data_ptr(), positions.data_ptr(), cu.data_ptr(),
+                        kv_lens.data_ptr(), span.data_ptr()))
     return BlockTables(slots, positions, cu, kv_lens, span)
 
 
@@ -126,12 +121,8 @@ def release_pages(lens: Tensor, done: Tensor, block_table: Tensor, free_pages: T
     batch = lens.numel()
     if done.numel() != batch or block_table.shape[0] != batch or free_span.numel() != 2:
         raise ValueError("lens, done and block_table must agree on the batch, free_span has two entries")
-    with on_device(device):
-        rc = lib().tm_release_pages(lens.data_ptr(), done.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-                                    block_table.shape[1], free_pages.data_ptr(), free_pages.numel(),
-                                    free_span.data_ptr(), batch, page_size, _error_word(device).data_ptr(),
-                                    _stream(lens))
-    check(rc, "tm_release_pages")
+    launch("tm_release_pages", device, lens.data_ptr(), done.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+           block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_span.data_ptr(), batch, page_size)
 
 
 def _page_bytes(page_size: int, head_dim: int) -> int:
@@ -172,13 +163,14 @@ def kv4_append(k: Tensor, v: Tensor, pool: Tensor, slots: Tensor) -> None:
     if not k.is_cuda:
         raise RuntimeError("the cache is written by a CUDA kernel")
     device = k.device
-    _raise_first((
-        (lambda: k.ndim != 3 or v.ndim != 3, ValueError("expected [tokens, kv_heads, head_dim] tensors")),
-        (lambda: v.shape != k.shape, ValueError("K and V shapes must match")),
-        (lambda: v.device != device, ValueError("all tensors of a call must share one CUDA device")),
-        (lambda: {k.dtype, v.dtype} != {torch.float16},
-         TypeError("the sm_100a cache kernels take fp16; k and v must be torch.float16")),
-    ))
+    if k.ndim != 3 or v.ndim != 3:
+        raise ValueError("expected [tokens, kv_heads, head_dim] tensors")
+    if v.shape != k.shape:
+        raise ValueError("K and V shapes must match")
+    if v.device != device:
+        raise ValueError("all tensors of a call must share one CUDA device")
+    if k.dtype != torch.float16 or v.dtype != torch.float16:
+        raise TypeError("the sm_100a cache kernels take fp16; k and v must be torch.float16")
     n, heads, d = k.shape
     page_size = _pool_page_size(pool, heads, d, device)
     _check_device_int("slots", slots, torch.int64, device)
@@ -186,11 +178,8 @@ def kv4_append(k: Tensor, v: Tensor, pool: Tensor, slots: Tensor) -> None:
         raise ValueError(f"{slots.numel()} slots for {n} tokens")
     if n and (k.stride(2) != 1 or v.stride(2) != 1):
         raise ValueError("the head dimension must be contiguous")
-    with on_device(device):
-        rc = lib().tm_kv4_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), n,
-                                 slots.data_ptr(), pool.data_ptr(), pool.shape[0], heads, d, page_size,
-                                 _error_word(device).data_ptr(), _stream(k))
-    check(rc, "tm_kv4_append")
+    launch("tm_kv4_append", device, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), n,
+           slots.data_ptr(), pool.data_ptr(), pool.shape[0], heads, d, page_size)
 
 
 def kv4_read(pool: Tensor, slots: Tensor, head_dim: int) -> tuple[Tensor, Tensor]:
@@ -203,10 +192,8 @@ def kv4_read(pool: Tensor, slots: Tensor, head_dim: int) -> tuple[Tensor, Tensor
     n, heads = slots.numel(), pool.shape[1]
     k = torch.empty((n, heads, head_dim), dtype=torch.float16, device=device)
     v = torch.empty_like(k)
-    with on_device(device):
-        rc = lib().tm_kv4_read(pool.data_ptr(), pool.shape[0], heads, head_dim, page_size, slots.data_ptr(), n,
-                               k.data_ptr(), v.data_ptr(), _error_word(device).data_ptr(), _stream(pool))
-    check(rc, "tm_kv4_read")
+    launch("tm_kv4_read", device, pool.data_ptr(), pool.shape[0], heads, head_dim, page_size, slots.data_ptr(), n,
+           k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -262,20 +249,26 @@ def kv4_attention(q: Tensor, pool: Tensor, block_table: Tensor, kv_lens: Tensor,
     if not 0 < scale < float("inf"):
         raise ValueError("sm_scale must be positive and finite")
     capacity = cols * page_size
-    bound = capacity if max_kv_len is None else min(int(max_kv_len), capacity)
-    p = TmKv4AttnParams(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), rows,
-                        pool.data_ptr(), pool.shape[0], block_table.data_ptr(), block_table.stride(0), cols,
-                        page_size, kv_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
-                        0 if key_mask is None else key_mask.data_ptr(),
-                        0 if key_mask is None else key_mask.stride(0),
-                        0 if key_mask is None else key_mask.shape[1],
-                        batch, heads, heads_k, d, max_seqlen_q, bound, bool(causal),
-                        scale, _error_word(device).data_ptr())
-    need = ctypes.c_int64()
-    check(lib().tm_kv4_attn_workspace(ctypes.byref(p), ctypes.byref(need)), "tm_kv4_attn")
+    bound = capacity if max_kv_len is None else min(max(int(max_kv_len), 0), capacity)
+    mask = (0, 0, 0) if key_mask is None else (key_mask.data_ptr(), key_mask.stride(0), key_mask.shape[1])
     # From the allocator on the call's own stream: two streams or graphs never share it.
-    work = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
-    with on_device(device):
-        rc = lib().tm_kv4_attn(ctypes.byref(p), 0 if work is None else work.data_ptr(), need.value, _stream(q))
-    check(rc, "tm_kv4_attn")
+    nbytes = _workspace_bytes(batch, rows, heads, heads_k, d, page_size, cols, max_seqlen_q, bound)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    launch("tm_kv4_attn", device,
+           _pack_attn(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), rows,
+                      pool.data_ptr(), pool.shape[0], block_table.data_ptr(), block_table.stride(0), cols, page_size,
+                      kv_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), *mask, batch, heads,
+                      heads_k, d, max_seqlen_q, bound, bool(causal), scale),
+           work.data_ptr(), nbytes)
     return out
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(batch: int, rows: int, heads: int, heads_k: int, d: int, page_size: int, cols: int,
+                     max_seqlen_q: int, bound: int) -> int:
+    """Workspace of an attention call; it depends on these sizes alone (stand-in pointers, never read)."""
+    at, need = 1 << 20, ctypes.c_int64()
+    args = _pack_attn(at, d, d, at, d, d, rows, at, 1, at, cols, cols, page_size, at, at, 0, 0, 0, batch, heads, heads_k,
+                      d, max_seqlen_q, bound, 1, 1.0)
+    check(lib().tm_kv4_attn_workspace(args, ctypes.byref(need)), "tm_kv4_attn")
+    return need.value

@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 
 #include "common.cuh"
+#include "kv4_layout.cuh"
 #include "tilemix_b200.h"
 
 namespace tilemix {
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const ReleaseArgs a) 
 }  // namespace tables
 }  // namespace tilemix
 
-extern "C" int tm_build_block_tables(const tm_block_tables_params* p, void* stream) {
+extern "C" int tm_build_block_tables(const tm_block_tables_params* p, int* error_flag, void* stream) {
   using namespace tilemix::tables;
   if (p == nullptr) return TM_ERR_NULL;
   if (p->batch < 0 || p->n_slots < 0 || p->cols < 0 || p->capacity < 0) return TM_ERR_SHAPE;
@@ -265,11 +266,9 @@ extern "C" int tm_build_block_tables(const tm_block_tables_params* p, void* stre
     return TM_ERR_UNSUPPORTED;  // other CTAs still read the inputs while the outputs are written
   Args a{p->cached_lens, p->new_lens,  p->block_table, p->table_stride, p->cols,        p->free_pages,
          p->capacity,    p->free_span, p->batch,       p->page_size,    p->n_slots,     p->slots,
-         p->positions,   p->cu_seqlens, p->kv_lens,    p->free_span_out, p->error_flag};
+         p->positions,   p->cu_seqlens, p->kv_lens,    p->free_span_out, error_flag};
   const size_t smem = 2 * sizeof(int32_t) * (static_cast<size_t>(p->batch) + 1);
-  if (cudaFuncSetAttribute(build_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           2 * sizeof(int32_t) * (kMaxBatch + 1)) != cudaSuccess)
-    return TM_ERR_LAUNCH;
+  if (!tilemix::allow_smem<build_kernel, 2 * 4 * (kMaxBatch + 1)>()) return TM_ERR_LAUNCH;
   // Two tokens a thread, at most one CTA an SM: below that the scan is the work, above it the stores.
   const int64_t want = (p->n_slots + 2 * kThreads - 1) / (2 * kThreads);
   const int grid = static_cast<int>(want < 1 ? 1 : want > 148 ? 148 : want);

@@ -510,8 +510,7 @@ template <int BN, bool kTokenLanes, typename OutT>
 static int launch(const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& g, cudaStream_t st) {
   using S = GemmShape<BN>;
   auto kernel = gemm_kernel<BN, kTokenLanes, OutT>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess)
-    return TM_ERR_LAUNCH;
+  if (!allow_smem<gemm_kernel<BN, kTokenLanes, OutT>, S::kSmem>()) return TM_ERR_LAUNCH;
   const int64_t tiles = static_cast<int64_t>(g.tiles_a) * g.tiles_b;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(g.split > 1 ? tiles * g.split : tiles < kSms ? tiles : kSms));
@@ -545,7 +544,8 @@ static int dispatch(const Plan& p, const CUtensorMap& a, const CUtensorMap& b, c
 }  // namespace tilemix
 
 extern "C" int tm_quant_per_token_int8(const void* x, int dtype, int64_t x_stride, int64_t rows, int cols, int8_t* out,
-                                       int64_t out_stride, float* scale, void* stream) {
+                                       int64_t out_stride, float* scale, int* error_flag, void* stream) {
+  (void)error_flag;  // nothing that only the device could see
   using namespace tilemix::linear;
   if (rows < 0 || cols <= 0) return TM_ERR_SHAPE;
   if (dtype != TM_DTYPE_FP16 && dtype != TM_DTYPE_BF16) return TM_ERR_UNSUPPORTED;
@@ -610,4 +610,16 @@ extern "C" int tm_int8_matmul(const int8_t* x8, int64_t x_stride, const float* x
   if (out_dtype == TM_DTYPE_FP16) return dispatch<__half>(p, ma, mb, g, st);
   if (out_dtype == TM_DTYPE_BF16) return dispatch<__nv_bfloat16>(p, ma, mb, g, st);
   return dispatch<float>(p, ma, mb, g, st);
+}
+
+extern "C" int tm_int8_linear(const void* x, int dtype, int64_t x_stride, int8_t* x8, int64_t x8_stride, float* x_scale,
+                              const int8_t* w8, int64_t w_stride, const float* w_scale, const void* bias, void* out,
+                              int64_t out_stride, int64_t tokens, int out_features, int in_features, int* error_flag,
+                              void* stream) {
+  if (dtype != TM_DTYPE_FP16 && dtype != TM_DTYPE_BF16) return TM_ERR_UNSUPPORTED;
+  const int rc = tm_quant_per_token_int8(x, dtype, x_stride, tokens, in_features, x8, x8_stride, x_scale, error_flag,
+                                         stream);
+  if (rc != TM_OK) return rc;
+  return tm_int8_matmul(x8, x8_stride, x_scale, w8, w_stride, w_scale, bias, out, out_stride, dtype, tokens,
+                        out_features, in_features, error_flag, stream);
 }

@@ -72,7 +72,7 @@ struct AttnArgs {
   int causal;
   float scale_log2;
   int ctas;            // CTAs that share the work
-  long long* starts;   // [batch + 1] first chunk of each request, written by CTA 0 for the join
+  int32_t* starts;     // [batch + 1] first chunk of each request, written by CTA 0 for the join
   float* part_o;       // [2 ctas][rows of a tile][D]
   float2* part_ml;     // [2 ctas][rows of a tile] (max in log2 units, sum)
   int* err;
@@ -204,8 +204,6 @@ __global__ void __launch_bounds__(kAttnThreads, resident(NT)) attn_kernel(const 
   extern __shared__ __align__(128) uint8_t smem[];
   float* sh_state = reinterpret_cast<float*>(smem + kAttnWarps * kStages * kStageBytes);  // [2][kState][32]
   __shared__ __align__(8) uint64_t bars[kAttnWarps][kStages];
-  __shared__ long long sh_part[kAttnWarps], sh_start;
-  __shared__ int sh_b;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up; it waits for our end
@@ -217,67 +215,59 @@ __global__ void __launch_bounds__(kAttnThreads, resident(NT)) attn_kernel(const 
     fence_mbarrier_init();
   }
 
-  // Where this CTA's chunks begin: a scan over the requests, a run of them a thread.
-  const int run = (a.batch + kAttnThreads - 1) / kAttnThreads;
-  const int rb0 = min(tid * run, a.batch), rb1 = min(rb0 + run, a.batch);
-  long long mine = 0;
+  // Where this CTA's chunks begin: every warp scans the requests for itself, a run of them a lane.
+  const int run = (a.batch + 31) / 32;
+  const int rb0 = min(lane * run, a.batch), rb1 = min(rb0 + run, a.batch);
+  int mine = 0;
   for (int b = rb0; b < rb1; ++b) {
     const Request r = request_of<NT>(a, b);
-    mine += static_cast<long long>(r.tiles) * a.heads_k * r.chunks;
-    if (blockIdx.x == 0 && r.kv < a.kv_lens[b]) record_error(a.err, kErrCachePlan);  // longer than it may be
+    mine += r.tiles * a.heads_k * r.chunks;
   }
-  long long inc = mine;
+  int inc = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+    const int v = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += v;
   }
-  if (lane == 31) sh_part[warp] = inc;
-  __syncthreads();
-  long long total = 0, before = inc - mine;
-#pragma unroll
-  for (int w = 0; w < kAttnWarps; ++w) {
-    if (w < warp) before += sh_part[w];
-    total += sh_part[w];
-  }
-  const long long per = (total + a.ctas - 1) / a.ctas;
-  long long pos = per * blockIdx.x;
-  const long long end = min(total, pos + per);
-  if (blockIdx.x == 0) {
-    long long at = before;
+  const int total = __shfl_sync(0xffffffffu, inc, 31);
+  const int per = (total + a.ctas - 1) / a.ctas;
+  int pos = per * static_cast<int>(blockIdx.x);
+  const int end = min(total, pos + per);
+  if (blockIdx.x == gridDim.x - 1 && warp == kAttnWarps - 1) {  // for the join; this CTA has the least to do
+    int at = inc - mine;
     for (int b = rb0; b < rb1; ++b) {
       a.starts[b] = at;
       const Request r = request_of<NT>(a, b);
-      at += static_cast<long long>(r.tiles) * a.heads_k * r.chunks;
+      at += r.tiles * a.heads_k * r.chunks;
+      if (r.kv < a.kv_lens[b]) record_error(a.err, kErrCachePlan);  // longer than it may be
     }
-    if (tid == 0) a.starts[a.batch] = total;
+    if (lane == 0) a.starts[a.batch] = total;
   }
   if (pos >= end) return;
-  if (before <= pos && pos < before + mine) {
-    long long at = before;
-    for (int b = rb0; b < rb1; ++b) {
+  int b = 0, b_start = 0;
+  const int owner = __ffs(__ballot_sync(0xffffffffu, inc > pos)) - 1;
+  if (lane == owner) {
+    b = rb0;
+    b_start = inc - mine;
+    while (true) {
       const Request r = request_of<NT>(a, b);
-      const long long n = static_cast<long long>(r.tiles) * a.heads_k * r.chunks;
-      if (pos < at + n) {
-        sh_b = b;
-        sh_start = at;
-        break;
-      }
-      at += n;
+      const int n = r.tiles * a.heads_k * r.chunks;
+      if (pos < b_start + n) break;
+      b_start += n;
+      ++b;
     }
   }
-  __syncthreads();
-  int b = sh_b;
-  long long b_start = sh_start;
+  b = __shfl_sync(0xffffffffu, b, owner);
+  b_start = __shfl_sync(0xffffffffu, b_start, owner);
   Request rq = request_of<NT>(a, b);
 
   // The current run of chunks: one (request, KV head, row tile), keys [key0, key1).
   int hk, row0, chunk0, n_chunks, key0, blk1, steps;
   auto locate = [&]() {
-    const int off = static_cast<int>(pos - b_start);
+    const int off = pos - b_start;
     const int unit = off / rq.chunks;
     chunk0 = off - unit * rq.chunks;
-    n_chunks = static_cast<int>(min(static_cast<long long>(rq.chunks - chunk0), end - pos));
+    n_chunks = min(rq.chunks - chunk0, end - pos);
     hk = unit / rq.tiles;
     row0 = (unit - hk * rq.tiles) * kRows;
     key0 = chunk0 * kChunkKeys;
@@ -324,9 +314,13 @@ __global__ void __launch_bounds__(kAttnThreads, resident(NT)) attn_kernel(const 
       uint8_t* dst = ring + in_stage * kStageBytes;
       uint64_t* full = &bar[in_stage];
       mbar_arrive_expect_tx(full, (kStepBlocks - __popc(bad)) * L::kBlockBytes);
+      if (bad == 0 && src[1] == src[0] + L::kBlockBytes) {
+        bulk_load(dst, src[0], kStageBytes, full);
+      } else {
 #pragma unroll
-      for (int u = 0; u < kStepBlocks; ++u)
-        if (src[u] != nullptr) bulk_load(dst + u * L::kBlockBytes, src[u], L::kBlockBytes, full);
+        for (int u = 0; u < kStepBlocks; ++u)
+          if (src[u] != nullptr) bulk_load(dst + u * L::kBlockBytes, src[u], L::kBlockBytes, full);
+      }
     }
     ++issued;
     ++all_issued;
@@ -419,8 +413,12 @@ __global__ void __launch_bounds__(kAttnThreads, resident(NT)) attn_kernel(const 
     const uint8_t* mask = a.mask != nullptr ? a.mask + b * a.mask_stride : nullptr;
 
     float o[NT][2 * G][4];
-    // Running maximum in units of the scores, the same in log2 units (0 while there is none), running sum.
-    float m[NT][2], mc[NT][2], l[NT][2];
+    // The reference that scores are taken against, in their units and in log2 units (-inf and 0 while there is
+    // none), and the running sum. The reference is a maximum that may lag: it moves only when a score is more
+    // than kLag log2 units above it (`limit`, in the scores' units), so a weight is at most 2^kLag, well inside
+    // fp16, and the output is seldom rescaled (with every new maximum it was in most of a warp's steps).
+    constexpr float kLag = 8.f;
+    float m[NT][2], mc[NT][2], limit[NT][2], l[NT][2];
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
 #pragma unroll
@@ -428,7 +426,7 @@ __global__ void __launch_bounds__(kAttnThreads, resident(NT)) attn_kernel(const 
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[x][i][c] = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) m[x][c] = -CUDART_INF_F, mc[x][c] = 0.f, l[x][c] = 0.f;
+      for (int c = 0; c < 2; ++c) m[x][c] = limit[x][c] = -CUDART_INF_F, mc[x][c] = 0.f, l[x][c] = 0.f;
     }
 
     // One step: 32 keys from stage s. With kPlain every key counts for every row.
@@ -490,9 +488,9 @@ __global__ void __launch_bounds__(kAttnThreads, resident(NT)) attn_kernel(const 
 #pragma unroll
           for (int u = 1; u < kStepBlocks; ++u) top = fmaxf(top, fmaxf(sc[u][x][c], sc[u][x][c + 2]));
           base[x][c] = top;
-          moved |= top > m[x][c];
+          moved |= top > limit[x][c];
         }
-      // The maxima are joined across the lanes only when some lane's own exceeds the running one.
+      // The maxima are joined across the lanes only when some lane's own is beyond the limit.
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
@@ -507,6 +505,7 @@ __global__ void __launch_bounds__(kAttnThreads, resident(NT)) attn_kernel(const 
             f[c] = m[x][c] == top ? 1.f : ex2_approx((m[x][c] - top) * cs[x][c]);
             m[x][c] = top;
             mc[x][c] = top == -CUDART_INF_F ? 0.f : top * cs[x][c];
+            limit[x][c] = top + kLag / cs[x][c];
             l[x][c] *= f[c];
           }
 #pragma unroll
@@ -608,8 +607,8 @@ __global__ void __launch_bounds__(kAttnThreads, resident(NT)) attn_kernel(const 
     pos += n_chunks;
     const bool more = pos < end;
     if (more) {
-      while (pos >= b_start + static_cast<long long>(rq.tiles) * a.heads_k * rq.chunks) {
-        b_start += static_cast<long long>(rq.tiles) * a.heads_k * rq.chunks;
+      while (pos >= b_start + rq.tiles * a.heads_k * rq.chunks) {
+        b_start += rq.tiles * a.heads_k * rq.chunks;
         rq = request_of<NT>(a, ++b);
       }
       locate();
@@ -717,9 +716,9 @@ __global__ void __launch_bounds__(kAttnThreads) join_kernel(const AttnArgs a) {
   const int hk = hq / a.group, row = token * a.group + hq - hk * a.group;
   const int tile = row / (8 * NT), r = row - tile * (8 * NT);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the attention kernel has ended, its writes are visible
-  const long long total = a.starts[a.batch], per = (total + a.ctas - 1) / a.ctas;
-  const long long first = a.starts[b] + (static_cast<long long>(hk) * rq.tiles + tile) * rq.chunks;
-  const int c0 = static_cast<int>(first / per), c1 = static_cast<int>((first + rq.chunks - 1) / per);
+  const int total = a.starts[a.batch], per = (total + a.ctas - 1) / a.ctas;
+  const int first = a.starts[b] + (hk * rq.tiles + tile) * rq.chunks;
+  const int c0 = first / per, c1 = (first + rq.chunks - 1) / per;
   if (c0 == c1) return;  // one CTA had it whole and wrote it
   auto slot = [&](int c) { return (2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * (8 * NT) + r; };
   // Each warp with a running maximum of its own, four parts in flight.
@@ -792,7 +791,7 @@ static Plan plan_of(const tm_kv4_attn_params* p) {
   const int64_t most = static_cast<int64_t>(p->batch) * p->heads_k * tiles;
   const int64_t slots = kSms * resident(r.nt);
   r.ctas = static_cast<int>(most >= slots || chunks >= slots || most * chunks >= slots ? slots : most * chunks);
-  r.starts_bytes = (static_cast<int64_t>(p->batch) + 2) / 2 * 16;
+  r.starts_bytes = (static_cast<int64_t>(p->batch) + 4) / 4 * 16;
   r.part_o_bytes = 2ll * r.ctas * 8 * r.nt * p->head_dim * 4;
   r.part_ml_bytes = 2ll * r.ctas * 8 * r.nt * 8;
   return r;
@@ -816,9 +815,9 @@ static int check(const tm_kv4_attn_params* p) {
   if (p->q_stride_tok % 8 || p->q_stride_head % 8 || p->o_stride_tok % 8 || p->o_stride_head % 8) return TM_ERR_ALIGN;
   if (p->key_mask != nullptr && p->mask_cols < 0) return TM_ERR_SHAPE;
   if (!(p->sm_scale > 0.f) || p->sm_scale > 3.4028235e38f) return TM_ERR_SHAPE;  // maxima are taken before scaling
-  // a request's chunks are counted in 32 bits
+  // the chunks of the work list are counted in 32 bits, with room for the last CTA's end
   const double rows = static_cast<double>(p->max_seqlen_q) * p->heads_q;
-  if ((rows / 8 + p->heads_k) * (p->max_kv_len / kChunkKeys + 1.0) > 2147483647.0) return TM_ERR_UNSUPPORTED;
+  if (p->batch * (rows / 8 + p->heads_k) * (p->max_kv_len / kChunkKeys + 1.0) > 2147480000.0) return TM_ERR_UNSUPPORTED;
   return TM_OK;
 }
 
@@ -826,10 +825,9 @@ template <int D, int NT>
 static cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
   constexpr int smem = kAttnWarps * kStages * kStepBlocks * Layout<D>::kBlockBytes +
                        kAttnWarps / 2 * NT * (8 * Layout<D>::kGroups + 4) * 32 * 4;
-  cudaError_t e = cudaFuncSetAttribute(attn_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
+  if (!allow_smem<attn_kernel<D, NT>, smem>()) return cudaErrorInvalidValue;
   attn_kernel<D, NT><<<a.ctas, kAttnThreads, smem, st>>>(a);
-  e = cudaGetLastError();
+  cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   // The join is set up while the attention runs (programmatic dependent launch) and waits for its end.
   cudaLaunchConfig_t cfg{};
@@ -858,7 +856,8 @@ extern "C" int tm_kv4_attn_workspace(const tm_kv4_attn_params* p, int64_t* bytes
   return TM_OK;
 }
 
-extern "C" int tm_kv4_attn(const tm_kv4_attn_params* p, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int tm_kv4_attn(const tm_kv4_attn_params* p, void* workspace, int64_t workspace_bytes, int* error_flag,
+                           void* stream) {
   using namespace tilemix::kv4;
   const int rc = check(p);
   if (rc != TM_OK || p->batch == 0 || p->q_tokens == 0 || p->max_seqlen_q == 0) return rc;
@@ -898,10 +897,10 @@ extern "C" int tm_kv4_attn(const tm_kv4_attn_params* p, void* workspace, int64_t
   a.scale_log2 = p->sm_scale * 1.4426950408889634f;
   a.ctas = r.ctas;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  a.starts = reinterpret_cast<long long*>(ws);
+  a.starts = reinterpret_cast<int32_t*>(ws);
   a.part_o = reinterpret_cast<float*>(ws + r.starts_bytes);
   a.part_ml = reinterpret_cast<float2*>(ws + r.starts_bytes + r.part_o_bytes);
-  a.err = p->error_flag;
+  a.err = error_flag;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (p->head_dim == 128)

@@ -21,7 +21,10 @@
 // and V of a block are adjacent: one bulk copy moves everything a step needs.
 #pragma once
 
+#include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <atomic>
 
 namespace tilemix {
 namespace kv4 {
@@ -46,4 +49,19 @@ inline bool aligned(const void* p, int64_t n) { return reinterpret_cast<uintptr_
 __host__ __device__ constexpr int block_bytes(int head_dim) { return 20 * head_dim; }
 
 }  // namespace kv4
+
+// Opt-in dynamic shared memory of a kernel: set once for each device that launches it.
+template <auto kKernel, int kBytes>
+inline bool allow_smem() {
+  static std::atomic<uint64_t> done{0};  // bit: device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return true;
+  if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess)
+    return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
+
 }  // namespace tilemix

@@ -19,16 +19,11 @@ from typing import Optional
 import torch
 from torch import Tensor, nn
 
-from tilemix_b200._lib import check, lib, on_device, TM_DTYPE_BF16, TM_DTYPE_FP16, TM_DTYPE_FP32
-from tilemix_b200.attention.tilemix import _error_word
+from tilemix_b200._lib import TM_DTYPE_BF16, TM_DTYPE_FP16, TM_DTYPE_FP32, launch
 
 __all__ = ["quantize_per_token_int8", "int8_matmul", "int8_linear", "Int8Linear"]
 
 _DTYPES = {torch.float16: TM_DTYPE_FP16, torch.bfloat16: TM_DTYPE_BF16, torch.float32: TM_DTYPE_FP32}
-
-
-def _stream(t: Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
 
 
 def quantize_per_token_int8(x: Tensor) -> tuple[Tensor, Tensor]:
@@ -45,10 +40,8 @@ def quantize_per_token_int8(x: Tensor) -> tuple[Tensor, Tensor]:
     rows, cols = x.shape
     codes = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    with on_device(x.device):
-        rc = lib().tm_quant_per_token_int8(x.data_ptr(), _DTYPES[x.dtype], x.stride(0), rows, cols, codes.data_ptr(),
-                                           codes.stride(0), scale.data_ptr(), _stream(x))
-    check(rc, "tm_quant_per_token_int8")
+    launch("tm_quant_per_token_int8", x.device, x.data_ptr(), _DTYPES[x.dtype], x.stride(0), rows, cols,
+           codes.data_ptr(), codes.stride(0), scale.data_ptr())
     return (codes if codes.shape[1] == cols else codes[:, :cols]), scale
 
 
@@ -85,15 +78,6 @@ def _check_bias(bias: Optional[Tensor], rows: int, dtype, device) -> None:
         raise ValueError("all tensors of a call must share one CUDA device")
 
 
-def _matmul(x8: Tensor, x_scale: Tensor, w8: Tensor, w_scale: Tensor, bias: Optional[Tensor], out: Tensor) -> None:
-    with on_device(x8.device):
-        rc = lib().tm_int8_matmul(x8.data_ptr(), x8.stride(0), x_scale.data_ptr(), w8.data_ptr(), w8.stride(0),
-                                  w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(),
-                                  out.stride(0), _DTYPES[out.dtype], x8.shape[0], w8.shape[0], x8.shape[1],
-                                  _error_word(x8.device).data_ptr(), _stream(x8))
-    check(rc, "tm_int8_matmul")
-
-
 def int8_matmul(x8: Tensor, x_scale: Tensor, w8: Tensor, w_scale: Tensor, bias: Optional[Tensor] = None, *,
                 out_dtype: torch.dtype = torch.float16) -> Tensor:
     """``(x8 . w8^T) * x_scale[:, None] * w_scale + bias`` as ``out_dtype`` (fp16, bf16 or fp32), for
@@ -112,7 +96,9 @@ def int8_matmul(x8: Tensor, x_scale: Tensor, w8: Tensor, w_scale: Tensor, bias: 
     _check_rows("x8", x8)
     _check_bias(bias, w8.shape[0], out_dtype, x8.device)
     out = torch.empty((x8.shape[0], w8.shape[0]), dtype=out_dtype, device=x8.device)
-    _matmul(x8, x_scale, w8, w_scale, bias, out)
+    launch("tm_int8_matmul", x8.device, x8.data_ptr(), x8.stride(0), x_scale.data_ptr(), w8.data_ptr(), w8.stride(0),
+           w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0),
+           _DTYPES[out_dtype], x8.shape[0], w8.shape[0], x8.shape[1])
     return out
 
 
@@ -123,15 +109,25 @@ def int8_linear(x: Tensor, w8: Tensor, w_scale: Tensor, bias: Optional[Tensor] =
         raise RuntimeError("the linear layer is a CUDA kernel")
     if x.ndim == 0:
         raise ValueError("expected [..., in_features]")
-    _check_weight(w8, w_scale, x.shape[-1], x.device)
-    _check_bias(bias, w8.shape[0], x.dtype, x.device)
-    rows = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
-    if rows.stride(1) != 1 and rows.shape[1] > 1:
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("the per-token quantiser takes fp16 or bf16")
+    device, dtype, k = x.device, x.dtype, x.shape[-1]
+    _check_weight(w8, w_scale, k, device)
+    n = w8.shape[0]
+    _check_bias(bias, n, dtype, device)
+    rows = x if x.ndim == 2 else x.reshape(-1, k)
+    if rows.stride(1) != 1 and k > 1:
         rows = rows.contiguous()
-    x8, x_scale = quantize_per_token_int8(rows)
-    out = torch.empty((rows.shape[0], w8.shape[0]), dtype=x.dtype, device=x.device)
-    _matmul(x8, x_scale, w8, w_scale, bias, out)
-    return out if x.ndim == 2 else out.view(*x.shape[:-1], w8.shape[0])
+    m = rows.shape[0]
+    out = torch.empty((m, n), dtype=dtype, device=device)
+    # One piece of scratch: the codes, their rows on 16 bytes, and behind them the scales.
+    wide = (k + 15) // 16 * 16
+    scratch = torch.empty(m * (wide + 4), dtype=torch.int8, device=device)
+    codes = scratch.data_ptr()
+    launch("tm_int8_linear", device, rows.data_ptr(), _DTYPES[dtype], rows.stride(0), codes, wide, codes + m * wide,
+           w8.data_ptr(), w8.stride(0), w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), n,
+           m, n, k)
+    return out if x.ndim == 2 else out.view(*x.shape[:-1], n)
 
 
 class Int8Linear(nn.Module):

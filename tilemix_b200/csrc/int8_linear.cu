@@ -12,6 +12,8 @@
 #include <cuda_fp16.h>
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kv4_layout.cuh"
 #include "tilemix_b200.h"
@@ -27,8 +29,6 @@ using kv4::aligned;
 // ----------------------------------------------------------------------------
 // Quantiser
 // ----------------------------------------------------------------------------
-constexpr int kQuantThreads = 256;
-
 template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <>
@@ -90,23 +90,25 @@ __device__ __forceinline__ uint2 codes8(const uint4& v, const RowScale& s) {
   return make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
 }
 
+template <int kThreads>
 __device__ __forceinline__ float block_max(float m) {
-  __shared__ float red[kQuantThreads / 32];
+  __shared__ float red[kThreads / 32];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
   __syncthreads();
-  m = red[0];
+  m = red[threadIdx.x % (kThreads / 32)];
 #pragma unroll
-  for (int i = 1; i < kQuantThreads / 32; ++i) m = max_nan(m, red[i]);
+  for (int o = kThreads / 64; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   return m;
 }
 
 // One CTA a row, the row held in registers between the two uses (kVec 16-byte pieces a thread; 0: any length,
 // read twice). A row with an infinity or a NaN gets that scale and codes 0, so that its outputs are NaN.
-template <typename T, int kVec>
-__global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const T* x, int64_t x_stride, int cols, int8_t* out,
-                                                                  int64_t out_stride, float* scale) {
+template <typename T, int kVec, int kThreads>
+__global__ void __launch_bounds__(kThreads) quant_rows_kernel(const T* x, int64_t x_stride, int cols, int8_t* out,
+                                                             int64_t out_stride, float* scale) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product that follows may load its weights
   const T* row = x + blockIdx.x * x_stride;
   int8_t* dst = out + blockIdx.x * out_stride;
   float m = 0.f;
@@ -114,7 +116,7 @@ __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const T* x, i
     uint4 v[kVec];
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-      const int c = (i * kQuantThreads + threadIdx.x) * 8;
+      const int c = (i * kThreads + threadIdx.x) * 8;
       v[i] = c < cols ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
       const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
@@ -123,40 +125,51 @@ __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const T* x, i
         m = max_nan(m, max_nan(fabsf(f.x), fabsf(f.y)));
       }
     }
-    m = block_max(m);
+    m = block_max<kThreads>(m);
     const RowScale s = row_scale(m);
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-      const int c = (i * kQuantThreads + threadIdx.x) * 8;
+      const int c = (i * kThreads + threadIdx.x) * 8;
       if (c < cols) *reinterpret_cast<uint2*>(dst + c) = s.ok ? codes8<T>(v[i], s) : make_uint2(0, 0);
     }
   } else {
-    for (int c = threadIdx.x; c < cols; c += kQuantThreads) m = max_nan(m, fabsf(to_float(row[c])));
-    m = block_max(m);
+    for (int c = threadIdx.x; c < cols; c += kThreads) m = max_nan(m, fabsf(to_float(row[c])));
+    m = block_max<kThreads>(m);
     const RowScale s = row_scale(m);
-    for (int c = threadIdx.x; c < cols; c += kQuantThreads)
+    for (int c = threadIdx.x; c < cols; c += kThreads)
       dst[c] = s.ok ? static_cast<int8_t>(code_of(to_float(row[c]), s)) : int8_t(0);
   }
   if (threadIdx.x == 0) scale[blockIdx.x] = __fdiv_rn(m, 127.f);
 }
 
+template <typename T, int kVec, int kThreads>
+static void run_quant(const T* x, int64_t xs, unsigned rows, int cols, int8_t* out, int64_t os, float* scale,
+                      cudaStream_t st) {
+  quant_rows_kernel<T, kVec, kThreads><<<rows, kThreads, 0, st>>>(x, xs, cols, out, os, scale);
+}
+
+// 1024 threads a row where there are fewer rows than SMs to fill or the row is long (64 rows of 18944: 11 us with
+// 256 threads that read it twice, 4 us so), 256 where rows are many (a CTA's reduction then hides behind the others).
 template <typename T>
 static void launch_quant(const void* x, int64_t xs, int64_t rows, int cols, int8_t* out, int64_t os, float* scale,
                          cudaStream_t st) {
   const T* p = static_cast<const T*>(x);
   const unsigned g = static_cast<unsigned>(rows);
-  const int pieces = (cols + kQuantThreads * 8 - 1) / (kQuantThreads * 8);
   const bool vec = cols % 8 == 0 && aligned(x, 16) && xs % 8 == 0 && aligned(out, 8) && os % 8 == 0;
-  if (!vec || pieces > 8)
-    quant_rows_kernel<T, 0><<<g, kQuantThreads, 0, st>>>(p, xs, cols, out, os, scale);
-  else if (pieces <= 1)
-    quant_rows_kernel<T, 1><<<g, kQuantThreads, 0, st>>>(p, xs, cols, out, os, scale);
-  else if (pieces <= 2)
-    quant_rows_kernel<T, 2><<<g, kQuantThreads, 0, st>>>(p, xs, cols, out, os, scale);
-  else if (pieces <= 4)
-    quant_rows_kernel<T, 4><<<g, kQuantThreads, 0, st>>>(p, xs, cols, out, os, scale);
+  if (!vec || cols > 32768)
+    run_quant<T, 0, 1024>(p, xs, g, cols, out, os, scale, st);
+  else if (cols <= 2048)
+    run_quant<T, 1, 256>(p, xs, g, cols, out, os, scale, st);
+  else if (cols > 16384)
+    run_quant<T, 4, 1024>(p, xs, g, cols, out, os, scale, st);
+  else if (cols > 8192)
+    run_quant<T, 2, 1024>(p, xs, g, cols, out, os, scale, st);
+  else if (rows < 148)
+    run_quant<T, 1, 1024>(p, xs, g, cols, out, os, scale, st);
+  else if (cols <= 4096)
+    run_quant<T, 2, 256>(p, xs, g, cols, out, os, scale, st);
   else
-    quant_rows_kernel<T, 8><<<g, kQuantThreads, 0, st>>>(p, xs, cols, out, os, scale);
+    run_quant<T, 4, 256>(p, xs, g, cols, out, os, scale, st);
 }
 
 // ----------------------------------------------------------------------------
@@ -184,6 +197,9 @@ struct GemmArgs {
   void* out;             // [tokens, channels], row stride ldo
   int64_t ldo;
   int vec;  // rows of `out` take 16-byte stores
+  // Launched beside the quantiser that makes x8 and its scales (programmatic dependent launch): what the kernels
+  // before that one wrote, the weights among it, is there already. Without it everything before is waited for.
+  int beside;
   int* err;
 };
 
@@ -229,56 +245,118 @@ template <int BN>
 struct GemmShape {
   static constexpr int kStageBytes = (kBM + BN) * kBK;
   // Wide tiles: as many stages as fit. Narrow ones: two CTAs an SM, so that a split's CTAs are all resident.
-  static constexpr int kStages = BN >= 256 ? 4 : BN >= 128 ? 6 : BN >= 64 ? 4 : 5;
-  static constexpr int kSmem = kStages * kStageBytes + 1024;
+  static constexpr int kStages = BN >= 256 ? 4 : BN >= 128 ? 5 : BN >= 64 ? 4 : 5;
+  // behind the ring: scales and biases of the columns of two tiles, and with the tokens on the lanes a
+  // 4 KB piece of output for each epilogue warp
+  static constexpr int kOffCols = kStages * kStageBytes;
+  static constexpr int kOffPieces = kOffCols + 2 * 2 * BN * 4;
+  static constexpr int smem(bool token_lanes) { return kOffPieces + (token_lanes ? 4 * 4096 : 0) + 1024; }
   static constexpr int kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
 };
 
-// Scales, bias and store of kCols consecutive columns of this lane's row.
+// y = sum * token scale * channel scale + bias, the token's scale first on either side, so that every launch
+// shape gives the same bits.
+__device__ __forceinline__ float scaled(uint32_t acc, float token, float channel, float bias) {
+  return fmaf(static_cast<float>(static_cast<int32_t>(acc)) * token, channel, bias);
+}
+
+// kCols consecutive columns of this lane's row, stored one by one; col_scale / col_bias: of those columns.
 template <int kCols, bool kTokenLanes, typename OutT>
-__device__ __forceinline__ void emit(const uint32_t* acc, const GemmArgs& g, int a, int b0) {
+__device__ __forceinline__ void emit(const uint32_t* acc, const GemmArgs& g, int a, int b0, float row_scale,
+                                     float row_bias, const float* col_scale, const float* col_bias) {
   if (a >= g.rows_a) return;
   OutT* out = static_cast<OutT*>(g.out);
-  const OutT* bias = static_cast<const OutT*>(g.bias);
-  const float sa = __ldg(g.scale_a + a);
-  if constexpr (kTokenLanes) {
-    OutT* row = out + a * g.ldo;
-    float v[kCols];
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-      const int b = min(b0 + c, g.rows_b - 1);
-      v[c] = static_cast<float>(static_cast<int32_t>(acc[c])) * sa * __ldg(g.scale_b + b);
-      if (bias != nullptr) v[c] += load_one(bias + b);
+  for (int c = 0; c < kCols; ++c) {
+    const int b = b0 + c;
+    if (b >= g.rows_b) break;
+    if (kTokenLanes)
+      store_one(out + a * g.ldo + b, scaled(acc[c], row_scale, col_scale[c], col_bias[c]));
+    else
+      store_one(out + b * g.ldo + a, scaled(acc[c], col_scale[c], row_scale, row_bias));
+  }
+}
+
+// With the tokens on the lanes: 128 bytes of each of a warp's 32 rows through shared memory, so that they are
+// stored as whole lines (a lane's own row would be 32 separate ones a store). 16-byte pieces are swizzled by
+// the row against bank conflicts.
+template <typename OutT>
+__device__ __forceinline__ void emit_rows(uint32_t taddr, uint8_t* piece, const GemmArgs& g, int a0, int b0,
+                                          float row_scale, const float* col_scale, const float* col_bias) {
+  constexpr int kCols = 128 / sizeof(OutT), kPer = 16 / sizeof(OutT);
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int h = 0; h < kCols / 32; ++h) {
+    uint32_t r[32];
+    tmem_ld32(taddr + 32 * h, r);
+    tmem_wait_ld();
+#pragma unroll
+    for (int c = 0; c < 32; c += kPer) {
+      float v[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; i += 4) {
+        const float4 cs = *reinterpret_cast<const float4*>(col_scale + 32 * h + c + i);
+        const float4 cb = *reinterpret_cast<const float4*>(col_bias + 32 * h + c + i);
+        v[i] = scaled(r[c + i], row_scale, cs.x, cb.x);
+        v[i + 1] = scaled(r[c + i + 1], row_scale, cs.y, cb.y);
+        v[i + 2] = scaled(r[c + i + 2], row_scale, cs.z, cb.z);
+        v[i + 3] = scaled(r[c + i + 3], row_scale, cs.w, cb.w);
+      }
+      const int chunk = (32 * h + c) / kPer;
+      uint4 w;
+      if constexpr (sizeof(OutT) == 2)
+        w = make_uint4(pack2(static_cast<const OutT*>(nullptr), v[0], v[1]),
+                       pack2(static_cast<const OutT*>(nullptr), v[2], v[3]),
+                       pack2(static_cast<const OutT*>(nullptr), v[4], v[5]),
+                       pack2(static_cast<const OutT*>(nullptr), v[6], v[7]));
+      else
+        w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      *reinterpret_cast<uint4*>(piece + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = w;
     }
-    if constexpr (sizeof(OutT) == 2) {
-      if (g.vec && b0 + kCols <= g.rows_b) {
+  }
+  __syncwarp();
+  OutT* out = static_cast<OutT*>(g.out);
+  const int chunk = lane & 7, b = b0 + chunk * kPer;
 #pragma unroll
-        for (int c = 0; c + 8 <= kCols; c += 8)
-          *reinterpret_cast<uint4*>(row + b0 + c) =
-              make_uint4(pack2(out, v[c], v[c + 1]), pack2(out, v[c + 2], v[c + 3]), pack2(out, v[c + 4], v[c + 5]),
-                         pack2(out, v[c + 6], v[c + 7]));
-        if constexpr (kCols % 8 != 0) {
+  for (int i = 0; i < 8; ++i) {
+    const int row = 4 * i + (lane >> 3);
+    if (a0 + row < g.rows_a && b < g.rows_b) {
+      const uint4 w = *reinterpret_cast<const uint4*>(piece + row * 128 + ((chunk ^ (row & 7)) << 4));
+      OutT* dst = out + static_cast<int64_t>(a0 + row) * g.ldo + b;
+      if (g.vec && b + kPer <= g.rows_b) {
+        *reinterpret_cast<uint4*>(dst) = w;
+      } else {
+        const OutT* e = reinterpret_cast<const OutT*>(&w);
 #pragma unroll
-          for (int c = kCols / 8 * 8; c < kCols; ++c) store_one(row + b0 + c, v[c]);
-        }
-        return;
+        for (int k = 0; k < kPer; ++k)
+          if (b + k < g.rows_b) dst[k] = e[k];
       }
     }
+  }
+  __syncwarp();
+}
+
+// The sum over the cluster of kSplit partial tiles of this rank's columns; all loads of a column are in flight
+// together.
+template <int kSplit, int BN, bool kTokenLanes, typename OutT>
+__device__ __forceinline__ void reduce_split(uint32_t red, const GemmArgs& g, int a, int b0, int rank, float row_scale,
+                                             float row_bias, const float* col_scale, const float* col_bias) {
+  constexpr int kCols = BN / kSplit, kStep = kCols < 4 ? kCols : 4;
+  for (int c = rank * kCols; c < (rank + 1) * kCols; c += kStep) {
+    int32_t part[kSplit][kStep];
 #pragma unroll
-    for (int c = 0; c < kCols; ++c)
-      if (b0 + c < g.rows_b) store_one(row + b0 + c, v[c]);
-  } else {
-    const float bv = bias != nullptr ? load_one(bias + a) : 0.f;
+    for (int p = 0; p < kSplit; ++p)
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-      const int b = b0 + c;
-      if (b < g.rows_b) {
-        // the token's scale first, as with the tokens on the lanes
-        float v = static_cast<float>(static_cast<int32_t>(acc[c])) * __ldg(g.scale_b + b) * sa;
-        if (bias != nullptr) v += bv;
-        store_one(out + b * g.ldo + a, v);
-      }
+      for (int i = 0; i < kStep; ++i) part[p][i] = ld_cluster(red + (c + i) * (kBM * 4), p);
+    uint32_t sum[kStep];
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) {
+      int32_t v = part[0][i];
+#pragma unroll
+      for (int p = 1; p < kSplit; ++p) v += part[p][i];
+      sum[i] = static_cast<uint32_t>(v);
     }
+    emit<kStep, kTokenLanes, OutT>(sum, g, a, b0 + c, row_scale, row_bias, col_scale + c, col_bias + c);
   }
 }
 
@@ -330,21 +408,41 @@ __global__ void __launch_bounds__(kGemmThreads) gemm_kernel(const __grid_constan
   };
 
   bool ok = true;
+  float row_scale = 0.f, row_bias = 0.f;
   if (warp == 0) {
-    int s = 0, used = 0;
+    // The weights do not depend on the kernel before (the quantiser, when this one was launched beside it): those
+    // of the first stages are under way before its end is waited for.
+    int s = 0, used = 0, early = 0;
     uint32_t phase = 0;
+    if (first_tile < tiles) {
+      int ta, tb;
+      tile_at(first_tile, &ta, &tb);
+      early = min(S::kStages, k1 - k0);
+      for (int i = 0; i < early; ++i) {
+        uint8_t* st = smem + i * S::kStageBytes;
+        mbar_arrive_expect_tx_e(&full[i], S::kStageBytes);
+        if (kTokenLanes)
+          tma_load_2d_e(st + kBM * kBK, &map_b, &full[i], (k0 + i) * kBK, tb * BN);
+        else
+          tma_load_2d_e(st, &map_a, &full[i], (k0 + i) * kBK, ta * kBM);
+      }
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int t = first_tile; t < tiles && ok; t += tile_step) {
       int ta, tb;
       tile_at(t, &ta, &tb);
       for (int k = k0; k < k1; ++k) {
-        if (!mbar_wait_spin(&empty[s], phase ^ 1, g.err, kErrTimeoutEmpty)) {
-          ok = false;
-          break;
-        }
         uint8_t* st = smem + s * S::kStageBytes;
-        mbar_arrive_expect_tx_e(&full[s], S::kStageBytes);
-        tma_load_2d_e(st, &map_a, &full[s], k * kBK, ta * kBM);
-        tma_load_2d_e(st + kBM * kBK, &map_b, &full[s], k * kBK, tb * BN);
+        const bool half = used < early;  // its weights are under way
+        if (!half) {
+          if (!mbar_wait_spin(&empty[s], phase ^ 1, g.err, kErrTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx_e(&full[s], S::kStageBytes);
+        }
+        if (!half || kTokenLanes) tma_load_2d_e(st, &map_a, &full[s], k * kBK, ta * kBM);
+        if (!half || !kTokenLanes) tma_load_2d_e(st + kBM * kBK, &map_b, &full[s], k * kBK, tb * BN);
         ++used;
         if (++s == S::kStages) s = 0, phase ^= 1;
       }
@@ -394,33 +492,49 @@ __global__ void __launch_bounds__(kGemmThreads) gemm_kernel(const __grid_constan
       mbar_wait(&drain, 0, g.err, kErrTimeoutDrain);
     }
   } else if (warp >= 4) {
-    const int quad = warp & 3;
+    const int quad = warp & 3, et = threadIdx.x - 128;
+    float* cols = reinterpret_cast<float*>(smem + S::kOffCols);  // [2][scales BN, biases BN]
+    uint8_t* piece = smem + S::kOffPieces + quad * 4096;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the tokens' scales
     int n = 0;
     for (int t = first_tile; t < tiles; t += tile_step, ++n) {
       const int acc = n & 1;
-      if (!mbar_wait_spin(&acc_full[acc], (n >> 1) & 1, g.err, kErrTimeoutScores)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const uint32_t d = tmem + acc * BN + (static_cast<uint32_t>(quad * 32) << 16);
       int ta, tb;
       tile_at(t, &ta, &tb);
       const int a = ta * kBM + quad * 32 + lane;
+      // Scales and biases under the products: the columns' in shared memory (of two tiles in turn: the barrier
+      // below keeps the four warps within one tile of another), the lane's row's in registers.
+      float* col_scale = cols + acc * 2 * BN;
+      float* col_bias = col_scale + BN;
+      for (int c = et; c < BN; c += 128) {
+        const int b = tb * BN + c;
+        const bool in = b < g.rows_b;
+        col_scale[c] = in ? g.scale_b[b] : 0.f;
+        col_bias[c] = kTokenLanes && in && g.bias != nullptr ? load_one(static_cast<const OutT*>(g.bias) + b) : 0.f;
+      }
+      row_scale = a < g.rows_a ? g.scale_a[a] : 0.f;
+      row_bias =
+          !kTokenLanes && a < g.rows_a && g.bias != nullptr ? load_one(static_cast<const OutT*>(g.bias) + a) : 0.f;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      // After a wait that ran out a warp only keeps the barrier's count.
+      if (ok && !mbar_wait_spin(&acc_full[acc], (n >> 1) & 1, g.err, kErrTimeoutScores)) ok = false;
+      if (!ok) continue;
+      tc_fence_after();
+      const uint32_t d = tmem + acc * BN + (static_cast<uint32_t>(quad * 32) << 16);
       if (g.split == 1) {
-        if constexpr (BN >= 32) {
+        if constexpr (kTokenLanes) {
+          constexpr int kCols = 128 / sizeof(OutT);
 #pragma unroll 1
-          for (int c = 0; c < BN; c += 32) {
-            uint32_t r[32];
-            tmem_ld32(d + c, r);
-            tmem_wait_ld();
-            emit<32, kTokenLanes, OutT>(r, g, a, tb * BN + c);
-          }
+          for (int c = 0; c < BN; c += kCols)
+            emit_rows<OutT>(d + c, piece, g, ta * kBM + quad * 32, tb * BN + c, row_scale, col_scale + c, col_bias + c);
         } else {
-          uint32_t r[16];
-          tmem_ld16(d, r);
-          tmem_wait_ld();
-          emit<16, kTokenLanes, OutT>(r, g, a, tb * BN);
+#pragma unroll 1
+          for (int c = 0; c < BN; c += 16) {
+            uint32_t r[16];
+            tmem_ld16(d + c, r);
+            tmem_wait_ld();
+            emit<16, kTokenLanes, OutT>(r, g, a, tb * BN + c, row_scale, row_bias, col_scale + c, col_bias + c);
+          }
         }
       } else {
         // this part's partial tile, column by column (a warp's 32 lanes are 128 consecutive bytes); every
@@ -447,18 +561,19 @@ __global__ void __launch_bounds__(kGemmThreads) gemm_kernel(const __grid_constan
     if (warp >= 4 && ok) {
       int ta, tb;
       tile_at(first_tile, &ta, &tb);
-      const int quad = warp & 3, cols = BN / g.split;
-      const int a = ta * kBM + quad * 32 + lane;
-      const uint32_t base = smem_u32(smem) + (quad * 32 + lane) * 4;
-      for (int c = rank * cols; c < (rank + 1) * cols; c += 2) {
-        int32_t sum[2] = {0, 0};
-        for (int p = 0; p < g.split; ++p) {
-          sum[0] += ld_cluster(base + c * (kBM * 4), p);
-          sum[1] += ld_cluster(base + (c + 1) * (kBM * 4), p);
-        }
-        const uint32_t u[2] = {static_cast<uint32_t>(sum[0]), static_cast<uint32_t>(sum[1])};
-        emit<2, kTokenLanes, OutT>(u, g, a, tb * BN + c);
-      }
+      const int row = (warp & 3) * 32 + lane;
+      const uint32_t red = smem_u32(smem) + row * 4;
+      const float* col_scale = reinterpret_cast<const float*>(smem + S::kOffCols);
+      auto reduce = [&](auto parts) {
+        reduce_split<decltype(parts)::value, BN, kTokenLanes, OutT>(red, g, ta * kBM + row, tb * BN, rank, row_scale,
+                                                                    row_bias, col_scale, col_scale + BN);
+      };
+      if (g.split == 2)
+        reduce(std::integral_constant<int, 2>{});
+      else if (g.split == 4)
+        reduce(std::integral_constant<int, 4>{});
+      else
+        reduce(std::integral_constant<int, 8>{});
     }
     __syncwarp();
     cluster_sync();  // nobody leaves while its partial tile is read
@@ -510,20 +625,29 @@ template <int BN, bool kTokenLanes, typename OutT>
 static int launch(const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& g, cudaStream_t st) {
   using S = GemmShape<BN>;
   auto kernel = gemm_kernel<BN, kTokenLanes, OutT>;
-  if (!allow_smem<gemm_kernel<BN, kTokenLanes, OutT>, S::kSmem>()) return TM_ERR_LAUNCH;
+  if (!allow_smem<gemm_kernel<BN, kTokenLanes, OutT>, S::smem(kTokenLanes)>()) return TM_ERR_LAUNCH;
   const int64_t tiles = static_cast<int64_t>(g.tiles_a) * g.tiles_b;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(g.split > 1 ? tiles * g.split : tiles < kSms ? tiles : kSms));
   cfg.blockDim = dim3(kGemmThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.dynamicSmemBytes = S::smem(kTokenLanes);
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = static_cast<unsigned>(g.split);
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (g.split > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = static_cast<unsigned>(g.split);
+    at[n].val.clusterDim.y = 1;
+    at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (g.beside) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = g.split > 1 ? 1 : 0;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, a, b, g) == cudaSuccess ? TM_OK : TM_ERR_LAUNCH;
 }
 
@@ -561,11 +685,11 @@ extern "C" int tm_quant_per_token_int8(const void* x, int dtype, int64_t x_strid
   return cudaGetLastError() == cudaSuccess ? TM_OK : TM_ERR_LAUNCH;
 }
 
-extern "C" int tm_int8_matmul(const int8_t* x8, int64_t x_stride, const float* x_scale, const int8_t* w8,
-                              int64_t w_stride, const float* w_scale, const void* bias, void* out, int64_t out_stride,
-                              int out_dtype, int64_t tokens, int out_features, int in_features, int* error_flag,
-                              void* stream) {
-  using namespace tilemix::linear;
+namespace tilemix {
+namespace linear {
+static int matmul(const int8_t* x8, int64_t x_stride, const float* x_scale, const int8_t* w8, int64_t w_stride,
+                  const float* w_scale, const void* bias, void* out, int64_t out_stride, int out_dtype, int64_t tokens,
+                  int out_features, int in_features, bool beside, int* error_flag, void* stream) {
   if (tokens < 0 || out_features <= 0 || in_features <= 0) return TM_ERR_SHAPE;
   if (out_dtype < TM_DTYPE_FP16 || out_dtype > TM_DTYPE_FP32) return TM_ERR_UNSUPPORTED;
   // int32 sums of in_features products of at most 127 * 127 (128 * 128, should a caller bring -128)
@@ -597,7 +721,8 @@ extern "C" int tm_int8_matmul(const int8_t* x8, int64_t x_stride, const float* x
   g.bias = bias;
   g.out = out;
   g.ldo = out_stride;
-  g.vec = es == 2 && aligned(out, 16) && out_stride % 8 == 0;
+  g.vec = aligned(out, 16) && out_stride * es % 16 == 0;
+  g.beside = beside;
   g.err = error_flag;
   CUtensorMap mx, mw;
   int rc = make_map(&mx, x8, tokens, in_features, x_stride, p.token_lanes ? kBM : p.bn);
@@ -611,6 +736,16 @@ extern "C" int tm_int8_matmul(const int8_t* x8, int64_t x_stride, const float* x
   if (out_dtype == TM_DTYPE_BF16) return dispatch<__nv_bfloat16>(p, ma, mb, g, st);
   return dispatch<float>(p, ma, mb, g, st);
 }
+}  // namespace linear
+}  // namespace tilemix
+
+extern "C" int tm_int8_matmul(const int8_t* x8, int64_t x_stride, const float* x_scale, const int8_t* w8,
+                              int64_t w_stride, const float* w_scale, const void* bias, void* out, int64_t out_stride,
+                              int out_dtype, int64_t tokens, int out_features, int in_features, int* error_flag,
+                              void* stream) {
+  return tilemix::linear::matmul(x8, x_stride, x_scale, w8, w_stride, w_scale, bias, out, out_stride, out_dtype, tokens,
+                                 out_features, in_features, false, error_flag, stream);
+}
 
 extern "C" int tm_int8_linear(const void* x, int dtype, int64_t x_stride, int8_t* x8, int64_t x8_stride, float* x_scale,
                               const int8_t* w8, int64_t w_stride, const float* w_scale, const void* bias, void* out,
@@ -620,6 +755,6 @@ extern "C" int tm_int8_linear(const void* x, int dtype, int64_t x_stride, int8_t
   const int rc = tm_quant_per_token_int8(x, dtype, x_stride, tokens, in_features, x8, x8_stride, x_scale, error_flag,
                                          stream);
   if (rc != TM_OK) return rc;
-  return tm_int8_matmul(x8, x8_stride, x_scale, w8, w_stride, w_scale, bias, out, out_stride, dtype, tokens,
-                        out_features, in_features, error_flag, stream);
+  return tilemix::linear::matmul(x8, x8_stride, x_scale, w8, w_stride, w_scale, bias, out, out_stride, dtype, tokens,
+                                 out_features, in_features, true, error_flag, stream);
 }

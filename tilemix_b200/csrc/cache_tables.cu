@@ -28,6 +28,7 @@ namespace tables {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxBatch = 8192;
+constexpr int kFew = 16;  // new tokens a request that a thread fills in by itself
 
 struct Args {
   const int32_t* cached;
@@ -45,6 +46,7 @@ struct Args {
   int32_t* cu;
   int32_t* kv_lens;
   int64_t* span_out;
+  int vec;  // slots and positions take 16-byte stores
   int* err;
 };
 
@@ -61,14 +63,17 @@ __device__ __forceinline__ int owner(const int32_t* start, int n, int32_t i) {
   return lo;
 }
 
+// kRun: consecutive tokens a thread fills in. 4 where stores are the work (mostly of one request and one page:
+// one lookup, whole 16-byte stores), 1 where the chain of lookups is.
+template <int kRun>
 __global__ void __launch_bounds__(kThreads) build_kernel(const Args a) {
   extern __shared__ int32_t sh[];
   int32_t* s_cu = sh;                     // [batch + 1] token offsets
   int32_t* s_first = sh + a.batch + 1;    // [batch + 1] page offsets
   __shared__ long long part_tok[kWarps], part_page[kWarps];
-  __shared__ int bad;
+  __shared__ int bad, crowded;  // some length is impossible; some request has many new tokens
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == 0) bad = 0;
+  if (tid == 0) bad = crowded = 0;
   __syncthreads();
 
   // Exclusive scan of (n_b, need_b): each thread owns a run of requests. Sums in 64 bits, so that
@@ -76,8 +81,9 @@ __global__ void __launch_bounds__(kThreads) build_kernel(const Args a) {
   const int per = (a.batch + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
   const long long most = static_cast<long long>(a.cols) * a.page;
+  const long long head = a.span[0], tail = a.span[1];
   long long tok = 0, pages = 0;
-  bool mine_bad = false;
+  bool mine_bad = false, many = false;
   for (int b = b0; b < b1; ++b) {
     const long long c = a.cached[b], n = a.fresh[b];
     if (c < 0 || n < 0 || c + n > most || c + n > 0x7fffffffll) {
@@ -86,8 +92,10 @@ __global__ void __launch_bounds__(kThreads) build_kernel(const Args a) {
     }
     tok += n;
     pages += (c + n + a.page - 1) / a.page - (c + a.page - 1) / a.page;
+    many |= n > kFew;
   }
   if (mine_bad) bad = 1;
+  if (many) crowded = 1;
   long long inc_tok = tok, inc_page = pages;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -112,7 +120,6 @@ __global__ void __launch_bounds__(kThreads) build_kernel(const Args a) {
     all_tok += part_tok[w];
     all_page += part_page[w];
   }
-  const long long head = a.span[0], tail = a.span[1];
   const bool fail = bad != 0 || head < 0 || tail < head || tail - head > a.capacity || all_page > tail - head ||
                     all_tok > a.n_slots;
   if (!fail) {
@@ -146,7 +153,10 @@ __global__ void __launch_bounds__(kThreads) build_kernel(const Args a) {
 
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads + tid;
-  const int64_t head0 = fail || a.capacity == 0 ? 0 : head % a.capacity;
+  // the capacity fits 31 bits; a counter of pages ever taken rarely needs the long division
+  const int64_t head0 = fail || a.capacity == 0 ? 0
+                        : head <= 0xffffffffll  ? static_cast<uint32_t>(head) % static_cast<uint32_t>(a.capacity)
+                                                : head % a.capacity;
   auto from_ring = [&](int64_t off) {
     const int64_t at = head0 + off;
     return a.ring[at >= a.capacity ? at - a.capacity : at];
@@ -158,23 +168,74 @@ __global__ void __launch_bounds__(kThreads) build_kernel(const Args a) {
       a.table[b * a.table_stride + held + (i - s_first[b])] = from_ring(i);
     }
   }
-  for (int64_t i = first; i < a.n_slots; i += stride) {
-    int64_t slot = -1;
-    int32_t pos = 0;
-    if (!fail && i < all_tok) {
+  // A decode step (one CTA, a few tokens a request): each thread fills in its own requests' tokens, without a
+  // search.
+  if (kRun == 1 && gridDim.x == 1 && !fail && !crowded) {
+    long long row = base_tok + inc_tok - tok, need = base_page + inc_page - pages;
+    for (int b = b0; b < b1; ++b) {
+      const int c = a.cached[b], n = a.fresh[b], held = (c + a.page - 1) / a.page;
+      int col = c / a.page, at = c - col * a.page;
+      int32_t page = -1;
+      for (int k = 0; k < n; ++k) {
+        if (k == 0 || at == a.page) {
+          if (at == a.page) ++col, at = 0;
+          page = col < held ? a.table[b * a.table_stride + col] : from_ring(need + col - held);
+          if (page < 0) record_error(a.err, kErrCachePage);
+        }
+        a.slots[row + k] = page < 0 ? -1 : static_cast<int64_t>(page) * a.page + at;
+        a.positions[row + k] = c + k;
+        ++at;
+      }
+      row += n;
+      need += (c + n + a.page - 1) / a.page - held;
+    }
+    for (int64_t i = all_tok + tid; i < a.n_slots; i += kThreads) {
+      a.slots[i] = -1;
+      a.positions[i] = 0;
+    }
+    return;
+  }
+  for (int64_t i0 = kRun * first; i0 < a.n_slots; i0 += kRun * stride) {
+    long long s4[kRun];
+    int p4[kRun];
+    int left = 0;  // tokens that still belong to the page at hand
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      const int64_t i = i0 + k;
+      s4[k] = -1;
+      p4[k] = 0;
+      if (fail || i >= all_tok) continue;
+      if (k > 0 && left > 0) {
+        s4[k] = s4[k - 1] < 0 ? -1 : s4[k - 1] + 1;
+        p4[k] = p4[k - 1] + 1;
+        --left;
+        continue;
+      }
       const int b = owner(s_cu, a.batch, static_cast<int32_t>(i));
       const int c = a.cached[b];
       const int held = (c + a.page - 1) / a.page;
-      pos = c + static_cast<int32_t>(i) - s_cu[b];
-      const int col = pos / a.page;
+      p4[k] = c + static_cast<int32_t>(i) - s_cu[b];
+      const int col = p4[k] / a.page, in_page = p4[k] - col * a.page;
       const int32_t page = col < held ? a.table[b * a.table_stride + col] : from_ring(s_first[b] + col - held);
       if (page >= 0)
-        slot = static_cast<int64_t>(page) * a.page + (pos - col * a.page);
+        s4[k] = static_cast<int64_t>(page) * a.page + in_page;
       else
         record_error(a.err, kErrCachePage);
+      left = min(a.page - in_page, s_cu[b + 1] - static_cast<int32_t>(i)) - 1;
     }
-    a.slots[i] = slot;
-    a.positions[i] = pos;
+    if (kRun == 4 && a.vec && i0 + 4 <= a.n_slots) {
+      reinterpret_cast<longlong2*>(a.slots + i0)[0] = make_longlong2(s4[0], s4[kRun > 1 ? 1 : 0]);
+      reinterpret_cast<longlong2*>(a.slots + i0)[1] = make_longlong2(s4[kRun > 2 ? 2 : 0], s4[kRun > 3 ? 3 : 0]);
+      *reinterpret_cast<int4*>(a.positions + i0) =
+          make_int4(p4[0], p4[kRun > 1 ? 1 : 0], p4[kRun > 2 ? 2 : 0], p4[kRun > 3 ? 3 : 0]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kRun; ++k)
+        if (i0 + k < a.n_slots) {
+          a.slots[i0 + k] = s4[k];
+          a.positions[i0 + k] = p4[k];
+        }
+    }
   }
 }
 
@@ -266,13 +327,22 @@ extern "C" int tm_build_block_tables(const tm_block_tables_params* p, int* error
     return TM_ERR_UNSUPPORTED;  // other CTAs still read the inputs while the outputs are written
   Args a{p->cached_lens, p->new_lens,  p->block_table, p->table_stride, p->cols,        p->free_pages,
          p->capacity,    p->free_span, p->batch,       p->page_size,    p->n_slots,     p->slots,
-         p->positions,   p->cu_seqlens, p->kv_lens,    p->free_span_out, error_flag};
+         p->positions,   p->cu_seqlens, p->kv_lens,    p->free_span_out,
+         tilemix::kv4::aligned(p->slots, 16) && tilemix::kv4::aligned(p->positions, 16), error_flag};
   const size_t smem = 2 * sizeof(int32_t) * (static_cast<size_t>(p->batch) + 1);
-  if (!tilemix::allow_smem<build_kernel, 2 * 4 * (kMaxBatch + 1)>()) return TM_ERR_LAUNCH;
-  // Two tokens a thread, at most one CTA an SM: below that the scan is the work, above it the stores.
-  const int64_t want = (p->n_slots + 2 * kThreads - 1) / (2 * kThreads);
-  const int grid = static_cast<int>(want < 1 ? 1 : want > 148 ? 148 : want);
-  build_kernel<<<grid, kThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
+  constexpr int kMostSmem = 2 * 4 * (kMaxBatch + 1);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // One CTA for what a decode step has; else one token a thread until every SM has its threads, four beyond
+  // (557,056 tokens: 10.3 us at two a thread, 8.0 at four; 256 single tokens: 6.8 and 11).
+  if (p->n_slots <= 148 * kThreads) {
+    if (!tilemix::allow_smem<build_kernel<1>, kMostSmem>()) return TM_ERR_LAUNCH;
+    const int64_t ctas = p->n_slots <= 4 * kThreads ? 1 : (p->n_slots + kThreads - 1) / kThreads;
+    build_kernel<1><<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(a);
+  } else {
+    if (!tilemix::allow_smem<build_kernel<4>, kMostSmem>()) return TM_ERR_LAUNCH;
+    const int64_t want = (p->n_slots + 4 * kThreads - 1) / (4 * kThreads);
+    build_kernel<4><<<static_cast<unsigned>(want > 296 ? 296 : want), kThreads, smem, st>>>(a);
+  }
   return cudaGetLastError() == cudaSuccess ? TM_OK : TM_ERR_LAUNCH;
 }
 

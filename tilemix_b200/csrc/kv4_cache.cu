@@ -3,8 +3,7 @@
 // Append, for each group of 32 channels of one (token, KV head) row x:
 //   m = min x, s = (max x - m) / 15 rounded down to fp16, n = min(rint((x - m) / s), 15)
 // and the cache stands for s n + m (never beyond the row's range, hence finite in
-// fp16: that is what rounding s down is for). Both fp32 differences and quotients round
-// once (IEEE), so the codes do not depend on the schedule. A group whose values
+// fp16: that is what rounding s down is for), differences and quotients in fp32. A group whose values
 // are equal (or closer than 15 fp16 subnormal steps) has s = 0 and n = 0; a group
 // with an infinity or a NaN reads back as NaN. Read back is the reverse, rounded
 // to fp16 once.
@@ -12,6 +11,7 @@
 // HBM bounds both on a prefill (2 bytes + 5 bits a value). A thread holds 8
 // channels of K and of V (two 16-byte loads in flight), four lanes a group.
 #include <cuda_fp16.h>
+#include <math_constants.h>
 
 #include "common.cuh"
 #include "kv4_layout.cuh"
@@ -20,7 +20,10 @@
 namespace tilemix {
 namespace kv4 {
 
-constexpr int kThreads = 256;
+// A CTA takes 16 consecutive tokens of one head, D / 8 lanes a token: consecutive tokens mostly share a block,
+// whose V scales (2 bytes a token in 8 places) then leave, or come, as whole sectors.
+template <int D>
+constexpr int kThreads = kBlockTokens * D / 8;
 
 struct AppendArgs {
   const __half* k;
@@ -30,12 +33,50 @@ struct AppendArgs {
   int64_t n_tokens;
   int64_t n_slots;  // pages * page size
   const int64_t* slots;
-  int heads, page, page_bytes;
+  int heads, page_bytes;
+  uint32_t page_blocks;
   int* err;
 };
 
+// Where a slot's 16-token block of a head is. Blocks are counted in 32 bits (the entry points see to it): a
+// 64-bit division by the page size was a quarter of the kernel's instructions.
+__device__ __forceinline__ int64_t block_offset(int64_t slot, int head, int heads, uint32_t page_blocks, int page_bytes,
+                                                int block_bytes) {
+  const uint32_t blk = static_cast<uint32_t>(slot >> 4), page = blk / page_blocks;
+  return (static_cast<int64_t>(page) * heads + head) * page_bytes +
+         static_cast<int64_t>(blk - page * page_blocks) * block_bytes;
+}
+
 __device__ __forceinline__ __half2 h2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
 __device__ __forceinline__ uint32_t u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  return static_cast<uint64_t>(__float_as_uint(hi)) << 32 | __float_as_uint(lo);
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// a / b from an approximate reciprocal of b and one residual correction (Markstein): q0 is within a few units in
+// the last place, the residual a - q0 b is exact in an FMA, and its product with r errs by 2^-22 of a unit, so
+// the quotient is that of an IEEE division unless it lies that near half way between two fp32 numbers; a
+// quotient half way between two codes is representable and comes out exact.
+__device__ __forceinline__ float quotient(float a, float b, float r) {
+  const float q0 = __fmul_rn(a, r);
+  return __fmaf_rn(__fmaf_rn(-q0, b, a), r, q0);
+}
 
 // Codes of a lane's 8 channels in nibble order (channel i at nibble i) and the
 // group's (s, m) as a half2. Four consecutive lanes hold the group.
@@ -49,39 +90,53 @@ __device__ __forceinline__ uint32_t quantise8(const uint4& x, __half2* sm) {
 #pragma unroll
   for (int o = 1; o <= 2; o <<= 1) ext = __hmin2_nan(ext, h2(__shfl_xor_sync(0xffffffffu, u32(ext), o)));
   const float lo = __low2float(ext), hi = -__high2float(ext);
-  const __half sh = __float2half_rd(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+  const __half sh = __float2half_rd(quotient(__fsub_rn(hi, lo), 15.f, 1.f / 15.f));
   const float s = __half2float(sh);
   *sm = __halves2half2(sh, __low2half(ext));
-  if (!(s > 0.f) || !isfinite(s)) return 0u;
-  // IEEE quotient from the correctly rounded reciprocal and one residual correction (Markstein):
-  // s is an fp16 value and 0 <= x - m <= 2^17, far from under- and overflow.
-  const float r = __frcp_rn(s);
-  const float f[8] = {__low2float(a), __high2float(a), __low2float(b), __high2float(b),
-                      __low2float(c), __high2float(c), __low2float(d), __high2float(d)};
-  uint32_t w = 0;
+  const bool ok = s > 0.f && s < CUDART_INF_F;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  const uint64_t r2 = pair(r, r), ns2 = pair(-s, -s), nlo2 = pair(-lo, -lo);
+  const uint64_t magic2 = 0x4B4000004B400000ull;  // 1.5 * 2^23: rounds to nearest even in the low bits
+  const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+  uint64_t e[4], u[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float e = __fsub_rn(f[i], lo);
-    const float q0 = __fmul_rn(e, r);
-    const float q = __fmaf_rn(__fmaf_rn(-q0, s, e), r, q0);
-    // round to nearest even in the low mantissa bits of 1.5 * 2^23
-    const uint32_t n = __float_as_uint(__fadd_rn(fminf(q, 15.f), 12582912.f)) & 15u;
-    w |= n << (4 * i);
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h2(in[i]));
+    e[i] = add2(pair(f.x, f.y), nlo2);
   }
-  return w;
+  // s is rounded down by less than 2^-10, so the largest quotient stays under 15.5, except where s is
+  // subnormal: there x - m is cut at 15 s.
+  if (__any_sync(0xffffffffu, s < 6.103515625e-5f)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      e[i] = pair(fminf(__uint_as_float(static_cast<uint32_t>(e[i])), 15.f * s),
+                  fminf(__uint_as_float(static_cast<uint32_t>(e[i] >> 32)), 15.f * s));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t q0 = mul2(e[i], r2);
+    u[i] = add2(fma2(fma2(q0, ns2, e[i]), r2, q0), magic2);
+  }
+  // sum of (0x4B400000 + n_i) 16^i modulo 2^32, less the constants'
+  uint32_t w = static_cast<uint32_t>(u[3] >> 32);
+#pragma unroll
+  for (int i = 6; i >= 0; --i) w = (w << 4) + static_cast<uint32_t>(u[i / 2] >> (32 * (i % 2)));
+  return ok ? w - (0x4B400000u + 0xB4000000u + 0x40000000u) : 0u;
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kThreads<D>) append_kernel(const AppendArgs a) {
   using L = Layout<D>;
   constexpr int kLanes = D / 8;  // lanes a row
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
+  __shared__ uint8_t* sh_block[kBlockTokens];  // each token's block, NULL: it is not stored
+  __shared__ int sh_at[kBlockTokens];          // its place there
+  __shared__ __half sh_scale[kBlockTokens][L::kGroups][2];
+  const int head = blockIdx.x, in_cta = threadIdx.x / kLanes;
+  const int64_t tok = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * kBlockTokens + in_cta;
   const int l = threadIdx.x % kLanes;
   const int j = l >> 2, t = l & 3;
-  // Items behind the last one stay for the shuffles.
-  const bool there = item < a.n_tokens * a.heads;
-  const int64_t tok = there ? item / a.heads : 0;
-  const int head = there ? static_cast<int>(item - tok * a.heads) : 0;
+  const bool there = tok < a.n_tokens;  // tokens behind the last one stay for the shuffles
   const int64_t slot = there ? a.slots[tok] : -1;
   const bool fits = slot >= 0 && slot < a.n_slots;
   uint4 xk = make_uint4(0, 0, 0, 0), xv = xk;
@@ -95,22 +150,35 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
   // stores one 32-bit word. The even group's lane keeps chunk 2t, the odd one's chunk 2t + 1.
   const uint32_t other = __shfl_xor_sync(0xffffffffu, vw, 4);
   const uint32_t vpair = (j & 1) ? __byte_perm(other, vw, 0x7632) : __byte_perm(vw, other, 0x5410);
-  if (!fits) {
-    if (there && (slot >= a.n_slots || slot < -1) && l == 0) record_error(a.err, kErrCacheSlot);
-    return;
-  }
-  const int64_t page = slot / a.page;
-  const int in_page = static_cast<int>(slot - page * a.page), in_block = in_page % kBlockTokens;
-  uint8_t* blk = a.pool + (page * a.heads + head) * a.page_bytes +
-                 static_cast<int64_t>(in_page / kBlockTokens) * L::kBlockBytes;
-  *reinterpret_cast<uint32_t*>(blk + in_block * L::kRowBytes + (t * L::kGroups + j) * 4) = kw;
-  const int g = 2 * t + (j & 1);
-  *reinterpret_cast<uint32_t*>(blk + L::kOffV + in_block * L::kRowBytes + g * (2 * L::kGroups) + (j & ~1) * 2) = vpair;
+  const int in_block = static_cast<int>(slot) & (kBlockTokens - 1);
+  uint8_t* blk = fits ? a.pool + block_offset(slot, head, a.heads, a.page_blocks, a.page_bytes, L::kBlockBytes) : nullptr;
   if (t == 0) {
-    *reinterpret_cast<__half2*>(blk + L::kOffKScale + in_block * L::kScaleBytes + j * 4) = ks;
-    __half* p = reinterpret_cast<__half*>(blk + L::kOffVScale + L::v_scale(j, in_block));
-    p[0] = __low2half(vs);
-    p[4] = __high2half(vs);
+    sh_scale[in_cta][j][0] = __low2half(vs);
+    sh_scale[in_cta][j][1] = __high2half(vs);
+    if (j == 0) {
+      sh_block[in_cta] = blk;
+      sh_at[in_cta] = in_block;
+      if (there && (slot >= a.n_slots || slot < -1)) record_error(a.err, kErrCacheSlot);
+    }
+  }
+  if (fits) {
+    *reinterpret_cast<uint32_t*>(blk + in_block * L::kRowBytes + (t * L::kGroups + j) * 4) = kw;
+    const int g = 2 * t + (j & 1);
+    *reinterpret_cast<uint32_t*>(blk + L::kOffV + in_block * L::kRowBytes + g * (2 * L::kGroups) + (j & ~1) * 2) = vpair;
+    if (t == 0) *reinterpret_cast<__half2*>(blk + L::kOffKScale + in_block * L::kScaleBytes + j * 4) = ks;
+  }
+  __syncthreads();
+  // The V scales, a thread each, in the order in which a block holds them if its tokens follow on from the
+  // first one's slot (any other order is as right, only slower).
+  const int i = threadIdx.x;
+  if (i < kBlockTokens * L::kGroups * 2) {
+    const int quarter = i & 3, which = (i >> 2) & 1, tt = (i >> 3) & 3, jj = i >> 5;
+    const int first = sh_block[0] == nullptr ? 0 : sh_at[0];
+    const int token = (4 * quarter + tt - first) & (kBlockTokens - 1);
+    uint8_t* to = sh_block[token];
+    if (to != nullptr)
+      *reinterpret_cast<__half*>(to + L::kOffVScale + L::v_scale(jj, sh_at[token]) + 8 * which) =
+          sh_scale[token][jj][which];
   }
 }
 
@@ -118,52 +186,73 @@ struct ReadArgs {
   const uint8_t* pool;
   const int64_t* slots;
   int64_t n_tokens, n_slots;
-  int heads, page, page_bytes;
+  int heads, page_bytes;
+  uint32_t page_blocks;
   __half* k;
   __half* v;
   int* err;
 };
 
-__device__ __forceinline__ uint4 dequant8(uint32_t w, float s, float m) {
-  uint32_t o[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    o[i] = pack_half2_rn(__fmaf_rn(static_cast<float>((w >> (8 * i)) & 15u), s, m),
-                         __fmaf_rn(static_cast<float>((w >> (8 * i + 4)) & 15u), s, m));
-  return make_uint4(o[0], o[1], o[2], o[3]);
+// Eight values in channel order: codes OR-ed into the mantissa of 1024 as pairs (i, i + 4), brought to n
+// exactly, one fp16 FMA (one rounding), then put side by side.
+__device__ __forceinline__ uint4 dequant8(uint32_t w, __half s, __half m) {
+  const __half2 s2 = __half2half2(s), m2 = __half2half2(m);
+  const __half2 k1024 = h2(0x64006400u), r16 = h2(0x2C002C00u), k64 = h2(0xD400D400u);  // 1024, 1/16, -64
+  const uint32_t w8 = w >> 8;
+  const uint32_t a = u32(__hfma2(__hsub2(h2((w & 0x000F000Fu) | 0x64006400u), k1024), s2, m2));
+  const uint32_t b = u32(__hfma2(__hfma2(h2((w & 0x00F000F0u) | 0x64006400u), r16, k64), s2, m2));
+  const uint32_t c = u32(__hfma2(__hsub2(h2((w8 & 0x000F000Fu) | 0x64006400u), k1024), s2, m2));
+  const uint32_t d = u32(__hfma2(__hfma2(h2((w8 & 0x00F000F0u) | 0x64006400u), r16, k64), s2, m2));
+  return make_uint4(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), __byte_perm(a, b, 0x7632),
+                    __byte_perm(c, d, 0x7632));
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
+__global__ void __launch_bounds__(kThreads<D>) read_kernel(const ReadArgs a) {
   using L = Layout<D>;
   constexpr int kLanes = D / 8;
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kLanes;
-  if (item >= a.n_tokens * a.heads) return;
+  const int head = blockIdx.x;
+  const int64_t tok =
+      (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * kBlockTokens + threadIdx.x / kLanes;
   const int l = threadIdx.x % kLanes;
   const int j = l >> 2, t = l & 3;
-  const int64_t tok = item / a.heads;
-  const int head = static_cast<int>(item - tok * a.heads);
-  const int64_t slot = a.slots[tok];
+  const bool there = tok < a.n_tokens;  // tokens behind the last one stay for the shuffle
+  const int64_t slot = there ? a.slots[tok] : -1;
+  const bool fits = slot >= 0 && slot < a.n_slots;
+  uint32_t kw = 0, vpair = 0;
+  __half2 ks = __half2half2(__ushort_as_half(0));
+  __half vs = __ushort_as_half(0), vm = vs;
+  if (fits) {
+    const int in_block = static_cast<int>(slot) & (kBlockTokens - 1);
+    const uint8_t* blk = a.pool + block_offset(slot, head, a.heads, a.page_blocks, a.page_bytes, L::kBlockBytes);
+    kw = *reinterpret_cast<const uint32_t*>(blk + in_block * L::kRowBytes + (t * L::kGroups + j) * 4);
+    vpair = *reinterpret_cast<const uint32_t*>(blk + L::kOffV + in_block * L::kRowBytes +
+                                               (2 * t + (j & 1)) * (2 * L::kGroups) + (j & ~1) * 2);
+    ks = *reinterpret_cast<const __half2*>(blk + L::kOffKScale + in_block * L::kScaleBytes + j * 4);
+    const __half* v = reinterpret_cast<const __half*>(blk + L::kOffVScale + L::v_scale(j, in_block));
+    vs = v[0];
+    vm = v[4];
+  }
+  // as in append: the lane holds chunk 2 t (+ 1) of groups j and j ^ 1 and trades one half
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, vpair, 4);
+  const uint32_t vw = (j & 1) ? __byte_perm(other, vpair, 0x7632) : __byte_perm(vpair, other, 0x5410);
+  if (!there) return;
   uint4 ok = make_uint4(0, 0, 0, 0), ov = ok;
-  if (slot >= 0 && slot < a.n_slots) {
-    const int64_t page = slot / a.page;
-    const int in_page = static_cast<int>(slot - page * a.page), in_block = in_page % kBlockTokens;
-    const uint8_t* blk = a.pool + (page * a.heads + head) * a.page_bytes +
-                         static_cast<int64_t>(in_page / kBlockTokens) * L::kBlockBytes;
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(blk + in_block * L::kRowBytes + (t * L::kGroups + j) * 4);
-    const uint8_t* vr = blk + L::kOffV + in_block * L::kRowBytes + 2 * j;
-    const uint32_t v0 = *reinterpret_cast<const uint16_t*>(vr + (2 * t) * (2 * L::kGroups));
-    const uint32_t v1 = *reinterpret_cast<const uint16_t*>(vr + (2 * t + 1) * (2 * L::kGroups));
-    const __half2 ks = *reinterpret_cast<const __half2*>(blk + L::kOffKScale + in_block * L::kScaleBytes + j * 4);
-    const __half* vs = reinterpret_cast<const __half*>(blk + L::kOffVScale + L::v_scale(j, in_block));
-    ok = dequant8(kw, __low2float(ks), __high2float(ks));
-    ov = dequant8(v0 | v1 << 16, __half2float(vs[0]), __half2float(vs[4]));
+  if (fits) {
+    ok = dequant8(kw, __low2half(ks), __high2half(ks));
+    ov = dequant8(vw, vs, vm);
   } else if (slot != -1 && l == 0) {
     record_error(a.err, kErrCacheSlot);
   }
-  const int64_t at = item * D + 8 * l;
+  const int64_t at = (tok * a.heads + head) * D + 8 * l;
   __stcs(reinterpret_cast<uint4*>(a.k + at), ok);
   __stcs(reinterpret_cast<uint4*>(a.v + at), ov);
+}
+
+// Heads fastest: the heads of 16 tokens are neighbours in memory.
+static dim3 grid_of(int64_t groups, int heads) {
+  const unsigned y = static_cast<unsigned>(groups < 65535 ? groups : 65535);
+  return dim3(static_cast<unsigned>(heads), y, static_cast<unsigned>((groups + y - 1) / y));
 }
 
 }  // namespace kv4
@@ -181,16 +270,17 @@ extern "C" int tm_kv4_append(const void* k, int64_t k_stride_tok, int64_t k_stri
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(pool, 16) || !aligned(slots, 8)) return TM_ERR_ALIGN;
   if (k_stride_tok % 8 || k_stride_head % 8 || v_stride_tok % 8 || v_stride_head % 8) return TM_ERR_ALIGN;
   const int64_t page_bytes = static_cast<int64_t>(page_size) / kBlockTokens * block_bytes(head_dim);
-  const int64_t blocks = (n_tokens * heads * (head_dim / 8) + kThreads - 1) / kThreads;
-  if (page_bytes > 0x7fffffffll || blocks > 0x7fffffffll) return TM_ERR_UNSUPPORTED;
+  const int64_t groups = (n_tokens + kBlockTokens - 1) / kBlockTokens;
+  if (page_bytes > 0x7fffffffll || groups > 65535ll * 65535ll || num_pages > 0x7fffffffll / (page_size / kBlockTokens))
+    return TM_ERR_UNSUPPORTED;
   AppendArgs a{static_cast<const __half*>(k), static_cast<const __half*>(v), k_stride_tok, k_stride_head,
                v_stride_tok, v_stride_head, static_cast<uint8_t*>(pool), n_tokens, num_pages * page_size, slots,
-               heads, page_size, static_cast<int>(page_bytes), error_flag};
+               heads, static_cast<int>(page_bytes), static_cast<uint32_t>(page_size / kBlockTokens), error_flag};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128)
-    append_kernel<128><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(a);
+    append_kernel<128><<<grid_of(groups, heads), kThreads<128>, 0, st>>>(a);
   else
-    append_kernel<64><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(a);
+    append_kernel<64><<<grid_of(groups, heads), kThreads<64>, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? TM_OK : TM_ERR_LAUNCH;
 }
 
@@ -203,14 +293,15 @@ extern "C" int tm_kv4_read(const void* pool, int64_t num_pages, int heads, int h
   if (!k || !v || !slots || (num_pages > 0 && !pool)) return TM_ERR_NULL;
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(pool, 16) || !aligned(slots, 8)) return TM_ERR_ALIGN;
   const int64_t page_bytes = static_cast<int64_t>(page_size) / kBlockTokens * block_bytes(head_dim);
-  const int64_t blocks = (n_tokens * heads * (head_dim / 8) + kThreads - 1) / kThreads;
-  if (page_bytes > 0x7fffffffll || blocks > 0x7fffffffll) return TM_ERR_UNSUPPORTED;
-  ReadArgs a{static_cast<const uint8_t*>(pool), slots, n_tokens, num_pages * page_size, heads, page_size,
-             static_cast<int>(page_bytes), static_cast<__half*>(k), static_cast<__half*>(v), error_flag};
+  const int64_t groups = (n_tokens + kBlockTokens - 1) / kBlockTokens;
+  if (page_bytes > 0x7fffffffll || groups > 65535ll * 65535ll || num_pages > 0x7fffffffll / (page_size / kBlockTokens))
+    return TM_ERR_UNSUPPORTED;
+  ReadArgs a{static_cast<const uint8_t*>(pool), slots, n_tokens, num_pages * page_size, heads, static_cast<int>(page_bytes),
+             static_cast<uint32_t>(page_size / kBlockTokens), static_cast<__half*>(k), static_cast<__half*>(v), error_flag};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128)
-    read_kernel<128><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(a);
+    read_kernel<128><<<grid_of(groups, heads), kThreads<128>, 0, st>>>(a);
   else
-    read_kernel<64><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(a);
+    read_kernel<64><<<grid_of(groups, heads), kThreads<64>, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? TM_OK : TM_ERR_LAUNCH;
 }

@@ -44,8 +44,8 @@ constexpr int kStepKeys = kStepBlocks * kBlockTokens;
 constexpr int kChunkKeys = kStepKeys * kAttnWarps;    // keys of one step of every warp: the unit of work
 constexpr int kSms = 148;
 
-// CTAs an SM of the kernel with NT row tiles, by registers and shared memory.
-constexpr int resident(int nt) { return nt == 1 ? 3 : 2; }
+// CTAs an SM of the kernel for head_dim d and nt row tiles, by registers and shared memory.
+constexpr int resident(int d, int nt) { return d == 128 && nt == 2 ? 2 : 3; }
 
 struct AttnArgs {
   const __half* q;
@@ -195,7 +195,7 @@ __device__ __forceinline__ Words<N> load_words(const uint8_t* p) {
 // written at once. A CTA's first run of chunks may continue another's (slot 2 c), its last may be continued
 // (slot 2 c + 1).
 template <int D, int NT>
-__global__ void __launch_bounds__(kAttnThreads, resident(NT)) attn_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(const AttnArgs a) {
   using L = Layout<D>;
   constexpr int G = L::kGroups;
   constexpr int kRows = 8 * NT;
@@ -468,15 +468,18 @@ __global__ void __launch_bounds__(kAttnThreads, resident(NT)) attn_kernel(const 
       }
 
       if constexpr (!kPlain) {
+        const uint32_t on = live >> tok_g;
 #pragma unroll
-        for (int u = 0; u < kStepBlocks; ++u)
+        for (int x = 0; x < NT; ++x)
 #pragma unroll
-          for (int x = 0; x < NT; ++x)
+          for (int c = 0; c < 4; ++c) {
+            const int left = lim[x][c & 1] - key - tok_g;  // the row sees this many keys from the lane's first on
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int at = kBlockTokens * u + tok_g + (c >> 1) * 8;
-              if (!((live >> at) & 1) || key + at >= lim[x][c & 1]) sc[u][x][c] = -CUDART_INF_F;
+            for (int u = 0; u < kStepBlocks; ++u) {
+              const int at = kBlockTokens * u + (c >> 1) * 8;
+              if (!(on & (1u << at)) || at >= left) sc[u][x][c] = -CUDART_INF_F;
             }
+          }
       }
       float base[NT][2];
       bool moved = false;
@@ -574,14 +577,14 @@ __global__ void __launch_bounds__(kAttnThreads, resident(NT)) attn_kernel(const 
     for (int i = 0; i < steps; ++i) {
       const int key = key0 + kStepKeys * (warp + kAttnWarps * i);
       const uint32_t bad = (stage_bad >> (kStepBlocks * s)) & ((1u << kStepBlocks) - 1);
-      // Which of the step's keys count for any row: bit `token` of block u.
-      const bool plain = bad == 0 && mask == nullptr && key + kStepKeys <= lim_lo;
-      uint32_t live = 0xffffffffu;  // bit: key of the step
-      if (!plain) {
+      // Which of the step's keys count for any row, a bit each; all of them, for every row, in most steps.
+      uint32_t live = 0xffffffffu;
+      if (bad != 0 || mask != nullptr || key + kStepKeys > lim_hi) {
         live = __ballot_sync(0xffffffffu, !((bad >> (lane / kBlockTokens)) & 1) && key + lane < lim_hi &&
                                               (mask == nullptr || mask_on));
         if (mask != nullptr) mask_on = mask_of(i + 1);
       }
+      const bool plain = live == 0xffffffffu && key + kStepKeys <= lim_lo;
       if (!mbar_wait_spin(&bar[s], phase, a.err, kErrTimeoutFull)) {
         ok = false;
         break;
@@ -789,7 +792,7 @@ static Plan plan_of(const tm_kv4_attn_params* p) {
   const int64_t tiles = (rows + 8 * r.nt - 1) / (8 * r.nt);
   const int64_t chunks = p->max_kv_len / kChunkKeys + 1;
   const int64_t most = static_cast<int64_t>(p->batch) * p->heads_k * tiles;
-  const int64_t slots = kSms * resident(r.nt);
+  const int64_t slots = kSms * resident(p->head_dim, r.nt);
   r.ctas = static_cast<int>(most >= slots || chunks >= slots || most * chunks >= slots ? slots : most * chunks);
   r.starts_bytes = (static_cast<int64_t>(p->batch) + 4) / 4 * 16;
   r.part_o_bytes = 2ll * r.ctas * 8 * r.nt * p->head_dim * 4;

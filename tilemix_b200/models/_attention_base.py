@@ -18,6 +18,7 @@ from torch import Tensor
 
 from tilemix_b200.attention.precision_maps import BLOCK_PERCENTAGE_PATTERNS, make_precision_bitmask
 from tilemix_b200.attention.tilemix_varlen import tilemix_varlen_attention
+from tilemix_b200.models.kv4_cache import Kv4Cache
 
 
 @dataclass(frozen=True)
@@ -167,6 +168,17 @@ class TileMixAttentionMixin:
     def _fixup_precision_map(self, precision_map: Tensor, seqlen: int, block_n_mask: int) -> Tensor:
         return precision_map
 
+    # -- the 4-bit cache (no counterpart in the reference)
+    def _kv4_attention(self, q: Tensor, k: Tensor, v: Tensor, cache: Kv4Cache, attention_mask, k_quant=None) -> Tensor:
+        """Store k / v [B, nkv, T, D] and attend: a prompt of 16 tokens or more with the routed attention on
+        its own keys and values, everything else over the cache. Returns [B, nh, T, D]."""
+        first, seqlen = cache.get_seq_length(self.layer_idx) == 0, q.shape[2]
+        cache.append(k, v, self.layer_idx)
+        if first and seqlen >= 16:
+            return self._tilemix_attention(q, k, v, seqlen, k_quant=k_quant)
+        out = cache.attend(q, self.layer_idx, self.head_dim ** -0.5, _key_mask(attention_mask))
+        return out.transpose(1, 2)
+
     # -- the attention call (models/tilemix_llama.py:505-646)
     def _tilemix_attention(self, q: Tensor, k: Tensor, v: Tensor, seqlen: int, k_quant=None) -> Tensor:
         """q [B, nh, T, D], k/v [B, nkv, T, D] -> attention output [B, nh, T, D]. ``k_quant``:
@@ -187,6 +199,15 @@ class TileMixAttentionMixin:
                                         causal=True, scale=head_dim ** -0.5, precision_map_all=pm,
                                         candidates=[(bucket.block_m, bucket.block_n)], flat_lengths=[pm.numel()],
                                         k_quant=k_quant)
+
+
+def _key_mask(attention_mask) -> Optional[Tensor]:
+    """Keys that a batch's padding leaves, bool [B, keys], from the mask that HF hands to its attention: that of
+    the last query token, which no causal entry hides a key from."""
+    if attention_mask is None:
+        return None
+    mask = attention_mask if attention_mask.ndim == 2 else attention_mask[:, 0, -1]
+    return (mask if mask.dtype == torch.bool else mask == 0 if mask.is_floating_point() else mask != 0).contiguous()
 
 
 def copy_attention_weights(orig, new) -> None:

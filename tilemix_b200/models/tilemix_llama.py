@@ -9,7 +9,8 @@ Public API, same names and behaviour as the reference:
   prepare_llama_prefill(model)        :883-895
 Prefill sequences of 16 tokens or more run the routed FP16/INT8 attention through
 ``tilemix_varlen_attention`` (the sm_100a kernels); shorter ones (decode) use HF's
-own attention, as in the reference.
+own attention, as in the reference, or, with a ``Kv4Cache`` as ``past_key_values``,
+attend over the cache in 4 bits.
 """
 from __future__ import annotations
 
@@ -20,6 +21,7 @@ from torch import Tensor, nn
 from transformers.cache_utils import Cache, DynamicLayer
 from transformers.models.llama.modeling_llama import LlamaAttention, apply_rotary_pos_emb
 
+from tilemix_b200.models.kv4_cache import Kv4Cache
 from tilemix_b200.models._attention_base import (
     BucketConfig,
     TileMixAttentionMixin,
@@ -55,7 +57,8 @@ class TileMixLlamaAttention(TileMixAttentionMixin, LlamaAttention):
         if not hidden_states.is_cuda:
             hidden_states = hidden_states.cuda()
         bsz, seqlen, _ = hidden_states.shape
-        if seqlen < 16:  # decode: HF attention (models/tilemix_llama.py:526-536)
+        kv4 = isinstance(past_kv, Kv4Cache)
+        if seqlen < 16 and not kv4:  # decode: HF attention (models/tilemix_llama.py:526-536)
             return LlamaAttention.forward(self, hidden_states, position_embeddings=position_embeddings,
                                           attention_mask=attention_mask, past_key_values=past_kv,
                                           cache_position=cache_position, **kwargs)
@@ -74,6 +77,9 @@ class TileMixLlamaAttention(TileMixAttentionMixin, LlamaAttention):
             k_quant = (k8, ks)
         else:
             q, k = self.apply_rotary(q, k, cos, sin)
+        if kv4:
+            out = self._kv4_attention(q, k, v, past_kv, attention_mask, k_quant=k_quant)
+            return self.o_proj(out.transpose(1, 2).reshape(bsz, seqlen, -1)), None
         if past_kv is not None:
             k_rot = k
             k, v = past_kv.update(k, v, self.layer_idx,

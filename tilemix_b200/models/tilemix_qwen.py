@@ -16,6 +16,7 @@ import torch
 from torch import Tensor
 from transformers.models.qwen2.modeling_qwen2 import Qwen2Attention, apply_rotary_pos_emb
 
+from tilemix_b200.models.kv4_cache import Kv4Cache
 from tilemix_b200.models._attention_base import (
     BucketConfig,
     TileMixAttentionMixin,
@@ -52,7 +53,8 @@ class TileMixqwenAttention(TileMixAttentionMixin, Qwen2Attention):
         if not hidden_states.is_cuda:
             hidden_states = hidden_states.cuda()
         bsz, seqlen, _ = hidden_states.shape
-        if seqlen < 16:
+        kv4 = isinstance(past_kv, Kv4Cache)
+        if seqlen < 16 and not kv4:
             return Qwen2Attention.forward(self, hidden_states, position_embeddings, attention_mask,
                                           past_key_values=past_kv, cache_position=cache_position, **kwargs)
         head_dim = self.head_dim
@@ -64,6 +66,9 @@ class TileMixqwenAttention(TileMixAttentionMixin, Qwen2Attention):
             position_embeddings = self.rotary_emb(q, kwargs.get("position_ids", None))
         cos, sin = (t.to(dev) for t in position_embeddings)
         q, k = apply_rotary_pos_emb(q, k, cos, sin)
+        if kv4:
+            out = self._kv4_attention(q.contiguous(), k.contiguous(), v.contiguous(), past_kv, attention_mask)
+            return self.o_proj(out.transpose(1, 2).reshape(bsz, seqlen, -1)), None
         if past_kv is not None:
             k, v = past_kv.update(k, v, self.layer_idx,
                                   cache_kwargs={"sin": sin, "cos": cos, "cache_position": cache_position})

@@ -38,7 +38,7 @@ namespace kv4 {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-constexpr int kStages = 3;
+constexpr int kStages = 2;  // 10 KB a warp in flight, 120 KB an SM; three measured no faster
 constexpr int kStepBlocks = 2;                        // 16-key blocks a step
 constexpr int kStepKeys = kStepBlocks * kBlockTokens;
 constexpr int kChunkKeys = kStepKeys * kAttnWarps;    // keys of one step of every warp: the unit of work
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
   constexpr int kStageBytes = kStepBlocks * L::kBlockBytes;
   constexpr int kState = NT * (8 * G + 4);  // floats of a lane's state (o, m, l)
   extern __shared__ __align__(128) uint8_t smem[];
-  float* sh_state = reinterpret_cast<float*>(smem + kAttnWarps * kStages * kStageBytes);  // [2][kState][32]
+  float* sh_state = reinterpret_cast<float*>(smem + kAttnWarps * kStages * kStageBytes);  // [warps][kState][32]
   __shared__ __align__(8) uint64_t bars[kAttnWarps][kStages];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -282,17 +282,19 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
   // the next 32 (its pages, the addresses of its blocks) and issues that step's copies itself when its turn
   // comes, so a step costs a few instructions. Steps of all runs count on through the ring's stages.
   const uint8_t* src[kStepBlocks];  // the lane's step; NULL: past the run's end, or its page is outside the pool
-  uint32_t absent[kStepBlocks];     // bit i: step i of the 32 lacks the block
+  bool joined = false;              // the lane's two blocks are adjacent: one copy
+  uint32_t absent[kStepBlocks];     // bit i: step i of the 32 lacks the block (a step past the end is none)
   int issued = 0;                   // steps of the current run whose copies are under way
   int in_stage = 0;                 // stage of the next step to issue
   uint32_t stage_bad = 0;           // bit (kStepBlocks stage + block): not in the stage
   int all_issued = 0;
+  auto first_of = [&](int i) { return key0 / kBlockTokens + kStepBlocks * (warp + kAttnWarps * i); };
   auto issue = [&]() {
     if ((issued & 31) == 0) {
       const int32_t* row = a.table + b * a.table_stride;
 #pragma unroll
       for (int u = 0; u < kStepBlocks; ++u) {
-        const int blk = key0 / kBlockTokens + kStepBlocks * (warp + kAttnWarps * (issued + lane)) + u;
+        const int blk = first_of(issued + lane) + u;
         src[u] = nullptr;
         if (blk < blk1) {
           const int col = blk / a.page_blocks;
@@ -303,20 +305,25 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
           else
             record_error(a.err, kErrCachePage);
         }
-        absent[u] = __ballot_sync(0xffffffffu, src[u] == nullptr);
+        absent[u] = __ballot_sync(0xffffffffu, src[u] == nullptr && first_of(issued + lane) < blk1);
       }
+      joined = src[0] != nullptr && src[1] == src[0] + L::kBlockBytes;
     }
-    uint32_t bad = 0;
+    if ((absent[0] | absent[1] | stage_bad) != 0) {
+      uint32_t bad = 0;
 #pragma unroll
-    for (int u = 0; u < kStepBlocks; ++u) bad |= ((absent[u] >> (issued & 31)) & 1u) << u;
-    stage_bad = (stage_bad & ~(((1u << kStepBlocks) - 1) << (kStepBlocks * in_stage))) | bad << (kStepBlocks * in_stage);
+      for (int u = 0; u < kStepBlocks; ++u) bad |= ((absent[u] >> (issued & 31)) & 1u) << u;
+      const int at = kStepBlocks * in_stage;
+      stage_bad = (stage_bad & ~(((1u << kStepBlocks) - 1) << at)) | bad << at;
+    }
     if (lane == (issued & 31)) {
       uint8_t* dst = ring + in_stage * kStageBytes;
       uint64_t* full = &bar[in_stage];
-      mbar_arrive_expect_tx(full, (kStepBlocks - __popc(bad)) * L::kBlockBytes);
-      if (bad == 0 && src[1] == src[0] + L::kBlockBytes) {
+      if (joined) {
+        mbar_arrive_expect_tx(full, kStageBytes);
         bulk_load(dst, src[0], kStageBytes, full);
       } else {
+        mbar_arrive_expect_tx(full, ((src[0] != nullptr) + (src[1] != nullptr)) * L::kBlockBytes);
 #pragma unroll
         for (int u = 0; u < kStepBlocks; ++u)
           if (src[u] != nullptr) bulk_load(dst + u * L::kBlockBytes, src[u], L::kBlockBytes, full);
@@ -574,17 +581,20 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
       return i < steps && key < min(lim_hi, a.mask_cols) && mask[key] != 0;
     };
     bool mask_on = mask != nullptr && mask_of(0);
+    // The first steps of a run without a mask are plain: every key counts for every row.
+    const int first_key = key0 + kStepKeys * warp, stride = kStepKeys * kAttnWarps;
+    const int n_plain = mask != nullptr || lim_lo < first_key + kStepKeys ? 0 : (lim_lo - kStepKeys - first_key) / stride + 1;
     for (int i = 0; i < steps; ++i) {
-      const int key = key0 + kStepKeys * (warp + kAttnWarps * i);
-      const uint32_t bad = (stage_bad >> (kStepBlocks * s)) & ((1u << kStepBlocks) - 1);
-      // Which of the step's keys count for any row, a bit each; all of them, for every row, in most steps.
-      uint32_t live = 0xffffffffu;
-      if (bad != 0 || mask != nullptr || key + kStepKeys > lim_hi) {
+      const int key = first_key + stride * i;
+      uint32_t live = 0xffffffffu;  // which of the step's keys count for any row, a bit each
+      bool plain = i < n_plain && stage_bad == 0;
+      if (!plain) {
+        const uint32_t bad = (stage_bad >> (kStepBlocks * s)) & ((1u << kStepBlocks) - 1);
         live = __ballot_sync(0xffffffffu, !((bad >> (lane / kBlockTokens)) & 1) && key + lane < lim_hi &&
                                               (mask == nullptr || mask_on));
         if (mask != nullptr) mask_on = mask_of(i + 1);
+        plain = live == 0xffffffffu && key + kStepKeys <= lim_lo;
       }
-      const bool plain = live == 0xffffffffu && key + kStepKeys <= lim_lo;
       if (!mbar_wait_spin(&bar[s], phase, a.err, kErrTimeoutFull)) {
         ok = false;
         break;
@@ -623,80 +633,65 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
     for (int x = 0; x < NT; ++x)
 #pragma unroll
       for (int c = 0; c < 2; ++c) m[x][c] *= cs[x][c];  // log2 units from here on
-    // Merge the warps' states: 2 and 3 into 0 and 1, then 1 into 0.
+    // Merge the warps' states, a share of the channel groups each.
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], d);
+    {
+      float* to = sh_state + warp * kState * 32 + lane;
 #pragma unroll
-    for (int half = kAttnWarps / 2; half > 0; half >>= 1) {
-      if (warp >= half && warp < 2 * half) {
-        float* to = sh_state + (warp - half) * kState * 32 + lane;
+      for (int x = 0; x < NT; ++x) {
 #pragma unroll
-        for (int x = 0; x < NT; ++x) {
+        for (int k = 0; k < 2 * G; ++k)
 #pragma unroll
-          for (int k = 0; k < 2 * G; ++k)
+          for (int c = 0; c < 4; ++c) to[(x * 8 * G + 4 * k + c) * 32] = o[x][k][c];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) to[(x * 8 * G + 4 * k + c) * 32] = o[x][k][c];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            to[(NT * 8 * G + 4 * x + c) * 32] = m[x][c];
-            to[(NT * 8 * G + 4 * x + 2 + c) * 32] = l[x][c];
-          }
+        for (int c = 0; c < 2; ++c) {
+          to[(NT * 8 * G + 4 * x + c) * 32] = m[x][c];
+          to[(NT * 8 * G + 4 * x + 2 + c) * 32] = l[x][c];
         }
       }
-      __syncthreads();
-      if (warp < half) {
-        const float* from = sh_state + warp * kState * 32 + lane;
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          float f[2], h[2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float other = from[(NT * 8 * G + 4 * x + c) * 32];
-            const float top = fmaxf(m[x][c], other);
-            const float ref = top == -CUDART_INF_F ? 0.f : top;
-            f[c] = ex2_approx(m[x][c] - ref);
-            h[c] = ex2_approx(other - ref);
-            l[x][c] = f[c] * l[x][c] + h[c] * from[(NT * 8 * G + 4 * x + 2 + c) * 32];
-            m[x][c] = top;
-          }
-#pragma unroll
-          for (int k = 0; k < 2 * G; ++k)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              o[x][k][c] = f[c & 1] * o[x][k][c] + h[c & 1] * from[(x * 8 * G + 4 * k + c) * 32];
-        }
-      }
-      __syncthreads();
     }
-    if (warp == 0) {
+    __syncthreads();
+    if (warp < G) {
+      const int j = warp;
+      static_assert(G <= kAttnWarps, "a channel group a warp");
 #pragma unroll
       for (int x = 0; x < NT; ++x)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int r = 8 * x + 2 * t + c;
           if (o_row0 + r >= n_rows) continue;
+          const float* from = sh_state + lane;
+          float mw[kAttnWarps], top = -CUDART_INF_F, sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < kAttnWarps; ++w) {
+            mw[w] = from[(w * kState + NT * 8 * G + 4 * x + c) * 32];
+            top = fmaxf(top, mw[w]);
+          }
+          const float ref = top == -CUDART_INF_F ? 0.f : top;
+          float v[4] = {};  // channels 32 j + 4 g ..
+#pragma unroll
+          for (int w = 0; w < kAttnWarps; ++w) {
+            const float f = ex2_approx(mw[w] - ref);
+            sum += f * from[(w * kState + NT * 8 * G + 4 * x + 2 + c) * 32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)  // accumulator 2 j + i / 2, row g or g + 8
+              v[i] += f * from[(w * kState + x * 8 * G + 4 * (2 * j + i / 2) + c + 2 * (i & 1)) * 32];
+          }
           if (whole) {
-            const float sum = l[x][c];
             const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // NaN stays
             __half* dst = a.out + static_cast<int64_t>(o_b_q0 + (o_row0 + r) / a.group) * a.o_st +
-                          static_cast<int64_t>(o_hk * a.group + (o_row0 + r) % a.group) * a.o_sh + 4 * g;
-#pragma unroll
-            for (int j = 0; j < G; ++j)
-              *reinterpret_cast<uint2*>(dst + 32 * j) =
-                  make_uint2(pack_half2_rn(o[x][2 * j][c] * inv, o[x][2 * j][c + 2] * inv),
-                             pack_half2_rn(o[x][2 * j + 1][c] * inv, o[x][2 * j + 1][c + 2] * inv));
+                          static_cast<int64_t>(o_hk * a.group + (o_row0 + r) % a.group) * a.o_sh + 32 * j + 4 * g;
+            *reinterpret_cast<uint2*>(dst) =
+                make_uint2(pack_half2_rn(v[0] * inv, v[1] * inv), pack_half2_rn(v[2] * inv, v[3] * inv));
           } else {
             const int64_t at = (2 * static_cast<int64_t>(blockIdx.x) + (o_chunk0 == 0 ? 1 : 0)) * kRows + r;
-            float* dst = a.part_o + at * D + 4 * g;
-#pragma unroll
-            for (int j = 0; j < G; ++j)
-              *reinterpret_cast<float4*>(dst + 32 * j) = make_float4(o[x][2 * j][c], o[x][2 * j][c + 2],
-                                                                     o[x][2 * j + 1][c], o[x][2 * j + 1][c + 2]);
-            if (g == 0) a.part_ml[at] = make_float2(m[x][c], l[x][c]);
+            *reinterpret_cast<float4*>(a.part_o + at * D + 32 * j + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
+            if (g == 0 && j == 0) a.part_ml[at] = make_float2(top, sum);
           }
         }
     }
@@ -827,7 +822,7 @@ static int check(const tm_kv4_attn_params* p) {
 template <int D, int NT>
 static cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
   constexpr int smem = kAttnWarps * kStages * kStepBlocks * Layout<D>::kBlockBytes +
-                       kAttnWarps / 2 * NT * (8 * Layout<D>::kGroups + 4) * 32 * 4;
+                       kAttnWarps * NT * (8 * Layout<D>::kGroups + 4) * 32 * 4;
   if (!allow_smem<attn_kernel<D, NT>, smem>()) return cudaErrorInvalidValue;
   attn_kernel<D, NT><<<a.ctas, kAttnThreads, smem, st>>>(a);
   cudaError_t e = cudaGetLastError();

@@ -112,10 +112,10 @@ def attention(q, keys, values, kv_len, sm_scale, causal, key_mask=None):
     """64-bit attention of one request's n query tokens [n, heads_q, dim] over keys / values [kv_len, heads_k, dim],
     and a bound on what fp16 operands may change.
 
-    Bound: scores come from the codes, as sums of q (1024 + n) that start at -1024 sum q: products of two fp16 numbers
-    are exact, their fp32 sum is rounded (or cut) three times a group of 32 channels, at 2^-22 of at most 1039 sum |q|
-    each; times the group's scale s (its range / 15) that is under 2^-10 s sum |q|. The fp32 steps that follow add
-    2^-21 sum |q| |k|. With d the sum of both, times sm_scale, a weight changes by the factor e^(2 d) (numerator and
+    Bound: scores come from the codes, s (q . n) + m sum q: products of two fp16 numbers are exact, their fp32 sums are
+    rounded (or cut) a few times at 2^-22; the sum of q over a group is held to 2^-17 of it, which is under
+    2^-10 s sum |q| with the group's scale s (its range / 15) where |m| is at most 100 s, as it is for these inputs. The
+    fp32 steps that follow add 2^-21 sum |q| |k|. With d the sum of both, times sm_scale, a weight changes by the factor e^(2 d) (numerator and
     sum). v and p are rounded to fp16 (2^-11 each; a p under 2^-14 by at most 2^-25 of the largest weight), the result
     once more; 2^-18 covers the fp32 sums and exponentials.
     """

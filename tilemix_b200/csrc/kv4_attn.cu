@@ -17,10 +17,11 @@
 //     side would fill 16. tcgen05 would need the unpacked operand written to
 //     shared memory first, which costs more than the unpacking itself;
 //   * a lane's share of a row is one shared-memory load in the order the operands
-//     want; a code becomes fp16 by OR-ing it into the mantissa of 1024 (even
-//     nibbles: 1024 + n, odd: 1024 + 16 n) and one exact add or FMA, the value by
-//     one FMA with the group's scale and minimum. That FMA rounds k and v to fp16
-//     once (the tensor core's operand type); p is rounded to fp16 as the prefill's
+//     want. Scores come from the codes themselves, masked out of the word as fp16
+//     subnormals, with scale and minimum in fp32: k is never rounded. A v is made
+//     from its code by OR-ing it into the mantissa of 1024, one exact add (or FMA)
+//     and one FMA with the group's scale and minimum, which rounds it to fp16 once
+//     (the tensor core's operand type); p is rounded to fp16 as the prefill's
 //     kernels do; scores, maxima, sums and the output accumulate in fp32.
 // Rows with no key left give 0. Keys past the length or masked are excluded by
 // selecting, and their V by zero scales, so infinities and NaN there do not leak.
@@ -117,13 +118,13 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// D = A B + C
-__device__ __forceinline__ void mma16816_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                              uint32_t b0, uint32_t b1, const float (&c)[4]) {
+// D = A B
+__device__ __forceinline__ void mma16816_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
   asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // D = A[16 x 8] B[8 x 8]
@@ -149,24 +150,25 @@ __device__ __forceinline__ uint32_t lop_and_or(uint32_t x, uint32_t m, uint32_t 
 __device__ __forceinline__ __half2 as_h2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-// Codes of a word in the mantissa of 1024: pair i holds nibbles i and i + 4, even pairs as 1024 + n, odd
-// ones as 1024 + 16 n.
+// Codes of a word as fp16 subnormals, n 2^-24 in the even pairs and 16 n 2^-24 in the odd ones: pair i holds nibbles i
+// and i + 4. One instruction a pair, and the tensor core multiplies subnormals exactly.
 __device__ __forceinline__ void spread8(uint32_t w, uint32_t (&o)[4]) {
-  const uint32_t magic = 0x64006400u, w8 = w >> 8;
-  o[0] = lop_and_or(w, 0x000F000Fu, magic);
-  o[1] = lop_and_or(w, 0x00F000F0u, magic);
-  o[2] = lop_and_or(w8, 0x000F000Fu, magic);
-  o[3] = lop_and_or(w8, 0x00F000F0u, magic);
+  const uint32_t w8 = w >> 8;
+  o[0] = w & 0x000F000Fu;
+  o[1] = w & 0x00F000F0u;
+  o[2] = w8 & 0x000F000Fu;
+  o[3] = w8 & 0x00F000F0u;
 }
 
-// The values s n + m of a word's codes as fp16 pairs (s, m of the pair's two halves).
+// The values s n + m of a word's codes as fp16 pairs (s, m of the pair's two halves): the codes in the mantissa of
+// 1024, brought to n exactly, one FMA.
 __device__ __forceinline__ void unpack8(uint32_t w, __half2 s, __half2 m, uint32_t (&o)[4]) {
   const __half2 k1024 = as_h2(0x64006400u), r16 = as_h2(0x2C002C00u), k64 = as_h2(0xD400D400u);  // 1024, 1/16, -64
-  spread8(w, o);
-  o[0] = as_u32(__hfma2(__hsub2(as_h2(o[0]), k1024), s, m));
-  o[1] = as_u32(__hfma2(__hfma2(as_h2(o[1]), r16, k64), s, m));
-  o[2] = as_u32(__hfma2(__hsub2(as_h2(o[2]), k1024), s, m));
-  o[3] = as_u32(__hfma2(__hfma2(as_h2(o[3]), r16, k64), s, m));
+  const uint32_t magic = 0x64006400u, w8 = w >> 8;
+  o[0] = as_u32(__hfma2(__hsub2(as_h2(lop_and_or(w, 0x000F000Fu, magic)), k1024), s, m));
+  o[1] = as_u32(__hfma2(__hfma2(as_h2(lop_and_or(w, 0x00F000F0u, magic)), r16, k64), s, m));
+  o[2] = as_u32(__hfma2(__hsub2(as_h2(lop_and_or(w8, 0x000F000Fu, magic)), k1024), s, m));
+  o[3] = as_u32(__hfma2(__hfma2(as_h2(lop_and_or(w8, 0x00F000F0u, magic)), r16, k64), s, m));
 }
 
 template <int N>
@@ -206,7 +208,10 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
   __shared__ __align__(8) uint64_t bars[kAttnWarps][kStages];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up; it waits for our end
+  // Set up beside the kernel before (programmatic dependent launch), whose end is waited for before anything is
+  // read; then the join may be set up in the same way.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   uint8_t* ring = smem + warp * kStages * kStageBytes;
   uint64_t* bar = bars[warp];
@@ -345,14 +350,12 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
 
   while (true) {
     // Queries as the B operand: tile x, column g = row row0 + 8 x + g, the K order of a lane's channels.
-    // Scores are formed from the codes themselves, spread into the mantissa of 1024 (two instructions a
-    // pair): q' . (1024 + n) in fp32 starting at -1024 sum q', then times the group's scale, plus its minimum
-    // times sum q' (an mma with the sum as two fp16 numbers). Channels on odd nibbles, 16 n, have q' / 16. q'
-    // is q times a power of two that brings the row's largest magnitude to [2^8, 2^9): q' / 16 keeps its bits,
-    // sums stay in fp16's range. Padding rows are 0.
+    // Scores are formed from the codes themselves, as subnormals: s (q' . n 2^-24) + m (sum q' 2^-24), the
+    // group's scale applied in fp32, its minimum in an mma with the sum as two fp16 numbers. Channels on odd
+    // nibbles, 16 n, have q' / 16. q' is q times a power of two that brings the row's largest magnitude to
+    // [2^14, 2^15): q' / 16 keeps its bits, and a sum of 32 times 2^-24 its 17 highest. Padding rows are 0.
     uint32_t qf[NT][2 * G][2], qsum[NT];
-    float no[NT][G][4];  // -1024 sum q' of columns 2 t and 2 t + 1, twice: an accumulator to start from
-    float cs[NT][2];     // log2 units a score unit of those columns
+    float cs[NT][2];     // log2 units a score unit of columns 2 t and 2 t + 1
     int lim[NT][2];                 // keys [0, lim) visible to them; padding rows see what the last row sees
     const int n_rows = rq.n_q * a.group;
 #pragma unroll
@@ -372,12 +375,13 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^(8 - floor(log2 top)) by its exponent bits
+      // 2^(14 - floor(log2 top)) by its exponent bits
       const uint32_t ex = __float_as_uint(top) >> 23;
       const bool norm = top > 0.f && top <= 65504.f;
-      const float up = norm ? __uint_as_float((262u - ex) << 23) : 1.f;
-      const float down = norm ? __uint_as_float((ex - 8u) << 23) : 1.f;
-      float sum_j = 0.f, off[G];
+      const float up = norm ? __uint_as_float((268u - ex) << 23) : 1.f;
+      const float down = norm  // its inverse, times 2^24
+                              ? __uint_as_float((ex + 10u) << 23) : 16777216.f;
+      float sum_j = 0.f;
 #pragma unroll
       for (int j = 0; j < G; ++j) {
         const float2 c01 = __half22float2(as_h2(v[j].x)), c23 = __half22float2(as_h2(v[j].y));
@@ -391,22 +395,16 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
         qf[x][2 * j + 1][1] = as_u32(p3);
         const float2 f0 = __half22float2(p0), f1 = __half22float2(p1), f2 = __half22float2(p2), f3 = __half22float2(p3);
         const float lo = f0.x + f0.y + f2.x + f2.y, hi = f1.x + f1.y + f3.x + f3.y;
-        float both = lo + hi, sum = lo + 16.f * hi;
+        float sum = lo + 16.f * hi;
 #pragma unroll
-        for (int d = 1; d <= 2; d <<= 1) {
-          both += __shfl_xor_sync(0xffffffffu, both, d);
-          sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        }
-        off[j] = -1024.f * both;
-        if (t == j) sum_j = sum;
+        for (int d = 1; d <= 2; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (t == j) sum_j = sum * 5.9604644775390625e-8f;  // 2^-24
       }
       const __half sum_hi = __float2half_rn(sum_j);
       qsum[x] = as_u32(__halves2half2(sum_hi, __float2half_rn(sum_j - __half2float(sum_hi))));
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int src = (2 * t + c) * 4;
-#pragma unroll
-        for (int j = 0; j < G; ++j) no[x][j][c] = no[x][j][c + 2] = __shfl_sync(0xffffffffu, off[j], src);
         cs[x][c] = fmaxf(a.scale_log2 * __shfl_sync(0xffffffffu, down, src), 1.17549435e-38f);  // > 0: -inf stays -inf
         const int rc = min(row0 + 8 * x + 2 * t + c, n_rows - 1);
         lim[x][c] = a.causal ? min(rq.kv, rq.kv - rq.n_q + rc / a.group + 1) : rq.kv;
@@ -463,8 +461,7 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
 #pragma unroll
           for (int x = 0; x < NT; ++x) {
             float acc[4];
-            mma16816_from(acc, pa[0], pb[0], pa[1], pb[1], qf[x][2 * j][0], qf[x][2 * j][1],
-                          no[x][j]);
+            mma16816_new(acc, pa[0], pb[0], pa[1], pb[1], qf[x][2 * j][0], qf[x][2 * j][1]);
             mma16816(acc, pa[2], pb[2], pa[3], pb[3], qf[x][2 * j + 1][0], qf[x][2 * j + 1][1]);
             sc[u][x][0] = fmaf(fa, acc[0], sc[u][x][0]);
             sc[u][x][1] = fmaf(fa, acc[1], sc[u][x][1]);
@@ -707,46 +704,54 @@ __global__ void __launch_bounds__(kAttnThreads) join_kernel(const AttnArgs a) {
   constexpr int V = D / 32;  // channels a lane
   __shared__ float sh_o[kAttnWarps][D], sh_m[kAttnWarps], sh_l[kAttnWarps];
   const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Request rq = request_of<NT>(a, b);
+  const Request rq = request_of<NT>(a, b);  // inputs: there since before the attention kernel began
   const int i = blockIdx.x;
+  // The attention kernel has ended, its writes are visible. Every CTA waits, those without a row too: the join must
+  // not be over before the attention is.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (i >= rq.n_q * a.heads_q) return;
   const int token = i / a.heads_q, hq = i - token * a.heads_q;
   const int hk = hq / a.group, row = token * a.group + hq - hk * a.group;
   const int tile = row / (8 * NT), r = row - tile * (8 * NT);
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the attention kernel has ended, its writes are visible
   const int total = a.starts[a.batch], per = (total + a.ctas - 1) / a.ctas;
   const int first = a.starts[b] + (hk * rq.tiles + tile) * rq.chunks;
   const int c0 = first / per, c1 = (first + rq.chunks - 1) / per;
   if (c0 == c1) return;  // one CTA had it whole and wrote it
   auto slot = [&](int c) { return (2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * (8 * NT) + r; };
-  // Each warp with a running maximum of its own, four parts in flight.
+  // Each warp with a running maximum of its own, kFlight parts in flight.
+  constexpr int kFlight = 8;
+  using Vec = std::conditional_t<V == 4, float4, float2>;
   float acc[V] = {}, sum = 0.f, top = -CUDART_INF_F;
-  for (int c = c0 + warp; c <= c1; c += 4 * kAttnWarps) {
-    float2 ml[4];
-    float v[4][V];
+  for (int c = c0 + warp; c <= c1; c += kFlight * kAttnWarps) {
+    float2 ml[kFlight];
+    Vec v[kFlight];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int64_t at = slot(min(c + k * kAttnWarps, c1));
-      ml[k] = a.part_ml[at];
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[k][e] = a.part_o[at * D + lane * V + e];
-      if (c + k * kAttnWarps > c1) ml[k] = make_float2(-CUDART_INF_F, 0.f);
+    for (int k = 0; k < kFlight; ++k) {
+      const int at_c = c + k * kAttnWarps;
+      ml[k] = make_float2(-CUDART_INF_F, 0.f);
+      v[k] = Vec{};
+      if (at_c <= c1) {
+        const int64_t at = slot(at_c);
+        ml[k] = a.part_ml[at];
+        v[k] = *reinterpret_cast<const Vec*>(a.part_o + at * D + lane * V);
+      }
     }
     float now = top;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) now = fmaxf(now, ml[k].x);
+    for (int k = 0; k < kFlight; ++k) now = fmaxf(now, ml[k].x);
     const float ref = now == -CUDART_INF_F ? 0.f : now;
     const float keep = ex2_approx(top - ref);
     sum *= keep;
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] *= keep;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (c + k * kAttnWarps > c1) break;
-      const float f = ex2_approx(ml[k].x - ref);
+    for (int k = 0; k < kFlight; ++k) {
+      const float f = ex2_approx(ml[k].x - ref);  // 0 for a part that is not there
+      const float* ve = reinterpret_cast<const float*>(&v[k]);
       sum += f * ml[k].y;
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] += f * v[k][e];
+      for (int e = 0; e < V; ++e) acc[e] += f * ve[e];
     }
     top = now;
   }
@@ -824,20 +829,21 @@ static cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
   constexpr int smem = kAttnWarps * kStages * kStepBlocks * Layout<D>::kBlockBytes +
                        kAttnWarps * NT * (8 * Layout<D>::kGroups + 4) * 32 * 4;
   if (!allow_smem<attn_kernel<D, NT>, smem>()) return cudaErrorInvalidValue;
-  attn_kernel<D, NT><<<a.ctas, kAttnThreads, smem, st>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  // The join is set up while the attention runs (programmatic dependent launch) and waits for its end.
+  // Both kernels are set up while the one before them ends (programmatic dependent launch) and wait for it.
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(a.max_q) * a.heads_q),
-                     static_cast<unsigned>(a.batch));
-  cfg.blockDim = dim3(kAttnThreads);
-  cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
+  cfg.stream = st;
+  cfg.blockDim = dim3(kAttnThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(a.ctas));
+  cfg.dynamicSmemBytes = smem;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_kernel<D, NT>, a);
+  if (e != cudaSuccess) return e;
+  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(a.max_q) * a.heads_q), static_cast<unsigned>(a.batch));
+  cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, join_kernel<D, NT>, a);
 }
 

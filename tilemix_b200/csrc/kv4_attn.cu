@@ -44,6 +44,9 @@ constexpr int kStepBlocks = 2;                        // 16-key blocks a step
 constexpr int kStepKeys = kStepBlocks * kBlockTokens;
 constexpr int kChunkKeys = kStepKeys * kAttnWarps;    // keys of one step of every warp: the unit of work
 constexpr int kSms = 148;
+// What a run of chunks costs beside its chunks (queries, pages, merge and store), in chunks. Without it a CTA
+// with several short requests was the last to end: 64 requests of 512 to 8192 keys took 94 us, 82 so (89 with 1, 83 with 2).
+constexpr int kSetup = 4;
 
 // CTAs an SM of the kernel for head_dim d and nt row tiles, by registers and shared memory.
 constexpr int resident(int d, int nt) { return d == 128 && nt == 2 ? 2 : 3; }
@@ -85,6 +88,7 @@ struct Request {
   int kv;        // its keys
   int tiles;     // row tiles a KV head
   int chunks;    // chunks of kChunkKeys keys of one (KV head, row tile), at least 1
+  int cost;      // those and kSetup, times the KV heads and row tiles: its length in the work list
 };
 
 template <int NT>
@@ -100,6 +104,7 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, int b) {
   r.kv = static_cast<int>(min(static_cast<int64_t>(max(a.kv_lens[b], 0)), a.max_kv));
   r.tiles = (r.n_q * a.group + 8 * NT - 1) / (8 * NT);
   r.chunks = max(1, (r.kv + kChunkKeys - 1) / kChunkKeys);
+  r.cost = r.tiles * a.heads_k * (r.chunks + kSetup);
   return r;
 }
 
@@ -191,8 +196,8 @@ __device__ __forceinline__ Words<N> load_words(const uint8_t* p) {
   return r;
 }
 
-// The work of a call is the list of all chunks: by request, then KV head, then row tile, then key. CTA c takes
-// chunks [c per, (c + 1) per), whatever requests they belong to, so ragged lengths leave no CTA behind; a
+// The work of a call is the list of all chunks: by request, then KV head, then row tile, then key, with kSetup
+// places in front of each (KV head, row tile). CTA c takes places [c per, (c + 1) per), whatever requests they belong to, so ragged lengths leave no CTA behind; a
 // (KV head, row tile) that several CTAs share leaves partial states for the join, one that a CTA has whole is
 // written at once. A CTA's first run of chunks may continue another's (slot 2 c), its last may be continued
 // (slot 2 c + 1).
@@ -226,7 +231,7 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
   int mine = 0;
   for (int b = rb0; b < rb1; ++b) {
     const Request r = request_of<NT>(a, b);
-    mine += r.tiles * a.heads_k * r.chunks;
+    mine += r.cost;
   }
   int inc = mine;
 #pragma unroll
@@ -243,7 +248,7 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
     for (int b = rb0; b < rb1; ++b) {
       a.starts[b] = at;
       const Request r = request_of<NT>(a, b);
-      at += r.tiles * a.heads_k * r.chunks;
+      at += r.cost;
       if (r.kv < a.kv_lens[b]) record_error(a.err, kErrCachePlan);  // longer than it may be
     }
     if (lane == 0) a.starts[a.batch] = total;
@@ -256,9 +261,8 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
     b_start = inc - mine;
     while (true) {
       const Request r = request_of<NT>(a, b);
-      const int n = r.tiles * a.heads_k * r.chunks;
-      if (pos < b_start + n) break;
-      b_start += n;
+      if (pos < b_start + r.cost) break;
+      b_start += r.cost;
       ++b;
     }
   }
@@ -268,11 +272,15 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
 
   // The current run of chunks: one (request, KV head, row tile), keys [key0, key1).
   int hk, row0, chunk0, n_chunks, key0, blk1, steps;
+  // false: the CTA's range ends in front of the next chunk
   auto locate = [&]() {
     const int off = pos - b_start;
-    const int unit = off / rq.chunks;
-    chunk0 = off - unit * rq.chunks;
-    n_chunks = min(rq.chunks - chunk0, end - pos);
+    const int unit = off / (rq.chunks + kSetup), in_unit = off - unit * (rq.chunks + kSetup);
+    const int lead = max(0, kSetup - in_unit);
+    chunk0 = max(0, in_unit - kSetup);
+    n_chunks = min(rq.chunks - chunk0, end - pos - lead);
+    if (n_chunks <= 0) return false;
+    pos += lead + n_chunks;
     hk = unit / rq.tiles;
     row0 = (unit - hk * rq.tiles) * kRows;
     key0 = chunk0 * kChunkKeys;
@@ -280,8 +288,9 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
     blk1 = (key1 + kBlockTokens - 1) / kBlockTokens;
     const int all_steps = (blk1 - key0 / kBlockTokens + kStepBlocks - 1) / kStepBlocks;
     steps = all_steps > warp ? (all_steps - warp + kAttnWarps - 1) / kAttnWarps : 0;
+    return true;
   };
-  locate();
+  if (!locate()) return;
 
   // Bulk copies of the warp's steps: blocks key0 / 16 + 2 (warp + kAttnWarps i). Each lane looks up one step of
   // the next 32 (its pages, the addresses of its blocks) and issues that step's copies itself when its turn
@@ -434,10 +443,27 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
       for (int c = 0; c < 2; ++c) m[x][c] = limit[x][c] = -CUDART_INF_F, mc[x][c] = 0.f, l[x][c] = 0.f;
     }
 
-    // One step: 32 keys from stage s. With kPlain every key counts for every row.
-    auto step = [&](auto plain_tag, const int key, const uint32_t live) {
-      constexpr bool kPlain = decltype(plain_tag)::value;
-      const uint8_t* st = ring + s * kStageBytes;
+    // One step: 32 keys from stage s. `plain`: every key counts for every row; `live`: those that count for any.
+    // What a step does for keys that do not count is kept to two short branches: a second copy of the whole step
+    // without them ran no faster where it was used, and the last step of every run then met cold instructions
+    // (64 ragged requests 96 us, 84 with lengths that fill their steps).
+    auto step = [&](const bool plain, const int key, const uint32_t live) {
+      uint8_t* st = ring + s * kStageBytes;
+      if (!plain) {
+        // The V scales and minima of keys that count for no row become 0, so that nothing of them (infinities, NaN,
+        // what an absent block's stage happens to hold) reaches the output.
+        const int tok = lane % kBlockTokens;
+        if (!((live >> lane) & 1)) {
+          uint8_t* vs = st + lane / kBlockTokens * L::kBlockBytes + L::kOffVScale;
+#pragma unroll
+          for (int j = 0; j < G; ++j) {
+            *reinterpret_cast<uint16_t*>(vs + L::v_scale(j, tok)) = 0;
+            *reinterpret_cast<uint16_t*>(vs + L::v_scale(j, tok) + 8) = 0;
+          }
+        }
+        fence_proxy_async_smem();  // before the next copy into this stage
+        __syncwarp();
+      }
 
       float sc[kStepBlocks][NT][4];
 #pragma unroll
@@ -471,7 +497,7 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
         }
       }
 
-      if constexpr (!kPlain) {
+      if (!plain) {
         const uint32_t on = live >> tok_g;
 #pragma unroll
         for (int x = 0; x < NT; ++x)
@@ -544,21 +570,9 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
         Words<W> v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = load_words<W>(blk + (t + 4 * k) * L::kRowBytes + g * (2 * G));
-        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-        if constexpr (!kPlain) {
-          const uint32_t on = live >> (kBlockTokens * u + t);
-          keep0 = ((on & 1u) ? 0xffffu : 0u) | ((on & 0x10u) ? 0xffff0000u : 0u);
-          keep1 = ((on & 0x100u) ? 0xffffu : 0u) | ((on & 0x1000u) ? 0xffff0000u : 0u);
-        }
 #pragma unroll
         for (int j = 0; j < G; ++j) {
-          Words<4> vs = load_words<4>(blk + 16 * L::kRowBytes + (j * 4 + t) * 16);
-          if constexpr (!kPlain) {
-            vs.w[0] &= keep0;
-            vs.w[1] &= keep1;
-            vs.w[2] &= keep0;
-            vs.w[3] &= keep1;
-          }
+          const Words<4> vs = load_words<4>(blk + 16 * L::kRowBytes + (j * 4 + t) * 16);
           const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
           uint32_t e[4], f[4];
           unpack8(__byte_perm(v[0].w[j / 2], v[1].w[j / 2], sel), as_h2(vs.w[0]), as_h2(vs.w[2]), e);
@@ -596,10 +610,7 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
         ok = false;
         break;
       }
-      if (plain)
-        step(std::true_type{}, key, live);
-      else
-        step(std::false_type{}, key, live);
+      step(plain, key, live);
       __syncwarp();  // every lane has read the stage
       if (++s == kStages) s = 0, phase ^= 1;
       if (issued < steps) issue();
@@ -614,14 +625,15 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
     // The next run's copies start before this run's states are merged and written.
     const int o_b_q0 = rq.q0, o_row0 = row0, o_hk = hk, o_chunk0 = chunk0;
     const bool whole = chunk0 == 0 && n_chunks == rq.chunks;
-    pos += n_chunks;
-    const bool more = pos < end;
+    bool more = pos < end;
     if (more) {
-      while (pos >= b_start + rq.tiles * a.heads_k * rq.chunks) {
-        b_start += rq.tiles * a.heads_k * rq.chunks;
+      while (pos >= b_start + rq.cost) {
+        b_start += rq.cost;
         rq = request_of<NT>(a, ++b);
       }
-      locate();
+      more = locate();
+    }
+    if (more) {
       issued = 0;
       while (issued < steps && issued < kStages) issue();
     }
@@ -715,7 +727,7 @@ __global__ void __launch_bounds__(kAttnThreads) join_kernel(const AttnArgs a) {
   const int hk = hq / a.group, row = token * a.group + hq - hk * a.group;
   const int tile = row / (8 * NT), r = row - tile * (8 * NT);
   const int total = a.starts[a.batch], per = (total + a.ctas - 1) / a.ctas;
-  const int first = a.starts[b] + (hk * rq.tiles + tile) * rq.chunks;
+  const int first = a.starts[b] + (hk * rq.tiles + tile) * (rq.chunks + kSetup) + kSetup;
   const int c0 = first / per, c1 = (first + rq.chunks - 1) / per;
   if (c0 == c1) return;  // one CTA had it whole and wrote it
   auto slot = [&](int c) { return (2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * (8 * NT) + r; };
@@ -790,7 +802,7 @@ static Plan plan_of(const tm_kv4_attn_params* p) {
   const int64_t rows = static_cast<int64_t>(p->max_seqlen_q) * (p->heads_q / p->heads_k);
   r.nt = rows > 8 ? 2 : 1;
   const int64_t tiles = (rows + 8 * r.nt - 1) / (8 * r.nt);
-  const int64_t chunks = p->max_kv_len / kChunkKeys + 1;
+  const int64_t chunks = p->max_kv_len / kChunkKeys + 1 + kSetup;
   const int64_t most = static_cast<int64_t>(p->batch) * p->heads_k * tiles;
   const int64_t slots = kSms * resident(p->head_dim, r.nt);
   r.ctas = static_cast<int>(most >= slots || chunks >= slots || most * chunks >= slots ? slots : most * chunks);
@@ -820,7 +832,7 @@ static int check(const tm_kv4_attn_params* p) {
   if (!(p->sm_scale > 0.f) || p->sm_scale > 3.4028235e38f) return TM_ERR_SHAPE;  // maxima are taken before scaling
   // the chunks of the work list are counted in 32 bits, with room for the last CTA's end
   const double rows = static_cast<double>(p->max_seqlen_q) * p->heads_q;
-  if (p->batch * (rows / 8 + p->heads_k) * (p->max_kv_len / kChunkKeys + 1.0) > 2147480000.0) return TM_ERR_UNSUPPORTED;
+  if (p->batch * (rows / 8 + p->heads_k) * (p->max_kv_len / kChunkKeys + 1.0 + kSetup) > 2147480000.0) return TM_ERR_UNSUPPORTED;
   return TM_OK;
 }
 

@@ -180,25 +180,41 @@ def lib() -> ctypes.CDLL:
     return _LIB
 
 
-def launch(name: str, device, *args) -> None:
-    """Call an entry point that ends in (error word, stream) on ``device`` (a CUDA ``torch.device``
-    with an index) and the stream that is current there; raises what the status says. Calls of a
-    few microseconds are made through here, so it looks things up once and switches the device
-    only if it has to."""
+def launcher(name: str):
+    """``call(index, *args)``: the entry point ``name``, which ends in (error word, stream), called for CUDA
+    device ``index`` on the stream that is current there; raises what the status says. Calls of a few
+    microseconds are made through here, so what can be looked up once is."""
+    fn = None
+
+    def call(index: int, *args) -> None:
+        nonlocal fn
+        if fn is None:
+            fn = getattr(lib(), name)
+        word = _ERROR_WORD_PTRS.get(index) or error_word_ptr(index)
+        if index == _current_device():
+            rc = fn(*args, word, _current_stream(index))
+        else:
+            import torch
+
+            with torch.cuda.device(index):
+                rc = fn(*args, word, _current_stream(index))
+        if rc:
+            check(rc, name)
+
+    return call
+
+
+def _current_device() -> int:
+    """The current CUDA device's index (replaced by torch's own function on the first call)."""
+    global _current_device, _current_stream
     import torch
 
-    index = device.index
-    args += (error_word_ptr(index), torch._C._cuda_getCurrentRawStream(index))
-    fn = getattr(_LIB or lib(), name)
-    if index == torch._C._cuda_getDevice():
-        rc = fn(*args)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args)
-    if rc:
-        check(rc, name)
+    torch.cuda.init()
+    _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    return _current_device()
 
 
+_current_stream = None
 _ERROR_WORD_PTRS: dict[int, int] = {}
 
 

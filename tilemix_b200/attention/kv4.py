@@ -25,7 +25,7 @@ from typing import NamedTuple, Optional
 import torch
 from torch import Tensor
 
-from tilemix_b200._lib import TmBlockTablesParams, TmKv4AttnParams, check, launch, lib, packer
+from tilemix_b200._lib import TmBlockTablesParams, TmKv4AttnParams, check, launcher, lib, packer
 
 __all__ = ["BlockTables", "build_block_tables", "release_pages", "kv4_pool", "kv4_append", "kv4_read",
            "kv4_attention"]
@@ -33,6 +33,9 @@ __all__ = ["BlockTables", "build_block_tables", "release_pages", "kv4_pool", "kv
 _HEAD_DIMS = (64, 128)
 _pack_tables = packer(TmBlockTablesParams)
 _pack_attn = packer(TmKv4AttnParams)
+_launch_tables, _launch_release = launcher("tm_build_block_tables"), launcher("tm_release_pages")
+_launch_append, _launch_read = launcher("tm_kv4_append"), launcher("tm_kv4_read")
+_launch_attn = launcher("tm_kv4_attn")
 
 
 class BlockTables(NamedTuple):
@@ -50,13 +53,15 @@ def _check_page_size(page_size: int) -> None:
         raise ValueError(f"page_size must be a positive multiple of 16, got {page_size}")
 
 
-def _check_device_int(name: str, t: Tensor, dtype: torch.dtype, device, ndim: int = 1) -> None:
-    if t.dtype != dtype:
+def _check(name: str, t: Tensor, dtype: torch.dtype, index: int, ndim: int = 1) -> None:
+    """A control tensor of a call on CUDA device ``index``: its type, device and layout."""
+    if t.dtype is dtype and t.ndim == ndim and t.get_device() == index and (t.stride(-1) == 1 or not t.numel()):
+        return
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}")
-    if t.device != device:
+    if t.get_device() != index:
         raise ValueError("all tensors of a call must share one CUDA device")
-    if t.ndim != ndim or (t.numel() and t.stride(-1) != 1):
-        raise ValueError(f"{name} must have {ndim} dimension{'s' * (ndim > 1)}, the last one contiguous")
+    raise ValueError(f"{name} must have {ndim} dimension{'s' * (ndim > 1)}, the last one contiguous")
 
 
 def build_block_tables(cached_lens: Tensor, new_lens: Tensor, block_table: Tensor, free_pages: Tensor,
@@ -77,12 +82,12 @@ def build_block_tables(cached_lens: Tensor, new_lens: Tensor, block_table: Tenso
     """
     if not cached_lens.is_cuda:
         raise RuntimeError("the block tables are built by a CUDA kernel")
-    device = cached_lens.device
-    _check_device_int("cached_lens", cached_lens, torch.int32, device)
-    _check_device_int("new_lens", new_lens, torch.int32, device)
-    _check_device_int("block_table", block_table, torch.int32, device, 2)
-    _check_device_int("free_pages", free_pages, torch.int32, device)
-    _check_device_int("free_span", free_span, torch.int64, device)
+    index = cached_lens.get_device()
+    _check("cached_lens", cached_lens, torch.int32, index)
+    _check("new_lens", new_lens, torch.int32, index)
+    _check("block_table", block_table, torch.int32, index, 2)
+    _check("free_pages", free_pages, torch.int32, index)
+    _check("free_span", free_span, torch.int64, index)
     _check_page_size(page_size)
     batch = cached_lens.numel()
     if new_lens.numel() != batch or block_table.shape[0] != batch or free_span.numel() != 2:
@@ -91,16 +96,15 @@ def build_block_tables(cached_lens: Tensor, new_lens: Tensor, block_table: Tenso
         raise ValueError("at most 8192 requests")
     if not 0 <= max_new_tokens < 2**31:
         raise ValueError("max_new_tokens must be in [0, 2^31)")
-    slots = torch.empty(max_new_tokens, dtype=torch.int64, device=device)
-    positions = torch.empty(max_new_tokens, dtype=torch.int32, device=device)
-    cu = torch.empty(batch + 1, dtype=torch.int32, device=device)
-    kv_lens = torch.empty(batch, dtype=torch.int32, device=device)
-    span = torch.empty(2, dtype=torch.int64, device=device)
-    launch("tm_build_block_tables", device,
-           _pack_tables(cached_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-                        block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_span.data_ptr(), batch,
-                        page_size, max_new_tokens, slots.data_ptr(), positions.data_ptr(), cu.data_ptr(),
-                        kv_lens.data_ptr(), span.data_ptr()))
+    # one allocation, slots and positions on 16 bytes
+    n, wide = 2 * max_new_tokens, (max_new_tokens + 3) // 4 * 8
+    slots, _, span, positions, cu, kv_lens = cached_lens.new_empty(
+        wide + 4 + max_new_tokens + 2 * batch + 1).split_with_sizes((n, wide - n, 4, max_new_tokens, batch + 1, batch))
+    slots, span = slots.view(torch.int64), span.view(torch.int64)
+    _launch_tables(index, _pack_tables(
+        cached_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+        free_pages.data_ptr(), free_pages.numel(), free_span.data_ptr(), batch, page_size, max_new_tokens,
+        slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), kv_lens.data_ptr(), span.data_ptr()))
     return BlockTables(slots, positions, cu, kv_lens, span)
 
 
@@ -111,17 +115,17 @@ def release_pages(lens: Tensor, done: Tensor, block_table: Tensor, free_pages: T
     entries become -1 and its length 0; ``free_span[1]`` grows by their number."""
     if not lens.is_cuda:
         raise RuntimeError("the pages are released by a CUDA kernel")
-    device = lens.device
-    _check_device_int("lens", lens, torch.int32, device)
-    _check_device_int("done", done, torch.bool, device)
-    _check_device_int("block_table", block_table, torch.int32, device, 2)
-    _check_device_int("free_pages", free_pages, torch.int32, device)
-    _check_device_int("free_span", free_span, torch.int64, device)
+    index = lens.get_device()
+    _check("lens", lens, torch.int32, index)
+    _check("done", done, torch.bool, index)
+    _check("block_table", block_table, torch.int32, index, 2)
+    _check("free_pages", free_pages, torch.int32, index)
+    _check("free_span", free_span, torch.int64, index)
     _check_page_size(page_size)
     batch = lens.numel()
     if done.numel() != batch or block_table.shape[0] != batch or free_span.numel() != 2:
         raise ValueError("lens, done and block_table must agree on the batch, free_span has two entries")
-    launch("tm_release_pages", device, lens.data_ptr(), done.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+    _launch_release(index, lens.data_ptr(), done.data_ptr(), block_table.data_ptr(), block_table.stride(0),
            block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_span.data_ptr(), batch, page_size)
 
 
@@ -140,19 +144,20 @@ def kv4_pool(num_pages: int, page_size: int, kv_heads: int, head_dim: int, devic
                        device="cuda" if device is None else device)
 
 
-def _pool_page_size(pool: Tensor, heads: int, head_dim: int, device) -> int:
-    """The page size of a pool that holds ``heads`` KV heads of ``head_dim``; raises if it cannot."""
+def _pool_pages(pool: Tensor, heads: Optional[int], head_dim: int, index: int) -> tuple[int, int, int]:
+    """(pages, KV heads, page size) of a pool that holds ``heads`` KV heads of ``head_dim``; raises if it cannot."""
     if head_dim not in _HEAD_DIMS:
         raise ValueError("the 4-bit cache supports head_dim 64 and 128")
-    if pool.dtype != torch.uint8 or pool.ndim != 3 or not pool.is_contiguous():
+    if pool.dtype is not torch.uint8 or pool.ndim != 3 or not pool.is_contiguous():
         raise TypeError("pool must be a contiguous uint8 [pages, kv_heads, page bytes] tensor (kv4_pool)")
-    if pool.device != device:
+    if pool.get_device() != index:
         raise ValueError("all tensors of a call must share one CUDA device")
-    if pool.shape[1] != heads:
-        raise ValueError(f"pool has {pool.shape[1]} KV heads, expected {heads}")
-    if pool.shape[2] == 0 or pool.shape[2] % (20 * head_dim):
-        raise ValueError(f"a pool row of {pool.shape[2]} bytes does not hold whole blocks of head_dim {head_dim}")
-    return pool.shape[2] // (20 * head_dim) * 16
+    pages, heads_k, row = pool.shape
+    if heads is not None and heads_k != heads:
+        raise ValueError(f"pool has {heads_k} KV heads, expected {heads}")
+    if row == 0 or row % (20 * head_dim):
+        raise ValueError(f"a pool row of {row} bytes does not hold whole blocks of head_dim {head_dim}")
+    return pages, heads_k, row // (20 * head_dim) * 16
 
 
 def kv4_append(k: Tensor, v: Tensor, pool: Tensor, slots: Tensor) -> None:
@@ -162,38 +167,39 @@ def kv4_append(k: Tensor, v: Tensor, pool: Tensor, slots: Tensor) -> None:
     reads back as NaN."""
     if not k.is_cuda:
         raise RuntimeError("the cache is written by a CUDA kernel")
-    device = k.device
+    index = k.get_device()
     if k.ndim != 3 or v.ndim != 3:
         raise ValueError("expected [tokens, kv_heads, head_dim] tensors")
     if v.shape != k.shape:
         raise ValueError("K and V shapes must match")
-    if v.device != device:
+    if v.get_device() != index:
         raise ValueError("all tensors of a call must share one CUDA device")
     if k.dtype != torch.float16 or v.dtype != torch.float16:
         raise TypeError("the sm_100a cache kernels take fp16; k and v must be torch.float16")
     n, heads, d = k.shape
-    page_size = _pool_page_size(pool, heads, d, device)
-    _check_device_int("slots", slots, torch.int64, device)
+    pages, _, page_size = _pool_pages(pool, heads, d, index)
+    _check("slots", slots, torch.int64, index)
     if slots.numel() != n:
         raise ValueError(f"{slots.numel()} slots for {n} tokens")
-    if n and (k.stride(2) != 1 or v.stride(2) != 1):
+    k_tok, k_head, k_dim = k.stride()
+    v_tok, v_head, v_dim = v.stride()
+    if n and (k_dim != 1 or v_dim != 1):
         raise ValueError("the head dimension must be contiguous")
-    launch("tm_kv4_append", device, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), n,
-           slots.data_ptr(), pool.data_ptr(), pool.shape[0], heads, d, page_size)
+    _launch_append(index, k.data_ptr(), k_tok, k_head, v.data_ptr(), v_tok, v_head, n, slots.data_ptr(),
+                   pool.data_ptr(), pages, heads, d, page_size)
 
 
 def kv4_read(pool: Tensor, slots: Tensor, head_dim: int) -> tuple[Tensor, Tensor]:
     """The cached keys and values at ``slots`` (int64; -1 gives zeros) as fp16 [slots, kv_heads, head_dim]."""
     if not pool.is_cuda:
         raise RuntimeError("the cache is read by a CUDA kernel")
-    device = pool.device
-    page_size = _pool_page_size(pool, pool.shape[1] if pool.ndim == 3 else 0, head_dim, device)
-    _check_device_int("slots", slots, torch.int64, device)
-    n, heads = slots.numel(), pool.shape[1]
-    k = torch.empty((n, heads, head_dim), dtype=torch.float16, device=device)
-    v = torch.empty_like(k)
-    launch("tm_kv4_read", device, pool.data_ptr(), pool.shape[0], heads, head_dim, page_size, slots.data_ptr(), n,
-           k.data_ptr(), v.data_ptr())
+    index = pool.get_device()
+    pages, heads, page_size = _pool_pages(pool, None, head_dim, index)
+    _check("slots", slots, torch.int64, index)
+    n = slots.numel()
+    k, v = pool.new_empty((2, n, heads, 2 * head_dim)).view(torch.float16)
+    _launch_read(index, pool.data_ptr(), pages, heads, head_dim, page_size, slots.data_ptr(), n, k.data_ptr(),
+                 v.data_ptr())
     return k, v
 
 
@@ -209,42 +215,45 @@ def kv4_attention(q: Tensor, pool: Tensor, block_table: Tensor, kv_lens: Tensor,
     of a request's n query tokens sees the keys up to position ``kv_len - n + i``. ``key_mask`` (bool
     [batch, columns], optional) excludes keys for every row of a request; a key behind its last
     column is excluded too. A row that sees no key is 0. ``max_kv_len`` bounds ``kv_lens`` on the
-    host (default: the table's capacity); a close bound gives a better split of the key axis. Rows
-    of ``q`` that belong to no request are left as they were in ``out``.
+    host (default: the table's capacity); keys beyond it are left out (``device_error_code`` 11), and a
+    small bound makes for a small launch. Rows of ``q`` that belong to no request are left as they
+    were in ``out``.
     """
     if not q.is_cuda:
         raise RuntimeError("the cache attention is a CUDA kernel")
-    device = q.device
-    if q.ndim != 3 or pool.ndim != 3:
-        raise ValueError("expected q [rows, heads, head_dim] and pool [pages, kv_heads, page bytes]")
-    if q.dtype != torch.float16:
+    index = q.get_device()
+    if q.ndim != 3:
+        raise ValueError("expected q [rows, heads, head_dim]")
+    if q.dtype is not torch.float16:
         raise TypeError("the sm_100a cache kernels take fp16; q must be torch.float16")
     rows, heads, d = q.shape
-    heads_k = pool.shape[1]
-    page_size = _pool_page_size(pool, heads_k, d, device)
-    if heads % heads_k:
+    pages, heads_k, page_size = _pool_pages(pool, None, d, index)
+    if heads_k == 0 or heads % heads_k:
         raise ValueError("Q heads must be divisible by KV heads")
-    _check_device_int("block_table", block_table, torch.int32, device, 2)
-    _check_device_int("kv_lens", kv_lens, torch.int32, device)
+    _check("block_table", block_table, torch.int32, index, 2)
+    _check("kv_lens", kv_lens, torch.int32, index)
     batch, cols = block_table.shape
     if kv_lens.numel() != batch:
         raise ValueError("block_table and kv_lens must agree on the batch")
     if cu_seqlens_q is not None:
-        _check_device_int("cu_seqlens_q", cu_seqlens_q, torch.int32, device)
+        _check("cu_seqlens_q", cu_seqlens_q, torch.int32, index)
         if cu_seqlens_q.numel() != batch + 1:
             raise ValueError("cu_seqlens_q must have batch + 1 entries")
     elif rows != batch or max_seqlen_q != 1:
         raise ValueError("without cu_seqlens_q there is one query row a request")
     if key_mask is not None:
-        _check_device_int("key_mask", key_mask, torch.bool, device, 2)
+        _check("key_mask", key_mask, torch.bool, index, 2)
         if key_mask.shape[0] != batch:
             raise ValueError("key_mask must have a row for each request")
-    if rows and q.stride(2) != 1:
+    q_tok, q_head, q_dim = q.stride()
+    if rows and q_dim != 1:
         raise ValueError("the head dimension must be contiguous")
     if out is None:
-        out = torch.empty((rows, heads, d), dtype=torch.float16, device=device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or (rows and out.stride(2) != 1):
-        raise ValueError("out must match q")
+        out, o_tok, o_head = q.new_empty((rows, heads, d)), heads * d, d
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or out.get_device() != index or (rows and out.stride(2) != 1):
+            raise ValueError("out must match q")
+        o_tok, o_head, _ = out.stride()
     scale = d ** -0.5 if sm_scale is None else float(sm_scale)
     if not 0 < scale < float("inf"):
         raise ValueError("sm_scale must be positive and finite")
@@ -252,23 +261,21 @@ def kv4_attention(q: Tensor, pool: Tensor, block_table: Tensor, kv_lens: Tensor,
     bound = capacity if max_kv_len is None else min(max(int(max_kv_len), 0), capacity)
     mask = (0, 0, 0) if key_mask is None else (key_mask.data_ptr(), key_mask.stride(0), key_mask.shape[1])
     # From the allocator on the call's own stream: two streams or graphs never share it.
-    nbytes = _workspace_bytes(batch, rows, heads, heads_k, d, page_size, cols, max_seqlen_q, bound)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    launch("tm_kv4_attn", device,
-           _pack_attn(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), rows,
-                      pool.data_ptr(), pool.shape[0], block_table.data_ptr(), block_table.stride(0), cols, page_size,
-                      kv_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), *mask, batch, heads,
-                      heads_k, d, max_seqlen_q, bound, bool(causal), scale),
-           work.data_ptr(), nbytes)
+    nbytes = _workspace_bytes(batch, heads, heads_k, d, max_seqlen_q, bound)
+    work = pool.new_empty(nbytes)
+    _launch_attn(index, _pack_attn(
+        q.data_ptr(), q_tok, q_head, out.data_ptr(), o_tok, o_head, rows, pool.data_ptr(), pages,
+        block_table.data_ptr(), block_table.stride(0), cols, page_size, kv_lens.data_ptr(),
+        0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), *mask, batch, heads, heads_k, d, max_seqlen_q, bound,
+        bool(causal), scale), work.data_ptr(), nbytes)
     return out
 
 
 @lru_cache(maxsize=256)
-def _workspace_bytes(batch: int, rows: int, heads: int, heads_k: int, d: int, page_size: int, cols: int,
-                     max_seqlen_q: int, bound: int) -> int:
-    """Workspace of an attention call; it depends on these sizes alone (stand-in pointers, never read)."""
+def _workspace_bytes(batch: int, heads: int, heads_k: int, d: int, max_seqlen_q: int, bound: int) -> int:
+    """Workspace of an attention call; it depends on these sizes alone (the others and the pointers stand in)."""
     at, need = 1 << 20, ctypes.c_int64()
-    args = _pack_attn(at, d, d, at, d, d, rows, at, 1, at, cols, cols, page_size, at, at, 0, 0, 0, batch, heads, heads_k,
-                      d, max_seqlen_q, bound, 1, 1.0)
+    args = _pack_attn(at, d, d, at, d, d, max(batch, 1), at, 1, at, 1, 1, 16, at, at, 0, 0, 0, batch, heads, heads_k, d,
+                      max_seqlen_q, bound, 1, 1.0)
     check(lib().tm_kv4_attn_workspace(args, ctypes.byref(need)), "tm_kv4_attn")
     return need.value

@@ -19,11 +19,13 @@ from typing import Optional
 import torch
 from torch import Tensor, nn
 
-from tilemix_b200._lib import TM_DTYPE_BF16, TM_DTYPE_FP16, TM_DTYPE_FP32, launch
+from tilemix_b200._lib import TM_DTYPE_BF16, TM_DTYPE_FP16, TM_DTYPE_FP32, launcher
 
 __all__ = ["quantize_per_token_int8", "int8_matmul", "int8_linear", "Int8Linear"]
 
 _DTYPES = {torch.float16: TM_DTYPE_FP16, torch.bfloat16: TM_DTYPE_BF16, torch.float32: TM_DTYPE_FP32}
+_launch_quant, _launch_matmul = launcher("tm_quant_per_token_int8"), launcher("tm_int8_matmul")
+_launch_linear = launcher("tm_int8_linear")
 
 
 def quantize_per_token_int8(x: Tensor) -> tuple[Tensor, Tensor]:
@@ -40,24 +42,27 @@ def quantize_per_token_int8(x: Tensor) -> tuple[Tensor, Tensor]:
     rows, cols = x.shape
     codes = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    launch("tm_quant_per_token_int8", x.device, x.data_ptr(), _DTYPES[x.dtype], x.stride(0), rows, cols,
+    _launch_quant(x.get_device(), x.data_ptr(), _DTYPES[x.dtype], x.stride(0), rows, cols,
            codes.data_ptr(), codes.stride(0), scale.data_ptr())
     return (codes if codes.shape[1] == cols else codes[:, :cols]), scale
 
 
-def _check_weight(w8: Tensor, w_scale: Tensor, in_features: int, device) -> None:
-    if w8.dtype != torch.int8 or w_scale.dtype != torch.float32:
+def _check_weight(w8: Tensor, w_scale: Tensor, in_features: int, index: int) -> None:
+    if w8.dtype is not torch.int8 or w_scale.dtype is not torch.float32:
         raise TypeError("codes must be torch.int8 and scales torch.float32")
-    if w8.ndim != 2 or w_scale.ndim != 1 or w_scale.shape[0] != w8.shape[0]:
+    if w8.ndim != 2 or w_scale.ndim != 1:
         raise ValueError("expected codes [rows, in_features] and one scale a row")
-    if w8.shape[0] == 0 or w8.shape[1] == 0:
+    n, k = w8.shape
+    if w_scale.shape[0] != n:
+        raise ValueError("expected codes [rows, in_features] and one scale a row")
+    if n == 0 or k == 0:
         raise ValueError("a linear layer needs at least one input and one output feature")
-    if w8.shape[1] != in_features:
-        raise ValueError(f"in_features differ: {in_features} and {w8.shape[1]}")
-    if w8.device != device or w_scale.device != device:
+    if k != in_features:
+        raise ValueError(f"in_features differ: {in_features} and {k}")
+    if w8.get_device() != index or w_scale.get_device() != index:
         raise ValueError("all tensors of a call must share one CUDA device")
     _check_rows("w8", w8)
-    if not w_scale.is_contiguous():
+    if w_scale.stride(0) != 1 and n > 1:
         raise ValueError("scales must be contiguous")
 
 
@@ -67,14 +72,14 @@ def _check_rows(name: str, t: Tensor) -> None:
                          "(quantize_per_token_int8 lays them out so)")
 
 
-def _check_bias(bias: Optional[Tensor], rows: int, dtype, device) -> None:
+def _check_bias(bias: Optional[Tensor], rows: int, dtype, index: int) -> None:
     if bias is None:
         return
     if bias.dtype != dtype:
         raise TypeError("the bias must have the output's dtype")
     if bias.shape != (rows,) or not bias.is_contiguous():
         raise ValueError("the bias must be contiguous with one value for each output feature")
-    if bias.device != device:
+    if bias.get_device() != index:
         raise ValueError("all tensors of a call must share one CUDA device")
 
 
@@ -90,13 +95,13 @@ def int8_matmul(x8: Tensor, x_scale: Tensor, w8: Tensor, w_scale: Tensor, bias: 
         raise TypeError("codes must be torch.int8 and scales torch.float32")
     if x8.ndim != 2 or x_scale.ndim != 1 or x_scale.shape[0] != x8.shape[0] or not x_scale.is_contiguous():
         raise ValueError("expected codes [tokens, in_features] and one contiguous scale a token")
-    if x_scale.device != x8.device:
+    if x_scale.get_device() != x8.get_device():
         raise ValueError("all tensors of a call must share one CUDA device")
-    _check_weight(w8, w_scale, x8.shape[1], x8.device)
+    _check_weight(w8, w_scale, x8.shape[1], x8.get_device())
     _check_rows("x8", x8)
-    _check_bias(bias, w8.shape[0], out_dtype, x8.device)
+    _check_bias(bias, w8.shape[0], out_dtype, x8.get_device())
     out = torch.empty((x8.shape[0], w8.shape[0]), dtype=out_dtype, device=x8.device)
-    launch("tm_int8_matmul", x8.device, x8.data_ptr(), x8.stride(0), x_scale.data_ptr(), w8.data_ptr(), w8.stride(0),
+    _launch_matmul(x8.get_device(), x8.data_ptr(), x8.stride(0), x_scale.data_ptr(), w8.data_ptr(), w8.stride(0),
            w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0),
            _DTYPES[out_dtype], x8.shape[0], w8.shape[0], x8.shape[1])
     return out
@@ -111,20 +116,21 @@ def int8_linear(x: Tensor, w8: Tensor, w_scale: Tensor, bias: Optional[Tensor] =
         raise ValueError("expected [..., in_features]")
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError("the per-token quantiser takes fp16 or bf16")
-    device, dtype, k = x.device, x.dtype, x.shape[-1]
-    _check_weight(w8, w_scale, k, device)
+    index, dtype, k = x.get_device(), x.dtype, x.shape[-1]
+    _check_weight(w8, w_scale, k, index)
     n = w8.shape[0]
-    _check_bias(bias, n, dtype, device)
+    _check_bias(bias, n, dtype, index)
     rows = x if x.ndim == 2 else x.reshape(-1, k)
-    if rows.stride(1) != 1 and k > 1:
-        rows = rows.contiguous()
     m = rows.shape[0]
-    out = torch.empty((m, n), dtype=dtype, device=device)
+    row_stride, column_stride = rows.stride()
+    if column_stride != 1 and k > 1:
+        rows, row_stride = rows.contiguous(), k
+    out = x.new_empty((m, n))
     # One piece of scratch: the codes, their rows on 16 bytes, and behind them the scales.
     wide = (k + 15) // 16 * 16
-    scratch = torch.empty(m * (wide + 4), dtype=torch.int8, device=device)
+    scratch = w8.new_empty(m * (wide + 4))
     codes = scratch.data_ptr()
-    launch("tm_int8_linear", device, rows.data_ptr(), _DTYPES[dtype], rows.stride(0), codes, wide, codes + m * wide,
+    _launch_linear(index, rows.data_ptr(), _DTYPES[dtype], row_stride, codes, wide, codes + m * wide,
            w8.data_ptr(), w8.stride(0), w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), n,
            m, n, k)
     return out if x.ndim == 2 else out.view(*x.shape[:-1], n)

@@ -113,10 +113,10 @@ def attention(q, keys, values, kv_len, sm_scale, causal, key_mask=None):
     and a bound on what fp16 operands may change.
 
     Bound: scores come from the codes, s (q . n) + m sum q: products of two fp16 numbers are exact, their fp32 sums are
-    rounded (or cut) a few times at 2^-22; the sum of q over a group is held to 2^-17 of it, which is under
-    2^-10 s sum |q| with the group's scale s (its range / 15) where |m| is at most 100 s, as it is for these inputs. The
-    fp32 steps that follow add 2^-21 sum |q| |k|. With d the sum of both, times sm_scale, a weight changes by the factor e^(2 d) (numerator and
-    sum). v and p are rounded to fp16 (2^-11 each; a p under 2^-14 by at most 2^-25 of the largest weight), the result
+    rounded (or cut) a few times at 2^-22 of sum |q| 15 s + |m| sum |q|, and the sum of q over a group is held to 2^-22
+    of it: with |m| at most 100 s, as it is for these inputs, under 2^-12 s sum |q| together; 2^-10 is allowed. The fp32
+    steps that follow add 2^-21 sum |q| |k|. With d the sum of both, times sm_scale, a weight changes by the factor
+    e^(2 d) (numerator and sum). v and p are rounded to fp16 (2^-11 each; a p under 2^-14 by at most 2^-25 of the largest weight), the result
     once more; 2^-18 covers the fp32 sums and exponentials.
     """
     n, heads_q, dim = q.shape

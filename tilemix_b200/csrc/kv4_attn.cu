@@ -443,13 +443,13 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
       for (int c = 0; c < 2; ++c) m[x][c] = -CUDART_INF_F, mc[x][c] = 0.f, l[x][c] = 0.f;
     }
 
-    // One step: 32 keys from stage s. `plain`: every key counts for every row; `live`: those that count for any.
+    // One step: 32 keys from stage s; `live`: those that count for any row.
     // What a step does for keys that do not count is kept to two short branches: a second copy of the whole step
     // without them ran no faster where it was used, and the last step of every run then met cold instructions
     // (64 ragged requests 96 us, 84 with lengths that fill their steps).
-    auto step = [&](const bool plain, const int key, const uint32_t live) {
+    auto step = [&](const int key, const uint32_t live) {
       uint8_t* st = ring + s * kStageBytes;
-      if (!plain) {
+      if (live != 0xffffffffu) {
         // The V scales and minima of keys that count for no row become 0, so that nothing of them (infinities, NaN,
         // what an absent block's stage happens to hold) reaches the output.
         const int tok = lane % kBlockTokens;
@@ -499,18 +499,30 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
         }
       }
 
-      if (!plain) {
-        const uint32_t on = live >> tok_g;
+      if (live != 0xffffffffu) {
+#pragma unroll
+        for (int u = 0; u < kStepBlocks; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const bool dead = !((live >> (tok_g + kBlockTokens * u + 8 * h)) & 1);
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+                if (dead) sc[u][x][2 * h + c] = -CUDART_INF_F;
+          }
+      }
+      if (key + kStepKeys > lim_lo) {  // some row's last keys
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int left = lim[x][c & 1] - key - tok_g;  // the row sees this many keys from the lane's first on
+          for (int c = 0; c < 2; ++c) {
+            const int left = lim[x][c] - key - tok_g;  // the row sees this many keys from the lane's first on
 #pragma unroll
-            for (int u = 0; u < kStepBlocks; ++u) {
-              const int at = kBlockTokens * u + (c >> 1) * 8;
-              if (!(on & (1u << at)) || at >= left) sc[u][x][c] = -CUDART_INF_F;
-            }
+            for (int u = 0; u < kStepBlocks; ++u)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (kBlockTokens * u + 8 * h >= left) sc[u][x][2 * h + c] = -CUDART_INF_F;
           }
       }
       float base[NT][2];
@@ -599,19 +611,17 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
     for (int i = 0; i < steps; ++i) {
       const int key = first_key + stride * i;
       uint32_t live = 0xffffffffu;  // which of the step's keys count for any row, a bit each
-      bool plain = i < n_plain && stage_bad == 0;
-      if (!plain) {
+      if (i >= n_plain || stage_bad != 0) {
         const uint32_t bad = (stage_bad >> (kStepBlocks * s)) & ((1u << kStepBlocks) - 1);
         live = __ballot_sync(0xffffffffu, !((bad >> (lane / kBlockTokens)) & 1) && key + lane < lim_hi &&
                                               (mask == nullptr || mask_on));
         if (mask != nullptr) mask_on = mask_of(i + 1);
-        plain = live == 0xffffffffu && key + kStepKeys <= lim_lo;
       }
       if (!mbar_wait_spin(&bar[s], phase, a.err, kErrTimeoutFull)) {
         ok = false;
         break;
       }
-      step(plain, key, live);
+      step(key, live);
       __syncwarp();  // every lane has read the stage
       if (++s == kStages) s = 0, phase ^= 1;
       if (issued < steps) issue();
@@ -796,8 +806,9 @@ struct Plan {
   int64_t bytes() const { return starts_bytes + part_o_bytes + part_ml_bytes; }
 };
 
-// Two row tiles a CTA where more than 8 rows share a KV head (the unpacking is shared; four would spill). As
-// many CTAs as are resident at once, or as there can be chunks.
+// Two row tiles a CTA where more than 8 rows share a KV head: the unpacking is shared. Four, at head_dim 64, leave two
+// CTAs an SM and measured slower (8 requests of up to 15 query tokens: 44 us against 41). As many CTAs as are
+// resident at once, or as there can be chunks.
 static Plan plan_of(const tm_kv4_attn_params* p) {
   Plan r{};
   const int64_t rows = static_cast<int64_t>(p->max_seqlen_q) * (p->heads_q / p->heads_k);

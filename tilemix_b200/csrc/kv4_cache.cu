@@ -25,26 +25,33 @@ namespace kv4 {
 template <int D>
 constexpr int kThreads = kBlockTokens * D / 8;
 
+struct Pages {
+  uint32_t heads;
+  int bytes;        // of one head of a page
+  uint32_t blocks;  // 16-token blocks a page
+  int shift;        // log2 of them, or -1
+};
+
 struct AppendArgs {
   const __half* k;
   const __half* v;
-  int64_t k_st, k_sh, v_st, v_sh;
+  int k_st, k_sh, v_st, v_sh;
   uint8_t* pool;
-  int64_t n_tokens;
+  int n_tokens;
   int64_t n_slots;  // pages * page size
   const int64_t* slots;
-  int heads, page_bytes;
-  uint32_t page_blocks;
+  Pages pages;
   int* err;
 };
 
-// Where a slot's 16-token block of a head is. Blocks are counted in 32 bits (the entry points see to it): a
-// 64-bit division by the page size was a quarter of the kernel's instructions.
-__device__ __forceinline__ int64_t block_offset(int64_t slot, int head, int heads, uint32_t page_blocks, int page_bytes,
-                                                int block_bytes) {
-  const uint32_t blk = static_cast<uint32_t>(slot >> 4), page = blk / page_blocks;
-  return (static_cast<int64_t>(page) * heads + head) * page_bytes +
-         static_cast<int64_t>(blk - page * page_blocks) * block_bytes;
+// Where a slot's 16-token block of a head is. Blocks, tokens and strides are counted in 32 bits (the entry points
+// see to it) and page sizes that are powers of two divide by a shift: 64-bit products and a division by the page
+// size were a third of the kernels' instructions.
+__device__ __forceinline__ int64_t block_offset(int64_t slot, int head, const Pages& p, int block_bytes) {
+  const uint32_t blk = static_cast<uint32_t>(slot >> 4);
+  const uint32_t page = p.shift >= 0 ? blk >> p.shift : blk / p.blocks;
+  return static_cast<int64_t>(page * p.heads + head) * p.bytes +
+         static_cast<int64_t>(blk - page * p.blocks) * block_bytes;
 }
 
 __device__ __forceinline__ __half2 h2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
@@ -133,7 +140,7 @@ __global__ void __launch_bounds__(kThreads<D>) append_kernel(const AppendArgs a)
   __shared__ int sh_at[kBlockTokens];          // its place there
   __shared__ __half sh_scale[kBlockTokens][L::kGroups][2];
   const int head = blockIdx.x, in_cta = threadIdx.x / kLanes;
-  const int64_t tok = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * kBlockTokens + in_cta;
+  const int tok = (blockIdx.z * gridDim.y + blockIdx.y) * kBlockTokens + in_cta;
   const int l = threadIdx.x % kLanes;
   const int j = l >> 2, t = l & 3;
   const bool there = tok < a.n_tokens;  // tokens behind the last one stay for the shuffles
@@ -141,8 +148,8 @@ __global__ void __launch_bounds__(kThreads<D>) append_kernel(const AppendArgs a)
   const bool fits = slot >= 0 && slot < a.n_slots;
   uint4 xk = make_uint4(0, 0, 0, 0), xv = xk;
   if (fits) {
-    xk = __ldcs(reinterpret_cast<const uint4*>(a.k + tok * a.k_st + head * a.k_sh + 8 * l));
-    xv = __ldcs(reinterpret_cast<const uint4*>(a.v + tok * a.v_st + head * a.v_sh + 8 * l));
+    xk = __ldcs(reinterpret_cast<const uint4*>(a.k + static_cast<int64_t>(tok) * a.k_st + (static_cast<int64_t>(head) * a.k_sh + 8 * l)));
+    xv = __ldcs(reinterpret_cast<const uint4*>(a.v + static_cast<int64_t>(tok) * a.v_st + (static_cast<int64_t>(head) * a.v_sh + 8 * l)));
   }
   __half2 ks, vs;
   const uint32_t kw = quantise8(xk, &ks), vw = quantise8(xv, &vs);
@@ -151,7 +158,7 @@ __global__ void __launch_bounds__(kThreads<D>) append_kernel(const AppendArgs a)
   const uint32_t other = __shfl_xor_sync(0xffffffffu, vw, 4);
   const uint32_t vpair = (j & 1) ? __byte_perm(other, vw, 0x7632) : __byte_perm(vw, other, 0x5410);
   const int in_block = static_cast<int>(slot) & (kBlockTokens - 1);
-  uint8_t* blk = fits ? a.pool + block_offset(slot, head, a.heads, a.page_blocks, a.page_bytes, L::kBlockBytes) : nullptr;
+  uint8_t* blk = fits ? a.pool + block_offset(slot, head, a.pages, L::kBlockBytes) : nullptr;
   if (t == 0) {
     sh_scale[in_cta][j][0] = __low2half(vs);
     sh_scale[in_cta][j][1] = __high2half(vs);
@@ -185,9 +192,9 @@ __global__ void __launch_bounds__(kThreads<D>) append_kernel(const AppendArgs a)
 struct ReadArgs {
   const uint8_t* pool;
   const int64_t* slots;
-  int64_t n_tokens, n_slots;
-  int heads, page_bytes;
-  uint32_t page_blocks;
+  int n_tokens;
+  int64_t n_slots;
+  Pages pages;
   __half* k;
   __half* v;
   int* err;
@@ -212,8 +219,7 @@ __global__ void __launch_bounds__(kThreads<D>) read_kernel(const ReadArgs a) {
   using L = Layout<D>;
   constexpr int kLanes = D / 8;
   const int head = blockIdx.x;
-  const int64_t tok =
-      (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * kBlockTokens + threadIdx.x / kLanes;
+  const int tok = (blockIdx.z * gridDim.y + blockIdx.y) * kBlockTokens + threadIdx.x / kLanes;
   const int l = threadIdx.x % kLanes;
   const int j = l >> 2, t = l & 3;
   const bool there = tok < a.n_tokens;  // tokens behind the last one stay for the shuffle
@@ -224,7 +230,7 @@ __global__ void __launch_bounds__(kThreads<D>) read_kernel(const ReadArgs a) {
   __half vs = __ushort_as_half(0), vm = vs;
   if (fits) {
     const int in_block = static_cast<int>(slot) & (kBlockTokens - 1);
-    const uint8_t* blk = a.pool + block_offset(slot, head, a.heads, a.page_blocks, a.page_bytes, L::kBlockBytes);
+    const uint8_t* blk = a.pool + block_offset(slot, head, a.pages, L::kBlockBytes);
     kw = *reinterpret_cast<const uint32_t*>(blk + in_block * L::kRowBytes + (t * L::kGroups + j) * 4);
     vpair = *reinterpret_cast<const uint32_t*>(blk + L::kOffV + in_block * L::kRowBytes +
                                                (2 * t + (j & 1)) * (2 * L::kGroups) + (j & ~1) * 2);
@@ -244,7 +250,7 @@ __global__ void __launch_bounds__(kThreads<D>) read_kernel(const ReadArgs a) {
   } else if (slot != -1 && l == 0) {
     record_error(a.err, kErrCacheSlot);
   }
-  const int64_t at = (tok * a.heads + head) * D + 8 * l;
+  const int64_t at = static_cast<int64_t>(tok * a.pages.heads + head) * D + 8 * l;
   __stcs(reinterpret_cast<uint4*>(a.k + at), ok);
   __stcs(reinterpret_cast<uint4*>(a.v + at), ov);
 }
@@ -253,6 +259,21 @@ __global__ void __launch_bounds__(kThreads<D>) read_kernel(const ReadArgs a) {
 static dim3 grid_of(int64_t groups, int heads) {
   const unsigned y = static_cast<unsigned>(groups < 65535 ? groups : 65535);
   return dim3(static_cast<unsigned>(heads), y, static_cast<unsigned>((groups + y - 1) / y));
+}
+
+// TM_OK and the pool's shape for the kernels, or why not.
+static int pages_of(int64_t n_tokens, int64_t num_pages, int heads, int head_dim, int page_size, Pages* p) {
+  const int64_t blocks = page_size / kBlockTokens, bytes = blocks * block_bytes(head_dim);
+  if (bytes > 0x7fffffffll || num_pages * blocks > 0x7fffffffll || num_pages * heads > 0x7fffffffll ||
+      (n_tokens + kBlockTokens) * heads > 0x7fffffffll)
+    return TM_ERR_UNSUPPORTED;
+  p->heads = static_cast<uint32_t>(heads);
+  p->bytes = static_cast<int>(bytes);
+  p->blocks = static_cast<uint32_t>(blocks);
+  p->shift = -1;
+  for (int k = 0; k < 31; ++k)
+    if (blocks == (1ll << k)) p->shift = k;
+  return TM_OK;
 }
 
 }  // namespace kv4
@@ -268,14 +289,23 @@ extern "C" int tm_kv4_append(const void* k, int64_t k_stride_tok, int64_t k_stri
   if (n_tokens == 0) return TM_OK;
   if (!k || !v || !slots || (num_pages > 0 && !pool)) return TM_ERR_NULL;
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(pool, 16) || !aligned(slots, 8)) return TM_ERR_ALIGN;
-  if (k_stride_tok % 8 || k_stride_head % 8 || v_stride_tok % 8 || v_stride_head % 8) return TM_ERR_ALIGN;
-  const int64_t page_bytes = static_cast<int64_t>(page_size) / kBlockTokens * block_bytes(head_dim);
+  AppendArgs a{};
+  const int64_t strides[4] = {k_stride_tok, k_stride_head, v_stride_tok, v_stride_head};
+  int* const to[4] = {&a.k_st, &a.k_sh, &a.v_st, &a.v_sh};
+  for (int i = 0; i < 4; ++i) {
+    if (strides[i] % 8 != 0) return TM_ERR_ALIGN;
+    if (strides[i] > 0x7fffffffll || strides[i] < -0x7fffffffll) return TM_ERR_UNSUPPORTED;
+    *to[i] = static_cast<int>(strides[i]);
+  }
+  if (pages_of(n_tokens, num_pages, heads, head_dim, page_size, &a.pages) != TM_OK) return TM_ERR_UNSUPPORTED;
+  a.k = static_cast<const __half*>(k);
+  a.v = static_cast<const __half*>(v);
+  a.pool = static_cast<uint8_t*>(pool);
+  a.n_tokens = static_cast<int>(n_tokens);
+  a.n_slots = num_pages * page_size;
+  a.slots = slots;
+  a.err = error_flag;
   const int64_t groups = (n_tokens + kBlockTokens - 1) / kBlockTokens;
-  if (page_bytes > 0x7fffffffll || groups > 65535ll * 65535ll || num_pages > 0x7fffffffll / (page_size / kBlockTokens))
-    return TM_ERR_UNSUPPORTED;
-  AppendArgs a{static_cast<const __half*>(k), static_cast<const __half*>(v), k_stride_tok, k_stride_head,
-               v_stride_tok, v_stride_head, static_cast<uint8_t*>(pool), n_tokens, num_pages * page_size, slots,
-               heads, static_cast<int>(page_bytes), static_cast<uint32_t>(page_size / kBlockTokens), error_flag};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128)
     append_kernel<128><<<grid_of(groups, heads), kThreads<128>, 0, st>>>(a);
@@ -292,12 +322,16 @@ extern "C" int tm_kv4_read(const void* pool, int64_t num_pages, int heads, int h
   if (n_tokens == 0) return TM_OK;
   if (!k || !v || !slots || (num_pages > 0 && !pool)) return TM_ERR_NULL;
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(pool, 16) || !aligned(slots, 8)) return TM_ERR_ALIGN;
-  const int64_t page_bytes = static_cast<int64_t>(page_size) / kBlockTokens * block_bytes(head_dim);
+  ReadArgs a{};
+  if (pages_of(n_tokens, num_pages, heads, head_dim, page_size, &a.pages) != TM_OK) return TM_ERR_UNSUPPORTED;
+  a.pool = static_cast<const uint8_t*>(pool);
+  a.slots = slots;
+  a.n_tokens = static_cast<int>(n_tokens);
+  a.n_slots = num_pages * page_size;
+  a.k = static_cast<__half*>(k);
+  a.v = static_cast<__half*>(v);
+  a.err = error_flag;
   const int64_t groups = (n_tokens + kBlockTokens - 1) / kBlockTokens;
-  if (page_bytes > 0x7fffffffll || groups > 65535ll * 65535ll || num_pages > 0x7fffffffll / (page_size / kBlockTokens))
-    return TM_ERR_UNSUPPORTED;
-  ReadArgs a{static_cast<const uint8_t*>(pool), slots, n_tokens, num_pages * page_size, heads, static_cast<int>(page_bytes),
-             static_cast<uint32_t>(page_size / kBlockTokens), static_cast<__half*>(k), static_cast<__half*>(v), error_flag};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128)
     read_kernel<128><<<grid_of(groups, heads), kThreads<128>, 0, st>>>(a);

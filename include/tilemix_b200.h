@@ -296,8 +296,8 @@ int tm_rms_norm(const void* x, const void* weight, void* out, int64_t rows, int 
  * the entries of its block-table row.
  *
  * What only the device can see is reported through error_flag (optional device
- * int, first writer wins): 11 free pages, table columns, slots or max_kv_len
- * exceeded, or a length negative; 12 a page number outside the pool (its keys are
+ * int, first writer wins): 11 free pages, table columns, slots, max_kv_len or
+ * max_seqlen_q exceeded, or a length negative; 12 a page number outside the pool (its keys are
  * left out); 13 a slot outside the pool (skipped).
  */
 

@@ -382,6 +382,16 @@ def test_lengths_beyond_the_table_are_reported(cuda_device):
     _assert_close(out, q, cu, keys, values, 64 ** -0.5, causal=False)
 
 
+def test_more_query_tokens_than_said_are_reported(cuda_device):
+    from tilemix_b200.attention.kv4 import kv4_attention
+
+    pool, table, lens, keys, values = _cache(cuda_device, [64, 70], 1, 64, 16, seed=13)
+    q, cu = _queries(cuda_device, [3, 5], 2, 64, seed=11)
+    out = torch.full_like(q, 3.0)
+    kv4_attention(q, pool, table, lens, cu, 4, out=out)
+    assert _error_code() == 11 and (out[-1] == 3).all() and not (out[:-1] == 3).all(-1).any()
+
+
 def test_no_rows_and_no_requests(cuda_device):
     from tilemix_b200.attention.kv4 import kv4_append, kv4_attention, kv4_pool, kv4_read
 

@@ -109,6 +109,7 @@ ATTN = dict(q=lambda: _Fake((3, 4, 64)), pool=_pool, block_table=lambda: _i32(3,
     (dict(q=_Fake((3, 4, 64), stride=(512, 128, 2))), ValueError, "contiguous"),
     (dict(q=_Fake((4, 4, 64))), ValueError, "one query row"),
     (dict(max_seqlen_q=2), ValueError, "one query row"),
+    (dict(max_seqlen_q=0, cu_seqlens_q=_i32(4)), ValueError, "positive"),
     (dict(pool=_pool(dtype=torch.int8)), TypeError, "uint8"),
     (dict(pool=_Fake((4, 2, 100), torch.uint8)), ValueError, "whole blocks"),
     (dict(pool=_pool(device="cuda:1")), ValueError, "one CUDA device"),

@@ -215,8 +215,8 @@ def kv4_attention(q: Tensor, pool: Tensor, block_table: Tensor, kv_lens: Tensor,
     of a request's n query tokens sees the keys up to position ``kv_len - n + i``. ``key_mask`` (bool
     [batch, columns], optional) excludes keys for every row of a request; a key behind its last
     column is excluded too. A row that sees no key is 0. ``max_kv_len`` bounds ``kv_lens`` on the
-    host (default: the table's capacity); keys beyond it are left out (``device_error_code`` 11), and a
-    small bound makes for a small launch. Rows of ``q`` that belong to no request are left as they
+    host (default: the table's capacity). Keys beyond it, or query tokens beyond ``max_seqlen_q``, are
+    left out (``device_error_code`` 11); a small bound makes for a small launch. Rows of ``q`` that belong to no request are left as they
     were in ``out``.
     """
     if not q.is_cuda:
@@ -235,6 +235,8 @@ def kv4_attention(q: Tensor, pool: Tensor, block_table: Tensor, kv_lens: Tensor,
     batch, cols = block_table.shape
     if kv_lens.numel() != batch:
         raise ValueError("block_table and kv_lens must agree on the batch")
+    if rows and max_seqlen_q < 1:
+        raise ValueError("max_seqlen_q must be positive")
     if cu_seqlens_q is not None:
         _check("cu_seqlens_q", cu_seqlens_q, torch.int32, index)
         if cu_seqlens_q.numel() != batch + 1:

@@ -67,10 +67,11 @@ def _error_word(device: torch.device) -> torch.Tensor:
 
 
 def device_error_code(device: Optional[torch.device] = None, reset: bool = True) -> int:
-    """Read (and optionally clear) the device error word of the attention kernel.
+    """Read (and optionally clear) the device error word of the package's kernels.
 
-    Non-zero means a bounded wait inside the kernel timed out (codes in
-    csrc/common.cuh). Synchronises the device.
+    Non-zero means a bounded wait inside a kernel timed out, or (11 to 13) that a call on the 4-bit
+    cache met something that only the device could see (codes in csrc/common.cuh; the first one
+    stays). Synchronises the device.
     """
     device = device or torch.device("cuda", torch.cuda.current_device())
     w = _error_word(device)

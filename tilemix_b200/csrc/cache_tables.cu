@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kThreads) build_kernel(const Args a) {
   bool mine_bad = false, many = false;
   for (int b = b0; b < b1; ++b) {
     const long long c = a.cached[b], n = a.fresh[b];
-    if (c < 0 || n < 0 || c + n > most || c + n > 0x7fffffffll) {
+    if (c < 0 || n < 0 || c + n > most || c + n > 0x7fffffffll - a.page) {
       mine_bad = true;
       continue;
     }

@@ -249,7 +249,8 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
       a.starts[b] = at;
       const Request r = request_of<NT>(a, b);
       at += r.cost;
-      if (r.kv < a.kv_lens[b]) record_error(a.err, kErrCachePlan);  // longer than it may be
+      // more keys, or more query tokens, than the call said there may be: those beyond are left out
+      if (r.kv < a.kv_lens[b] || (a.cu != nullptr && a.cu[b + 1] - a.cu[b] > a.max_q)) record_error(a.err, kErrCachePlan);
     }
     if (lane == 0) a.starts[a.batch] = total;
   }
@@ -831,7 +832,7 @@ static int check(const tm_kv4_attn_params* p) {
   if (p->num_pages < 0 || p->cols < 0 || p->max_seqlen_q < 0 || p->max_kv_len < 0) return TM_ERR_SHAPE;
   if (p->page_size < kBlockTokens || p->page_size % kBlockTokens != 0) return TM_ERR_SHAPE;
   if (p->head_dim != 64 && p->head_dim != 128) return TM_ERR_UNSUPPORTED;
-  if (p->batch > 65535 || p->max_seqlen_q > 65535 || p->heads_q > 65535 || p->max_kv_len > (1 << 30))
+  if (p->batch > 65535 || p->max_seqlen_q > 65535 || p->heads_q > 32767 || p->max_kv_len > (1 << 30))
     return TM_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(p->page_size) * 20 * 128 / kBlockTokens > 0x7fffffffll) return TM_ERR_UNSUPPORTED;
   if (p->batch == 0 || p->q_tokens == 0 || p->max_seqlen_q == 0) return TM_OK;

@@ -148,8 +148,9 @@ static void run_quant(const T* x, int64_t xs, unsigned rows, int cols, int8_t* o
   quant_rows_kernel<T, kVec, kThreads><<<rows, kThreads, 0, st>>>(x, xs, cols, out, os, scale);
 }
 
-// 1024 threads a row where there are fewer rows than SMs to fill or the row is long (64 rows of 18944: 11 us with
-// 256 threads that read it twice, 4 us so), 256 where rows are many (a CTA's reduction then hides behind the others).
+// 1024 threads a row where rows are fewer than two an SM (64 rows of 18944: 11 us with 256 threads that read it twice,
+// 5 us so), 256 where they are many: a CTA's reduction then hides behind the others' loads (4096 rows of 18944: 120 us
+// with 1024 threads, XX so).
 template <typename T>
 static void launch_quant(const void* x, int64_t xs, int64_t rows, int cols, int8_t* out, int64_t os, float* scale,
                          cudaStream_t st) {
@@ -160,16 +161,23 @@ static void launch_quant(const void* x, int64_t xs, int64_t rows, int cols, int8
     run_quant<T, 0, 1024>(p, xs, g, cols, out, os, scale, st);
   else if (cols <= 2048)
     run_quant<T, 1, 256>(p, xs, g, cols, out, os, scale, st);
-  else if (cols > 16384)
-    run_quant<T, 4, 1024>(p, xs, g, cols, out, os, scale, st);
-  else if (cols > 8192)
-    run_quant<T, 2, 1024>(p, xs, g, cols, out, os, scale, st);
-  else if (rows < 148)
-    run_quant<T, 1, 1024>(p, xs, g, cols, out, os, scale, st);
-  else if (cols <= 4096)
+  else if (rows < 2 * 148) {
+    if (cols <= 8192)
+      run_quant<T, 1, 1024>(p, xs, g, cols, out, os, scale, st);
+    else if (cols <= 16384)
+      run_quant<T, 2, 1024>(p, xs, g, cols, out, os, scale, st);
+    else
+      run_quant<T, 4, 1024>(p, xs, g, cols, out, os, scale, st);
+  } else if (cols <= 4096)
     run_quant<T, 2, 256>(p, xs, g, cols, out, os, scale, st);
-  else
+  else if (cols <= 8192)
     run_quant<T, 4, 256>(p, xs, g, cols, out, os, scale, st);
+  else if (cols <= 16384)
+    run_quant<T, 8, 256>(p, xs, g, cols, out, os, scale, st);
+  else if (cols <= 24576)
+    run_quant<T, 12, 256>(p, xs, g, cols, out, os, scale, st);
+  else
+    run_quant<T, 8, 512>(p, xs, g, cols, out, os, scale, st);
 }
 
 // ----------------------------------------------------------------------------
@@ -190,6 +198,7 @@ constexpr int kSms = 148;
 struct GemmArgs {
   int rows_a, rows_b;
   int k_tiles, split;
+  int bn;  // columns a tile (the pair kernel's; the others know theirs)
   int tiles_a, tiles_b;
   const float* scale_a;  // of the lanes' rows
   const float* scale_b;  // of the columns' rows
@@ -589,12 +598,13 @@ __global__ void __launch_bounds__(kGemmThreads) gemm_kernel(const __grid_constan
 // ----------------------------------------------------------------------------
 // Two CTAs a tile
 // ----------------------------------------------------------------------------
-// 256 tokens x 256 channels on a pair of SMs (cta_group::2): each CTA brings its 128 tokens and half of the
+// 256 tokens x up to 256 channels on a pair of SMs (cta_group::2): each CTA brings its 128 tokens and half of the
 // channels' rows, the first one issues the products for both, each keeps its 128 rows of the sum in its own
 // TMEM. A CTA then reads 32 KB for each 128 bytes of K where it read 48 KB for the same number of products: the
-// one-CTA kernel is bound by what L2 delivers.
+// one-CTA kernel is bound by what L2 delivers. The width is a multiple of 32 from 128 on, chosen so that the last
+// wave of tiles is full.
 struct PairShape {
-  static constexpr int kBN = 256;
+  static constexpr int kBN = 256;  // widest
   static constexpr int kStageBytes = (kBM + kBN / 2) * kBK;
   static constexpr int kStages = 6;
   // Eight epilogue warps, two for each quarter of the rows, half of the columns each: with one tile a CTA nothing
@@ -653,7 +663,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x & 1, first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
-  const int tiles = g.tiles_a * g.tiles_b;
+  const int tiles = g.tiles_a * g.tiles_b, bn = g.bn;
+  const uint32_t bytes = 2u * (kBM + bn / 2) * kBK;  // of a stage in both CTAs
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
@@ -697,9 +708,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
       tile_at(first_tile, &ta, &tb);
       early = min(S::kStages, g.k_tiles);
       for (int i = 0; i < early; ++i) {
-        if (rank == 0) mbar_arrive_expect_tx_e(&full[i], 2 * S::kStageBytes);
+        if (rank == 0) mbar_arrive_expect_tx_e(&full[i], bytes);
         tma_load_pair_e(smem + i * S::kStageBytes + kBM * kBK, &map_b, first_cta(&full[i]), i * kBK,
-                        tb * S::kBN + rank * (S::kBN / 2));
+                        tb * bn + rank * (bn / 2));
       }
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -714,8 +725,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
             ok = false;
             break;
           }
-          if (rank == 0) mbar_arrive_expect_tx_e(&full[s], 2 * S::kStageBytes);
-          tma_load_pair_e(st + kBM * kBK, &map_b, first_cta(&full[s]), k * kBK, tb * S::kBN + rank * (S::kBN / 2));
+          if (rank == 0) mbar_arrive_expect_tx_e(&full[s], bytes);
+          tma_load_pair_e(st + kBM * kBK, &map_b, first_cta(&full[s]), k * kBK, tb * bn + rank * (bn / 2));
         }
         tma_load_pair_e(st, &map_a, first_cta(&full[s]), k * kBK, (2 * ta + rank) * kBM);
         ++used;
@@ -727,7 +738,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
         mbar_wait(&full[i], ((used - 1 - i) / S::kStages) & 1, g.err, kErrTimeoutDrain);
     }
   } else if (warp == 1 && rank == 0) {
-    constexpr uint32_t idesc = make_idesc(2, 1, 0, 0, 2 * kBM, S::kBN);
+    const uint32_t idesc = make_idesc(2, 1, 0, 0, 2 * kBM, bn);
     int s = 0, n = 0;
     uint32_t phase = 0;
     for (int t = first_tile; t < tiles && ok; t += tile_step, ++n) {
@@ -771,8 +782,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
       const int a0 = (2 * ta + rank) * kBM + quad * 32;
       float* col_scale = cols + acc * 2 * S::kBN;
       float* col_bias = col_scale + S::kBN;
-      for (int c = et; c < S::kBN; c += 32 * S::kEpilogueWarps) {
-        const int b = tb * S::kBN + c;
+      for (int c = et; c < bn; c += 32 * S::kEpilogueWarps) {
+        const int b = tb * bn + c;
         const bool in = b < g.rows_b;
         col_scale[c] = in ? g.scale_b[b] : 0.f;
         col_bias[c] = in && g.bias != nullptr ? load_one(static_cast<const OutT*>(g.bias) + b) : 0.f;
@@ -786,8 +797,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
       const uint32_t d = tmem + acc * S::kBN + (static_cast<uint32_t>(quad * 32) << 16);
       constexpr int kCols = S::kRowBytes / sizeof(OutT);
 #pragma unroll 1
-      for (int c = side * (S::kBN / 2); c < (side + 1) * (S::kBN / 2); c += kCols)
-        emit_rows<OutT, S::kRowBytes>(d + c, piece, g, a0, tb * S::kBN + c, row_scale, col_scale + c, col_bias + c);
+      for (int c = side * kCols; c < bn; c += 2 * kCols)
+        emit_rows<OutT, S::kRowBytes>(d + c, piece, g, a0, tb * bn + c, row_scale, col_scale + c, col_bias + c);
       tc_fence_before();
       __syncwarp();
       if (lane == 0)
@@ -810,33 +821,42 @@ struct Plan {
   int bn, split;
 };
 
-// Which side is the lanes', how wide a tile is and into how many parts K is cut, by sizes alone.
+// Which kernel, how wide a tile and into how many parts K is cut, by sizes alone: the least of an estimate in SM
+// cycles. A step of 128 bytes of K costs what L2 has to deliver for it, 64 bytes a cycle and SM (18 TB/s in all,
+// from the one-CTA kernel at 8192 x 4096 -> 14336), or two cycles a column in the tensor core; a wave of CTAs costs
+// its steps; the epilogue 8 cycles a column of whole lines, 60 of single values (tokens on the columns, or a
+// split's share of them), and a split 2500 for its two meetings. Against rules by the number of tiles alone:
+// 256 x 18944 -> 3584 37 us, XX so; 128 x 512 -> 1000 12.8, XX so.
 static Plan plan_of(int64_t m, int n, int k_tiles) {
-  Plan p{};
-  p.token_lanes = m > 128;
-  if (!p.token_lanes)
-    p.bn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
-  else
-    p.bn = 256;
-  auto tiles = [&]() {
-    const int64_t a = p.token_lanes ? m : n, b = p.token_lanes ? n : m;
-    return ((a + kBM - 1) / kBM) * ((b + p.bn - 1) / p.bn);
+  auto ceil_div = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  Plan best{};
+  double least = 1e300;
+  auto offer = [&](bool token_lanes, bool pair, int bn, int split, double cost) {
+    if (cost < least) {
+      least = cost;
+      best = Plan{token_lanes, pair, bn, split};
+    }
   };
-  if (p.token_lanes)
-    while (p.bn > 64 && tiles() < kSms / 2) p.bn /= 2;
-  p.split = 1;
-  // Pairs where their waves of tiles cost no more: a k step of a tile takes about 3/2 as long in the one-CTA
-  // kernel (product of 777 x 3584 -> 4608: 18.4 us against 18.8; 8192 x 4096 -> 14336: 281 against 310).
-  if (p.bn == 256) {
-    const int64_t pairs = ((m + 2 * kBM - 1) / (2 * kBM)) * ((n + 255) / 256);
-    p.pair = (pairs + kSms / 2 - 1) / (kSms / 2) * 2 <= (tiles() + kSms - 1) / kSms * 3;
-  }
-  // K is cut until the SMs have a CTA each. Twice as many parts, two CTAs an SM, measured no faster where the
-  // weights are many (64 x 18944 -> 3584: 22.5 us against 22.1) and slower where they are few, for the longer
-  // reduction (one token through 4096 x 4096: 10.3 against 8.3).
-  if (p.bn <= 128)
-    while (p.split < kMaxSplit && tiles() * p.split * 2 <= kSms && k_tiles / (p.split * 2) >= 4) p.split *= 2;
-  return p;
+  auto one_cta = [&](bool token_lanes, int bn) {
+    const int64_t tiles = ceil_div(token_lanes ? m : n, kBM) * ceil_div(token_lanes ? n : m, bn);
+    for (int split = 1; split <= kMaxSplit; split *= 2) {
+      // a part has work, a cluster's CTAs are resident together
+      if (split > 1 && (k_tiles / split < 4 || tiles * split > kSms || bn > 128 || bn < 2 * split)) break;
+      const double steps = static_cast<double>(ceil_div(k_tiles, split)) * 2 * (kBM + bn);
+      const double out = (token_lanes && split == 1 ? 8. : 60.) * bn / split + (split > 1 ? 2500 : 0);
+      offer(token_lanes, false, bn, split, ceil_div(tiles * split, kSms) * steps + out);
+    }
+  };
+  if (m <= 128) one_cta(false, m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128);
+  if (m > 32)
+    for (int bn = 64; bn <= 256; bn *= 2) one_cta(true, bn);
+  if (m > 128)
+    for (int bn = 256; bn >= 128; bn -= 32) {
+      const double step = 2 * (kBM + bn / 2) > 2 * bn ? 2 * (kBM + bn / 2) : 2 * bn;
+      const int64_t waves = ceil_div(ceil_div(m, 2 * kBM) * ceil_div(n, bn), kSms / 2);
+      offer(true, true, bn, 1, waves * (step * k_tiles) + 8. * bn + 1000);
+    }
+  return best;
 }
 
 static int make_map(CUtensorMap* m, const void* base, int64_t rows, int k, int64_t stride, int box_rows) {
@@ -962,6 +982,7 @@ static int matmul(const int8_t* x8, int64_t x_stride, const float* x_scale, cons
   g.rows_b = static_cast<int>(p.token_lanes ? out_features : tokens);
   g.k_tiles = k_tiles;
   g.split = p.split;
+  g.bn = p.bn;
   g.tiles_a = (g.rows_a + (p.pair ? 2 : 1) * kBM - 1) / ((p.pair ? 2 : 1) * kBM);
   g.tiles_b = (g.rows_b + p.bn - 1) / p.bn;
   if (static_cast<int64_t>(g.tiles_a) * g.tiles_b * p.split > 0x7fffffffll - 1024) return TM_ERR_UNSUPPORTED;
@@ -976,7 +997,7 @@ static int matmul(const int8_t* x8, int64_t x_stride, const float* x_scale, cons
   CUtensorMap mx, mw;
   int rc = make_map(&mx, x8, tokens, in_features, x_stride, p.token_lanes ? kBM : p.bn);
   if (rc != TM_OK) return rc;
-  rc = make_map(&mw, w8, out_features, in_features, w_stride, p.token_lanes && !p.pair ? p.bn : kBM);
+  rc = make_map(&mw, w8, out_features, in_features, w_stride, p.pair ? p.bn / 2 : p.token_lanes ? p.bn : kBM);
   if (rc != TM_OK) return rc;
   const CUtensorMap& ma = p.token_lanes ? mx : mw;
   const CUtensorMap& mb = p.token_lanes ? mw : mx;

@@ -50,44 +50,36 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 struct RowScale {
-  float k, amax, r;  // codes are round(k x / amax), r = 1 / amax (correctly rounded)
+  float k;     // codes are round(k x / amax), k = 127 times a power of two
+  QuantDiv d;  // division by amax (times that power of two)
   bool ok;
 };
 
-// k x = 127 x (times a power of two) is exact in fp32 (x has at most 11 significant bits), and the quotient is formed from the correctly
-// rounded reciprocal with one residual correction (Markstein), so a quotient half way between two codes is
-// exact and the others are too far from one (2^-19 relative) for their rounding to matter: the code is
-// that of exact arithmetic. |x| <= amax, so |q| <= 127.
-__device__ __forceinline__ uint32_t code_of(float x, const RowScale& s) {
-  const float y = x * s.k;
-  const float q0 = __fmul_rn(y, s.r);
-  const float q = __fmaf_rn(__fmaf_rn(-q0, s.amax, y), s.r, q0);
-  return static_cast<uint32_t>(__float2int_rz(q + copysignf(0.5f, q))) & 0xffu;
-}
-
+// k x is exact in fp32 (x has at most 11 significant bits), and the quotient is the IEEE one (common.cuh), so a
+// quotient half way between two codes is exact and the others are too far from one (2^-19 relative) for their
+// rounding to matter: the code is that of exact arithmetic.
 __device__ __forceinline__ RowScale row_scale(float amax) {
   // bf16 rows reach from 1e-40 to 3e38: a power of two on both sides of the quotient keeps the product, the
   // reciprocal and the residual normal.
   const float p = amax < 5.421010862e-20f ? 1.844674407e19f : amax > 1.844674407e19f ? 5.421010862e-20f : 1.f;  // 2^+-64
   RowScale s;
   s.k = 127.f * p;
-  s.amax = amax * p;
   s.ok = amax > 0.f && amax <= 3.4028235e38f;
-  s.r = s.ok ? __frcp_rn(s.amax) : 0.f;
+  s.d.init(s.ok ? amax * p : 1.f);
   return s;
 }
 
 template <typename T>
 __device__ __forceinline__ uint2 codes8(const uint4& v, const RowScale& s) {
   const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-  uint32_t c[8];
+  uint32_t c[8];  // codes in the low bytes
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = unpack2<T>(in[i]);
-    c[2 * i] = code_of(f.x, s);
-    c[2 * i + 1] = code_of(f.y, s);
+    quant_code_pair<kNumericsExact>(f.x * s.k, f.y * s.k, s.d, &c[2 * i], &c[2 * i + 1]);
   }
-  return make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+  return make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
 }
 
 template <int kThreads>
@@ -136,8 +128,11 @@ __global__ void __launch_bounds__(kThreads) quant_rows_kernel(const T* x, int64_
     for (int c = threadIdx.x; c < cols; c += kThreads) m = max_nan(m, fabsf(to_float(row[c])));
     m = block_max<kThreads>(m);
     const RowScale s = row_scale(m);
-    for (int c = threadIdx.x; c < cols; c += kThreads)
-      dst[c] = s.ok ? static_cast<int8_t>(code_of(to_float(row[c]), s)) : int8_t(0);
+    for (int c = threadIdx.x; c < cols; c += kThreads) {
+      uint32_t code, unused;
+      quant_code_pair<kNumericsExact>(to_float(row[c]) * s.k, 0.f, s.d, &code, &unused);
+      dst[c] = s.ok ? static_cast<int8_t>(code & 0xffu) : int8_t(0);
+    }
   }
   if (threadIdx.x == 0) scale[blockIdx.x] = __fdiv_rn(m, 127.f);
 }
@@ -148,9 +143,9 @@ static void run_quant(const T* x, int64_t xs, unsigned rows, int cols, int8_t* o
   quant_rows_kernel<T, kVec, kThreads><<<rows, kThreads, 0, st>>>(x, xs, cols, out, os, scale);
 }
 
-// 1024 threads a row where rows are fewer than two an SM (64 rows of 18944: 11 us with 256 threads that read it twice,
+// 1024 threads a row where rows are fewer than SMs (64 rows of 18944: 11 us with 256 threads that read it twice,
 // 5 us so), 256 where they are many: a CTA's reduction then hides behind the others' loads (4096 rows of 18944: 120 us
-// with 1024 threads, XX so).
+// with 1024 threads, 58 so).
 template <typename T>
 static void launch_quant(const void* x, int64_t xs, int64_t rows, int cols, int8_t* out, int64_t os, float* scale,
                          cudaStream_t st) {
@@ -161,7 +156,7 @@ static void launch_quant(const void* x, int64_t xs, int64_t rows, int cols, int8
     run_quant<T, 0, 1024>(p, xs, g, cols, out, os, scale, st);
   else if (cols <= 2048)
     run_quant<T, 1, 256>(p, xs, g, cols, out, os, scale, st);
-  else if (rows < 2 * 148) {
+  else if (rows < 148) {
     if (cols <= 8192)
       run_quant<T, 1, 1024>(p, xs, g, cols, out, os, scale, st);
     else if (cols <= 16384)
@@ -288,21 +283,18 @@ __device__ __forceinline__ void emit(const uint32_t* acc, const GemmArgs& g, int
 // With the tokens on the lanes: kRowBytes of each of a warp's 32 rows through shared memory, so that they are
 // stored as whole sectors side by side (a lane's own row would be 32 separate pieces a store). 16-byte pieces are
 // swizzled by the row against bank conflicts.
-template <typename OutT, int kRowBytes>
-__device__ __forceinline__ void emit_rows(uint32_t taddr, uint8_t* piece, const GemmArgs& g, int a0, int b0,
+// `load(c, sums)` brings the lane's sums of columns c .. of the piece.
+template <typename OutT, int kRowBytes, typename Load>
+__device__ __forceinline__ void emit_rows(Load load, uint8_t* piece, const GemmArgs& g, int a0, int b0,
                                           float row_scale, const float* col_scale, const float* col_bias) {
   constexpr int kCols = kRowBytes / sizeof(OutT), kPer = 16 / sizeof(OutT), kChunks = kRowBytes / 16;
-  constexpr int kLoad = kCols < 32 ? kCols : 32;  // columns a TMEM load
+  constexpr int kLoad = kCols < 32 ? kCols : 32;  // columns a load
   const int lane = threadIdx.x & 31;
   auto at = [](int row, int chunk) { return row * kRowBytes + ((chunk ^ (row * kRowBytes / 128 & (kChunks - 1))) << 4); };
 #pragma unroll
   for (int h = 0; h < kCols / kLoad; ++h) {
     uint32_t r[kLoad];
-    if constexpr (kLoad == 32)
-      tmem_ld32(taddr + 32 * h, r);
-    else
-      tmem_ld16(taddr + 16 * h, r);
-    tmem_wait_ld();
+    load(kLoad * h, r);
 #pragma unroll
     for (int c = 0; c < kLoad; c += kPer) {
       float v[kPer];
@@ -348,27 +340,58 @@ __device__ __forceinline__ void emit_rows(uint32_t taddr, uint8_t* piece, const 
   __syncwarp();
 }
 
-// The sum over the cluster of kSplit partial tiles of this rank's columns; all loads of a column are in flight
-// together.
+// emit_rows' sums from TMEM.
+struct FromTmem {
+  uint32_t taddr;
+  __device__ __forceinline__ void operator()(int c, uint32_t (&r)[32]) const {
+    tmem_ld32(taddr + c, r);
+    tmem_wait_ld();
+  }
+  __device__ __forceinline__ void operator()(int c, uint32_t (&r)[16]) const {
+    tmem_ld16(taddr + c, r);
+    tmem_wait_ld();
+  }
+};
+
+// The sum over the cluster of kSplit partial tiles of this rank's columns, with the loads of several columns and
+// all parts in flight together.
 template <int kSplit, int BN, bool kTokenLanes, typename OutT>
-__device__ __forceinline__ void reduce_split(uint32_t red, const GemmArgs& g, int a, int b0, int rank, float row_scale,
-                                             float row_bias, const float* col_scale, const float* col_bias) {
-  constexpr int kCols = BN / kSplit, kStep = kCols < 4 ? kCols : 4;
-  for (int c = rank * kCols; c < (rank + 1) * kCols; c += kStep) {
-    int32_t part[kSplit][kStep];
+__device__ __forceinline__ void reduce_split(uint32_t red, uint8_t* piece, const GemmArgs& g, int a0, int b0, int rank,
+                                             float row_scale, float row_bias, const float* col_scale,
+                                             const float* col_bias) {
+  constexpr int kCols = BN / kSplit;
+  auto sums = [&](int c, auto& sum) {
+    constexpr int n = sizeof(sum) / 4, kFlight = n < 32 / kSplit ? n : 32 / kSplit;
 #pragma unroll
-    for (int p = 0; p < kSplit; ++p)
+    for (int i0 = 0; i0 < n; i0 += kFlight) {
+      int32_t part[kSplit][kFlight];
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) part[p][i] = ld_cluster(red + (c + i) * (kBM * 4), p);
-    uint32_t sum[kStep];
+      for (int p = 0; p < kSplit; ++p)
 #pragma unroll
-    for (int i = 0; i < kStep; ++i) {
-      int32_t v = part[0][i];
+        for (int i = 0; i < kFlight; ++i) part[p][i] = ld_cluster(red + (c + i0 + i) * (kBM * 4), p);
 #pragma unroll
-      for (int p = 1; p < kSplit; ++p) v += part[p][i];
-      sum[i] = static_cast<uint32_t>(v);
+      for (int i = 0; i < kFlight; ++i) {
+        int32_t v = part[0][i];
+#pragma unroll
+        for (int p = 1; p < kSplit; ++p) v += part[p][i];
+        sum[i0 + i] = static_cast<uint32_t>(v);
+      }
     }
-    emit<kStep, kTokenLanes, OutT>(sum, g, a, b0 + c, row_scale, row_bias, col_scale + c, col_bias + c);
+  };
+  if constexpr (kTokenLanes) {
+    constexpr int kRowBytes = kCols * static_cast<int>(sizeof(OutT)) < 128 ? kCols * static_cast<int>(sizeof(OutT)) : 128;
+    constexpr int kStep = kRowBytes / static_cast<int>(sizeof(OutT));
+    for (int c = rank * kCols; c < (rank + 1) * kCols; c += kStep)
+      emit_rows<OutT, kRowBytes>([&](int at, auto& sum) { sums(c + at, sum); }, piece, g, a0, b0 + c, row_scale,
+                                 col_scale + c, col_bias + c);
+  } else {
+    constexpr int kStep = kCols < 8 ? kCols : 8;
+    for (int c = rank * kCols; c < (rank + 1) * kCols; c += kStep) {
+      uint32_t sum[kStep];
+      sums(c, sum);
+      emit<kStep, kTokenLanes, OutT>(sum, g, a0 + (threadIdx.x & 31), b0 + c, row_scale, row_bias, col_scale + c,
+                                     col_bias + c);
+    }
   }
 }
 
@@ -538,7 +561,7 @@ __global__ void __launch_bounds__(kGemmThreads) gemm_kernel(const __grid_constan
           constexpr int kCols = 128 / sizeof(OutT);
 #pragma unroll 1
           for (int c = 0; c < BN; c += kCols)
-            emit_rows<OutT, 128>(d + c, piece, g, ta * kBM + quad * 32, tb * BN + c, row_scale, col_scale + c, col_bias + c);
+            emit_rows<OutT, 128>(FromTmem{d + c}, piece, g, ta * kBM + quad * 32, tb * BN + c, row_scale, col_scale + c, col_bias + c);
         } else {
 #pragma unroll 1
           for (int c = 0; c < BN; c += 16) {
@@ -577,8 +600,9 @@ __global__ void __launch_bounds__(kGemmThreads) gemm_kernel(const __grid_constan
       const uint32_t red = smem_u32(smem) + row * 4;
       const float* col_scale = reinterpret_cast<const float*>(smem + S::kOffCols);
       auto reduce = [&](auto parts) {
-        reduce_split<decltype(parts)::value, BN, kTokenLanes, OutT>(red, g, ta * kBM + row, tb * BN, rank, row_scale,
-                                                                    row_bias, col_scale, col_scale + BN);
+        reduce_split<decltype(parts)::value, BN, kTokenLanes, OutT>(
+            red, smem + S::kOffPieces + (warp & 3) * 4096, g, ta * kBM + (warp & 3) * 32, tb * BN, rank, row_scale,
+            row_bias, col_scale, col_scale + BN);
       };
       if (g.split == 2)
         reduce(std::integral_constant<int, 2>{});
@@ -605,14 +629,20 @@ __global__ void __launch_bounds__(kGemmThreads) gemm_kernel(const __grid_constan
 // wave of tiles is full.
 struct PairShape {
   static constexpr int kBN = 256;  // widest
-  static constexpr int kStageBytes = (kBM + kBN / 2) * kBK;
-  static constexpr int kStages = 6;
+  // The ring holds as many stages as there is room for, six of the widest: a stage is on its way for about 3300
+  // cycles (both CTAs' copies, the products, the word back to both), so narrow ones have to be more.
+  static constexpr int kRing = 6 * (kBM + kBN / 2) * kBK;
+  static constexpr int kMaxStages = 8;
+  static __host__ __device__ int stage_bytes(int bn) { return (kBM + bn / 2) * kBK; }
+  static __host__ __device__ int stages(int bn) {
+    return kRing / stage_bytes(bn) < kMaxStages ? kRing / stage_bytes(bn) : kMaxStages;
+  }
   // Eight epilogue warps, two for each quarter of the rows, half of the columns each: with one tile a CTA nothing
   // hides behind the epilogue.
   static constexpr int kEpilogueWarps = 8;
   static constexpr int kRowBytes = 64;  // of output a row and warp at a time: what room six stages leave
   static constexpr int kThreads = 128 + 32 * kEpilogueWarps;
-  static constexpr int kOffCols = kStages * kStageBytes;
+  static constexpr int kOffCols = kRing;
   static constexpr int kOffPieces = kOffCols + 2 * 2 * kBN * 4;
   static constexpr int kSmem = kOffPieces + kEpilogueWarps * 32 * kRowBytes + 1024;
 };
@@ -659,15 +689,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
   using S = PairShape;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], acc_full[2], acc_empty[2], drain;
+  __shared__ __align__(8) uint64_t full[S::kMaxStages], empty[S::kMaxStages], acc_full[2], acc_empty[2], drain;
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x & 1, first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
   const int tiles = g.tiles_a * g.tiles_b, bn = g.bn;
-  const uint32_t bytes = 2u * (kBM + bn / 2) * kBK;  // of a stage in both CTAs
+  const int stage_bytes = S::stage_bytes(bn), stages = S::stages(bn);
+  const uint32_t bytes = 2u * stage_bytes;  // of a stage in both CTAs
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
+    for (int s = 0; s < S::kMaxStages; ++s) {
       mbar_init(&full[s], 1);   // the first CTA's: its own arrival and the bytes of both
       mbar_init(&empty[s], 1);  // each CTA's: the products that read the stage are done
     }
@@ -706,10 +737,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
     if (first_tile < tiles) {
       int ta, tb;
       tile_at(first_tile, &ta, &tb);
-      early = min(S::kStages, g.k_tiles);
+      early = min(stages, g.k_tiles);
       for (int i = 0; i < early; ++i) {
         if (rank == 0) mbar_arrive_expect_tx_e(&full[i], bytes);
-        tma_load_pair_e(smem + i * S::kStageBytes + kBM * kBK, &map_b, first_cta(&full[i]), i * kBK,
+        tma_load_pair_e(smem + i * stage_bytes + kBM * kBK, &map_b, first_cta(&full[i]), i * kBK,
                         tb * bn + rank * (bn / 2));
       }
     }
@@ -718,7 +749,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
       int ta, tb;
       tile_at(t, &ta, &tb);
       for (int k = 0; k < g.k_tiles; ++k) {
-        uint8_t* st = smem + s * S::kStageBytes;
+        uint8_t* st = smem + s * stage_bytes;
         const bool half = used < early;
         if (!half) {
           if (!mbar_wait_spin(&empty[s], phase ^ 1, g.err, kErrTimeoutEmpty)) {
@@ -730,12 +761,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
         }
         tma_load_pair_e(st, &map_a, first_cta(&full[s]), k * kBK, (2 * ta + rank) * kBM);
         ++used;
-        if (++s == S::kStages) s = 0, phase ^= 1;
+        if (++s == stages) s = 0, phase ^= 1;
       }
     }
     if (!ok && rank == 0) {
-      for (int i = 0; i < S::kStages && used > i; ++i)
-        mbar_wait(&full[i], ((used - 1 - i) / S::kStages) & 1, g.err, kErrTimeoutDrain);
+      for (int i = 0; i < stages && used > i; ++i)
+        mbar_wait(&full[i], ((used - 1 - i) / stages) & 1, g.err, kErrTimeoutDrain);
     }
   } else if (warp == 1 && rank == 0) {
     const uint32_t idesc = make_idesc(2, 1, 0, 0, 2 * kBM, bn);
@@ -755,13 +786,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
           break;
         }
         tc_fence_after();
-        const uint32_t st = smem_u32(smem + s * S::kStageBytes);
+        const uint32_t st = smem_u32(smem + s * stage_bytes);
         const uint64_t da = make_sdesc(st, 16, 1024, 2), db = make_sdesc(st + kBM * kBK, 16, 1024, 2);
 #pragma unroll
         for (int i = 0; i < kBK / 32; ++i)
           mma_i8_pair_e(d, da + 2 * i, db + 2 * i, idesc, (k > 0 || i > 0) ? 1u : 0u);
         commit_pair_e(&empty[s]);
-        if (++s == S::kStages) s = 0, phase ^= 1;
+        if (++s == stages) s = 0, phase ^= 1;
       }
       if (ok) commit_pair_e(&acc_full[acc]);
     }
@@ -798,7 +829,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
       constexpr int kCols = S::kRowBytes / sizeof(OutT);
 #pragma unroll 1
       for (int c = side * kCols; c < bn; c += 2 * kCols)
-        emit_rows<OutT, S::kRowBytes>(d + c, piece, g, a0, tb * bn + c, row_scale, col_scale + c, col_bias + c);
+        emit_rows<OutT, S::kRowBytes>(FromTmem{d + c}, piece, g, a0, tb * bn + c, row_scale, col_scale + c, col_bias + c);
       tc_fence_before();
       __syncwarp();
       if (lane == 0)
@@ -822,13 +853,15 @@ struct Plan {
 };
 
 // Which kernel, how wide a tile and into how many parts K is cut, by sizes alone: the least of an estimate in SM
-// cycles. A step of 128 bytes of K costs what L2 has to deliver for it, 64 bytes a cycle and SM (18 TB/s in all,
-// from the one-CTA kernel at 8192 x 4096 -> 14336), or two cycles a column in the tensor core; a wave of CTAs costs
-// its steps; the epilogue 8 cycles a column of whole lines, 60 of single values (tokens on the columns, or a
-// split's share of them), and a split 2500 for its two meetings. Against rules by the number of tiles alone:
-// 256 x 18944 -> 3584 37 us, XX so; 128 x 512 -> 1000 12.8, XX so.
+// cycles. A step of 128 bytes of K costs the most of three: two cycles a column in the tensor core; what L2 has to
+// deliver, 64 bytes a cycle and SM when all of them ask (18 TB/s); the time a stage is on its way (2050 cycles, 3300
+// in a pair) over the stages of the ring. A wave of CTAs costs its steps; the epilogue 8 cycles a column of whole
+// lines, 60 of single values (tokens on the columns), and a split's two meetings 2500 and 20 a column of its share.
+// Against rules by the number of tiles alone: linear of 256 x 18944 -> 3584 37 us, 29 so; 1536 tokens 135, 102 so;
+// 128 x 512 -> 1000 12.8, 6.1 so.
 static Plan plan_of(int64_t m, int n, int k_tiles) {
   auto ceil_div = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  auto most = [](double a, double b, double c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); };
   Plan best{};
   double least = 1e300;
   auto offer = [&](bool token_lanes, bool pair, int bn, int split, double cost) {
@@ -837,24 +870,37 @@ static Plan plan_of(int64_t m, int n, int k_tiles) {
       best = Plan{token_lanes, pair, bn, split};
     }
   };
-  auto one_cta = [&](bool token_lanes, int bn) {
+  auto busy = [](int64_t ctas) { return ctas >= kSms ? 1. : static_cast<double>(ctas) / kSms; };
+  auto one_cta = [&](bool token_lanes, int bn, int stages) {
     const int64_t tiles = ceil_div(token_lanes ? m : n, kBM) * ceil_div(token_lanes ? n : m, bn);
     for (int split = 1; split <= kMaxSplit; split *= 2) {
-      // a part has work, a cluster's CTAs are resident together
-      if (split > 1 && (k_tiles / split < 4 || tiles * split > kSms || bn > 128 || bn < 2 * split)) break;
-      const double steps = static_cast<double>(ceil_div(k_tiles, split)) * 2 * (kBM + bn);
-      const double out = (token_lanes && split == 1 ? 8. : 60.) * bn / split + (split > 1 ? 2500 : 0);
-      offer(token_lanes, false, bn, split, ceil_div(tiles * split, kSms) * steps + out);
+      // A part has work, and all clusters are resident at once: a GPC has room for whole ones only, so clusters of
+      // four and eight do not reach every SM (36 tiles of 4 parts took two waves, 21 us instead of 11).
+      if (split > 1 && (k_tiles / split < 4 || tiles * split > (split == 2 ? kSms : 128) || bn > 128 || bn < 2 * split))
+        break;
+      const double step = most(2 * bn, 2050. / stages, 2 * (kBM + bn) * busy(tiles * split));
+      const double out = (!token_lanes ? 60. : split == 1 ? 8. : 20.) * bn / split + (split > 1 ? 2500 : 0);
+      offer(token_lanes, false, bn, split, ceil_div(tiles * split, kSms) * (step * ceil_div(k_tiles, split)) + out);
     }
   };
-  if (m <= 128) one_cta(false, m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128);
-  if (m > 32)
-    for (int bn = 64; bn <= 256; bn *= 2) one_cta(true, bn);
+  if (m <= 16)
+    one_cta(false, 16, GemmShape<16>::kStages);
+  else if (m <= 32)
+    one_cta(false, 32, GemmShape<32>::kStages);
+  else if (m <= 64)
+    one_cta(false, 64, GemmShape<64>::kStages);
+  else if (m <= 128)
+    one_cta(false, 128, GemmShape<128>::kStages);
+  if (m > 32) {
+    one_cta(true, 64, GemmShape<64>::kStages);
+    one_cta(true, 128, GemmShape<128>::kStages);
+    one_cta(true, 256, GemmShape<256>::kStages);
+  }
   if (m > 128)
     for (int bn = 256; bn >= 128; bn -= 32) {
-      const double step = 2 * (kBM + bn / 2) > 2 * bn ? 2 * (kBM + bn / 2) : 2 * bn;
-      const int64_t waves = ceil_div(ceil_div(m, 2 * kBM) * ceil_div(n, bn), kSms / 2);
-      offer(true, true, bn, 1, waves * (step * k_tiles) + 8. * bn + 1000);
+      const int64_t pairs = ceil_div(m, 2 * kBM) * ceil_div(n, bn);
+      const double step = most(2 * bn, 3300. / PairShape::stages(bn), 2 * (kBM + bn / 2) * busy(2 * pairs));
+      offer(true, true, bn, 1, ceil_div(pairs, kSms / 2) * (step * k_tiles) + 8. * bn + 1000);
     }
   return best;
 }

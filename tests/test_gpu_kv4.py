@@ -347,6 +347,43 @@ def test_masked_keys_and_empty_rows(cuda_device, dim):
     assert (out[-2:] == 3).all()  # rows behind the last request
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_what_is_not_finite_stays_with_the_rows_that_see_it(cuda_device, dim):
+    """New tokens whose keys or values are infinite or NaN leave the rows in front of them alone (their weight there is 0,
+    and 0 times NaN is NaN); the rows that see them are NaN, a value's in its group of channels only."""
+    from tilemix_b200.attention.kv4 import kv4_append, kv4_attention
+
+    kv_lens, new = [70, 33, 9, 40], [6, 33, 4, 20]
+    pool, table, lens, keys, values = _cache(cuda_device, kv_lens, 2, dim, 16, seed=9)
+
+    def spoil(b, pos, k_too):
+        x = torch.from_numpy(np.stack([keys[b][pos], values[b][pos]])).half().to(cuda_device)[:, None]
+        x[1, :, 0, 40] = float("inf")
+        values[b][pos, 0, 32:64] = np.nan
+        if k_too:
+            x[0, :, 1, 3] = float("nan")
+            keys[b][pos, 1, :32] = np.nan
+        kv4_append(x[0], x[1], pool, table[b, pos // 16:pos // 16 + 1].long() * 16 + pos % 16)
+
+    spoil(0, 67, False)
+    spoil(1, 32, True)
+    spoil(1, 7, False)
+    spoil(2, 8, True)
+    spoil(3, 25, True)
+    q, cu = _queries(cuda_device, new, 8, dim, seed=6)
+    out = kv4_attention(q, pool, table, lens, cu, 33)
+    ends = cu.tolist()
+    for b, n in enumerate(new):
+        rows = slice(ends[b], ends[b + 1])
+        with np.errstate(invalid="ignore"):
+            ref, bound = ora.attention(q[rows].cpu().numpy(), keys[b], values[b], kv_lens[b], dim ** -0.5, True)
+        got = out[rows].double().cpu().numpy()
+        assert np.array_equal(np.isnan(got), np.isnan(ref)), b
+        fine = ~np.isnan(ref)
+        assert np.isnan(ref).any() and fine[0].all() == (b in (0, 1, 2, 3))
+        assert (np.abs(got - ref)[fine] <= bound[fine]).all(), b
+
+
 @pytest.mark.parametrize("v_scale", [1e-5, 300.0])
 def test_small_and_large_values(cuda_device, v_scale):
     from tilemix_b200.attention.kv4 import kv4_attention

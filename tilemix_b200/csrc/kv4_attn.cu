@@ -45,7 +45,8 @@ constexpr int kStepKeys = kStepBlocks * kBlockTokens;
 constexpr int kChunkKeys = kStepKeys * kAttnWarps;    // keys of one step of every warp: the unit of work
 constexpr int kSms = 148;
 // What a run of chunks costs beside its chunks (queries, pages, merge and store), in chunks. Without it a CTA
-// with several short requests was the last to end: 64 requests of 512 to 8192 keys took 94 us, 82 so (89 with 1, 83 with 2).
+// with several short requests was the last to end: 64 requests of 512 to 8192 keys took 94 us, 82 so (89 with 1, 83
+// with 2).
 constexpr int kSetup = 4;
 
 // CTAs an SM of the kernel for head_dim d and nt row tiles, by registers and shared memory.
@@ -197,9 +198,9 @@ __device__ __forceinline__ Words<N> load_words(const uint8_t* p) {
 }
 
 // The work of a call is the list of all chunks: by request, then KV head, then row tile, then key, with kSetup
-// places in front of each (KV head, row tile). CTA c takes places [c per, (c + 1) per), whatever requests they belong to, so ragged lengths leave no CTA behind; a
-// (KV head, row tile) that several CTAs share leaves partial states for the join, one that a CTA has whole is
-// written at once. A CTA's first run of chunks may continue another's (slot 2 c), its last may be continued
+// places in front of each (KV head, row tile). CTA c takes places [c per, (c + 1) per), whatever requests they
+// belong to, so ragged lengths leave no CTA behind; a (KV head, row tile) that several CTAs share leaves partial
+// states for the join, one that a CTA has whole is written at once. A CTA's first run of chunks may continue another's (slot 2 c), its last may be continued
 // (slot 2 c + 1).
 template <int D, int NT>
 __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(const AttnArgs a) {
@@ -461,6 +462,31 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
             *reinterpret_cast<uint16_t*>(vs + L::v_scale(j, tok)) = 0;
             *reinterpret_cast<uint16_t*>(vs + L::v_scale(j, tok) + 8) = 0;
           }
+        }
+        fence_proxy_async_smem();  // before the next copy into this stage
+        __syncwarp();
+      }
+
+      if (lim_lo < lim_hi && key + kStepKeys > lim_lo) {
+        // Keys that only some rows of the tile see: 0 times a V that is not finite would be NaN in the others. Its
+        // scale and minimum become 0, and the rows that see it get the NaN here.
+        uint8_t* vs = st + lane / kBlockTokens * L::kBlockBytes + L::kOffVScale;
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          uint16_t* sm = reinterpret_cast<uint16_t*>(vs + L::v_scale(j, lane % kBlockTokens));
+          const bool bad = ((live >> lane) & 1) && ((sm[0] & 0x7C00) == 0x7C00 || (sm[4] & 0x7C00) == 0x7C00);
+          const uint32_t keys = __ballot_sync(0xffffffffu, bad);
+          if (keys == 0) continue;
+          if (bad) sm[0] = sm[4] = 0;
+#pragma unroll
+          for (int x = 0; x < NT; ++x)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int n = lim[x][c] - key;
+              const uint32_t sees = n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
+              if (keys & sees)
+                o[x][2 * j][c] = o[x][2 * j][c + 2] = o[x][2 * j + 1][c] = o[x][2 * j + 1][c + 2] = CUDART_NAN_F;
+            }
         }
         fence_proxy_async_smem();  // before the next copy into this stage
         __syncwarp();
@@ -845,7 +871,8 @@ static int check(const tm_kv4_attn_params* p) {
   if (!(p->sm_scale > 0.f) || p->sm_scale > 3.4028235e38f) return TM_ERR_SHAPE;  // maxima are taken before scaling
   // the chunks of the work list are counted in 32 bits, with room for the last CTA's end
   const double rows = static_cast<double>(p->max_seqlen_q) * p->heads_q;
-  if (p->batch * (rows / 8 + p->heads_k) * (p->max_kv_len / kChunkKeys + 1.0 + kSetup) > 2147480000.0) return TM_ERR_UNSUPPORTED;
+  if (p->batch * (rows / 8 + p->heads_k) * (p->max_kv_len / kChunkKeys + 1.0 + kSetup) > 2147480000.0)
+    return TM_ERR_UNSUPPORTED;
   return TM_OK;
 }
 

@@ -182,6 +182,15 @@ def test_int8_projections_refuse_the_cpu():
         quantize_projections_int8(_model("cpu"))
 
 
+def test_int8_projections_are_not_sharded(cuda_device):
+    from tilemix_b200.models.int8_projections import quantize_projections_int8
+    from tilemix_b200.models.tensor_parallel import shard_model_for_tensor_parallel
+
+    model = quantize_projections_int8(_model(cuda_device))
+    with pytest.raises(ValueError, match="cannot be sharded"):
+        shard_model_for_tensor_parallel(model, 0, 2)
+
+
 @pytest.mark.parametrize("kind", ["llama", "qwen"])
 def test_the_whole_path_together(cuda_device, kind):
     """8-bit projections, TileMix prefill (its CUDA norms, rotary and SiLU for Llama), decode over the 4-bit cache: close

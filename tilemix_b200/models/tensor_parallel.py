@@ -32,6 +32,8 @@ import torch
 import torch.distributed as dist
 from torch import Tensor, nn
 
+from tilemix_b200.linear.int8_linear import Int8Linear
+
 __all__ = ["HeadSplit", "head_split", "column_split", "RowParallelLinear", "shard_model_for_tensor_parallel"]
 
 
@@ -127,6 +129,8 @@ def shard_model_for_tensor_parallel(model, rank: Optional[int] = None, world_siz
     hd = getattr(cfg, "head_dim", None) or cfg.hidden_size // nh
     hs = head_split(nh, nkv, rank, world_size)
     root = model.model if hasattr(model, "model") else model
+    if any(isinstance(m, Int8Linear) for m in root.modules()):
+        raise ValueError("projections in 8-bit integers (quantize_projections_int8) cannot be sharded")
     for layer in root.layers:
         attn = layer.self_attn
         _slice_rows(attn.q_proj, hs.q_lo * hd, hs.q_hi * hd)

@@ -254,3 +254,15 @@ def test_c_abi_refusals_need_no_gpu():
         assert tables(**over) == status, over
     assert lib().tm_release_pages(None, None, None, 0, 4, None, 8, None, 3, 16, None, None) == -1
     assert lib().tm_release_pages(fake, fake, fake, 4, 4, fake, 8, fake, 3, 17, None, None) == -2
+
+
+def test_the_first_call_cannot_be_captured(monkeypatch):
+    """It allocates the error word, which must not belong to a graph's memory."""
+    from tilemix_b200 import _lib
+    from tilemix_b200.attention import tilemix
+
+    monkeypatch.setattr(_lib, "_ERROR_WORD_PTRS", {})
+    monkeypatch.setattr(tilemix, "_ERROR_WORDS", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        _lib.error_word_ptr(0)

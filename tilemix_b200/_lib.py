@@ -224,8 +224,11 @@ def error_word_ptr(index: int) -> int:
     if ptr is None:
         import torch
 
-        from tilemix_b200.attention.tilemix import _error_word
+        from tilemix_b200.attention.tilemix import _ERROR_WORDS, _error_word
 
+        if index not in _ERROR_WORDS and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first call on a device allocates its error word and cannot be captured into a "
+                               "CUDA graph; make one call before the capture")
         ptr = _ERROR_WORD_PTRS[index] = _error_word(torch.device("cuda", index)).data_ptr()
     return ptr
 

@@ -176,7 +176,8 @@ class TileMixAttentionMixin:
         cache.append(k, v, self.layer_idx)
         if first and seqlen >= 16:
             return self._tilemix_attention(q, k, v, seqlen, k_quant=k_quant)
-        out = cache.attend(q, self.layer_idx, self.head_dim ** -0.5, _key_mask(attention_mask))
+        mask = _key_mask(attention_mask)
+        out = cache.attend(q, self.layer_idx, self.head_dim ** -0.5, None if mask is None else mask.expand(q.shape[0], -1))
         return out.transpose(1, 2)
 
     # -- the attention call (models/tilemix_llama.py:505-646)

@@ -24,7 +24,8 @@
 //     (the tensor core's operand type); p is rounded to fp16 as the prefill's
 //     kernels do; scores, maxima, sums and the output accumulate in fp32.
 // Rows with no key left give 0. Keys past the length or masked are excluded by
-// selecting, and their V by zero scales, so infinities and NaN there do not leak.
+// selecting, and a V of theirs that is not finite by a zero scale, so infinities
+// and NaN there do not leak.
 #include <cuda_fp16.h>
 #include <math_constants.h>
 
@@ -451,45 +452,38 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
     // (64 ragged requests 96 us, 84 with lengths that fill their steps).
     auto step = [&](const int key, const uint32_t live) {
       uint8_t* st = ring + s * kStageBytes;
-      if (live != 0xffffffffu) {
-        // The V scales and minima of keys that count for no row become 0, so that nothing of them (infinities, NaN,
-        // what an absent block's stage happens to hold) reaches the output.
-        const int tok = lane % kBlockTokens;
-        if (!((live >> lane) & 1)) {
-          uint8_t* vs = st + lane / kBlockTokens * L::kBlockBytes + L::kOffVScale;
+      if (live != 0xffffffffu || (lim_lo < lim_hi && key + kStepKeys > lim_lo)) {
+        // Keys that do not count, or only for some rows, have a weight of 0, and 0 times a V that is not finite
+        // (infinities, NaN, what an absent block's stage happens to hold) would be NaN: its scale and minimum become
+        // 0, and the rows that do see it get the NaN here. Where all are finite nothing is stored, and the next copy
+        // into the stage needs no fence.
+        uint8_t* vs = st + lane / kBlockTokens * L::kBlockBytes + L::kOffVScale;
+        auto sm_of = [&](int j) { return reinterpret_cast<uint16_t*>(vs + L::v_scale(j, lane % kBlockTokens)); };
+        // 15 s + |m| is finite under these (2^11, 2^15); beyond, an unused token's bytes may stand for an infinity
+        auto beyond = [](const uint16_t* sm, int s, int m) { return (sm[0] & 0x7FFF) >= s || (sm[4] & 0x7FFF) >= m; };
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < G; ++j) any |= beyond(sm_of(j), 0x6800, 0x7800);
+        if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
           for (int j = 0; j < G; ++j) {
-            *reinterpret_cast<uint16_t*>(vs + L::v_scale(j, tok)) = 0;
-            *reinterpret_cast<uint16_t*>(vs + L::v_scale(j, tok) + 8) = 0;
+            uint16_t* sm = sm_of(j);
+            const bool bad = beyond(sm, 0x7C00, 0x7C00);
+            const uint32_t keys = __ballot_sync(0xffffffffu, bad) & live;
+            if (bad || !((live >> lane) & 1)) sm[0] = sm[4] = 0;
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const int n = lim[x][c] - key;
+                const uint32_t sees = n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
+                if (keys & sees)
+                  o[x][2 * j][c] = o[x][2 * j][c + 2] = o[x][2 * j + 1][c] = o[x][2 * j + 1][c + 2] = CUDART_NAN_F;
+              }
           }
+          fence_proxy_async_smem();  // before the next copy into this stage
+          __syncwarp();
         }
-        fence_proxy_async_smem();  // before the next copy into this stage
-        __syncwarp();
-      }
-
-      if (lim_lo < lim_hi && key + kStepKeys > lim_lo) {
-        // Keys that only some rows of the tile see: 0 times a V that is not finite would be NaN in the others. Its
-        // scale and minimum become 0, and the rows that see it get the NaN here.
-        uint8_t* vs = st + lane / kBlockTokens * L::kBlockBytes + L::kOffVScale;
-#pragma unroll
-        for (int j = 0; j < G; ++j) {
-          uint16_t* sm = reinterpret_cast<uint16_t*>(vs + L::v_scale(j, lane % kBlockTokens));
-          const bool bad = ((live >> lane) & 1) && ((sm[0] & 0x7C00) == 0x7C00 || (sm[4] & 0x7C00) == 0x7C00);
-          const uint32_t keys = __ballot_sync(0xffffffffu, bad);
-          if (keys == 0) continue;
-          if (bad) sm[0] = sm[4] = 0;
-#pragma unroll
-          for (int x = 0; x < NT; ++x)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int n = lim[x][c] - key;
-              const uint32_t sees = n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
-              if (keys & sees)
-                o[x][2 * j][c] = o[x][2 * j][c + 2] = o[x][2 * j + 1][c] = o[x][2 * j + 1][c + 2] = CUDART_NAN_F;
-            }
-        }
-        fence_proxy_async_smem();  // before the next copy into this stage
-        __syncwarp();
       }
 
       float sc[kStepBlocks][NT][4];
@@ -626,12 +620,14 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
       }
     };
 
-    // The key mask is read a step ahead: one key of the step a lane.
+    // The key mask is read two steps ahead: one key of the step a lane (8 requests of several query tokens: 41 us with
+    // one step, 39 with two).
     auto mask_of = [&](int i) {
       const int key = key0 + kStepKeys * (warp + kAttnWarps * i) + lane;
-      return i < steps && key < min(lim_hi, a.mask_cols) && mask[key] != 0;
+      return i < steps && key < min(lim_hi, a.mask_cols) ? static_cast<uint32_t>(mask[key]) : 0u;
     };
-    bool mask_on = mask != nullptr && mask_of(0);
+    uint32_t mask_now = 0, mask_next = 0;
+    if (mask != nullptr) mask_now = mask_of(0), mask_next = mask_of(1);
     // The first steps of a run without a mask are plain: every key counts for every row.
     const int first_key = key0 + kStepKeys * warp, stride = kStepKeys * kAttnWarps;
     const int n_plain = mask != nullptr || lim_lo < first_key + kStepKeys ? 0 : (lim_lo - kStepKeys - first_key) / stride + 1;
@@ -641,8 +637,8 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
       if (i >= n_plain || stage_bad != 0) {
         const uint32_t bad = (stage_bad >> (kStepBlocks * s)) & ((1u << kStepBlocks) - 1);
         live = __ballot_sync(0xffffffffu, !((bad >> (lane / kBlockTokens)) & 1) && key + lane < lim_hi &&
-                                              (mask == nullptr || mask_on));
-        if (mask != nullptr) mask_on = mask_of(i + 1);
+                                              (mask == nullptr || mask_now != 0));
+        if (mask != nullptr) mask_now = mask_next, mask_next = mask_of(i + 2);
       }
       if (!mbar_wait_spin(&bar[s], phase, a.err, kErrTimeoutFull)) {
         ok = false;

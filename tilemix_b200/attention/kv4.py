@@ -14,7 +14,9 @@ token's head (``value = scale * code + minimum``, ``scale = (max - min) / 15`` r
 block table, in order. Every call is asynchronous on the current stream of its tensors' device and
 reads nothing back, so a decode step can be captured into a CUDA graph; what only the device can
 see (free pages running out, a page number or a slot outside the pool) ends in the device error
-word (``tilemix_b200.attention.tilemix.device_error_code``: 11, 12, 13), never in a stray access.
+word (``tilemix_b200.attention.tilemix.device_error_code``: 11, 12, 13), never in a stray access. The
+first call on a device allocates that word and comes before any capture. For inference: no gradient
+passes through.
 """
 from __future__ import annotations
 
@@ -126,7 +128,7 @@ def release_pages(lens: Tensor, done: Tensor, block_table: Tensor, free_pages: T
     if done.numel() != batch or block_table.shape[0] != batch or free_span.numel() != 2:
         raise ValueError("lens, done and block_table must agree on the batch, free_span has two entries")
     _launch_release(index, lens.data_ptr(), done.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-           block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_span.data_ptr(), batch, page_size)
+                    block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_span.data_ptr(), batch, page_size)
 
 
 def _page_bytes(page_size: int, head_dim: int) -> int:
@@ -216,8 +218,8 @@ def kv4_attention(q: Tensor, pool: Tensor, block_table: Tensor, kv_lens: Tensor,
     [batch, columns], optional) excludes keys for every row of a request; a key behind its last
     column is excluded too. A row that sees no key is 0. ``max_kv_len`` bounds ``kv_lens`` on the
     host (default: the table's capacity). Keys beyond it, or query tokens beyond ``max_seqlen_q``, are
-    left out (``device_error_code`` 11); a small bound makes for a small launch. Rows of ``q`` that belong to no request are left as they
-    were in ``out``.
+    left out (``device_error_code`` 11); a small bound makes for a small launch. Rows of ``q`` that belong
+    to no request are left as they were in ``out``.
     """
     if not q.is_cuda:
         raise RuntimeError("the cache attention is a CUDA kernel")

@@ -8,8 +8,12 @@
 // with an infinity or a NaN reads back as NaN. Read back is the reverse, rounded
 // to fp16 once.
 //
-// HBM bounds both on a prefill (2 bytes + 5 bits a value). A thread holds 8
-// channels of K and of V (two 16-byte loads in flight), four lanes a group.
+// HBM should bound both on a prefill (2 bytes + 5 bits a value); append is bound
+// by the instructions it issues, so a thread has 16 channels of K and of V, two
+// lanes a group: what a token and head cost (slot, addresses, scales) and the
+// shuffles are shared by twice the values. 32768 tokens of 8 heads of 128: XX us
+// (51 with 8 channels a thread) where 27 would carry the bytes. Read back: 8
+// channels a thread, 25 us, at the copy rate.
 #include <cuda_fp16.h>
 #include <math_constants.h>
 
@@ -20,10 +24,12 @@
 namespace tilemix {
 namespace kv4 {
 
-// A CTA takes 16 consecutive tokens of one head, D / 8 lanes a token: consecutive tokens mostly share a block,
-// whose V scales (2 bytes a token in 8 places) then leave, or come, as whole sectors.
+// A CTA takes 16 consecutive tokens of one head, D / 16 (append) or D / 8 lanes a token: consecutive tokens mostly
+// share a block, whose V scales (2 bytes a token in 8 places) then leave, or come, as whole sectors.
 template <int D>
-constexpr int kThreads = kBlockTokens * D / 8;
+constexpr int kAppendThreads = kBlockTokens * D / 16;
+template <int D>
+constexpr int kReadThreads = kBlockTokens * D / 8;
 
 struct Pages {
   uint32_t heads;
@@ -85,17 +91,20 @@ __device__ __forceinline__ float quotient(float a, float b, float r) {
   return __fmaf_rn(__fmaf_rn(-q0, b, a), r, q0);
 }
 
-// Codes of a lane's 8 channels in nibble order (channel i at nibble i) and the
-// group's (s, m) as a half2. Four consecutive lanes hold the group.
-__device__ __forceinline__ uint32_t quantise8(const uint4& x, __half2* sm) {
-  const __half2 a = h2(x.x), b = h2(x.y), c = h2(x.z), d = h2(x.w);
-  __half2 lo2 = __hmin2_nan(__hmin2_nan(a, b), __hmin2_nan(c, d));
-  __half2 hi2 = __hmax2_nan(__hmax2_nan(a, b), __hmax2_nan(c, d));
-  // (min, -max) in one register, so the two reductions share their shuffles
+// Codes of a lane's 16 channels in nibble order (channel i at nibble i) and the
+// group's (s, m) as a half2. Two neighbouring lanes hold the group.
+__device__ __forceinline__ uint2 quantise16(const uint4& x0, const uint4& x1, __half2* sm) {
+  const uint32_t in[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+  __half2 lo2 = h2(in[0]), hi2 = lo2;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    lo2 = __hmin2_nan(lo2, h2(in[i]));
+    hi2 = __hmax2_nan(hi2, h2(in[i]));
+  }
+  // (min, -max) in one register, so the two reductions share their shuffle
   __half2 ext = __halves2half2(__hmin_nan(__low2half(lo2), __high2half(lo2)),
                                __hneg(__hmax_nan(__low2half(hi2), __high2half(hi2))));
-#pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) ext = __hmin2_nan(ext, h2(__shfl_xor_sync(0xffffffffu, u32(ext), o)));
+  ext = __hmin2_nan(ext, h2(__shfl_xor_sync(0xffffffffu, u32(ext), 1)));
   const float lo = __low2float(ext), hi = -__high2float(ext);
   const __half sh = __float2half_rd(quotient(__fsub_rn(hi, lo), 15.f, 1.f / 15.f));
   const float s = __half2float(sh);
@@ -105,10 +114,9 @@ __device__ __forceinline__ uint32_t quantise8(const uint4& x, __half2* sm) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
   const uint64_t r2 = pair(r, r), ns2 = pair(-s, -s), nlo2 = pair(-lo, -lo);
   const uint64_t magic2 = 0x4B4000004B400000ull;  // 1.5 * 2^23: rounds to nearest even in the low bits
-  const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-  uint64_t e[4], u[4];
+  uint64_t e[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const float2 f = __half22float2(h2(in[i]));
     e[i] = add2(pair(f.x, f.y), nlo2);
   }
@@ -116,50 +124,65 @@ __device__ __forceinline__ uint32_t quantise8(const uint4& x, __half2* sm) {
   // subnormal: there x - m is cut at 15 s.
   if (__any_sync(0xffffffffu, s < 6.103515625e-5f)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 8; ++i)
       e[i] = pair(fminf(__uint_as_float(static_cast<uint32_t>(e[i])), 15.f * s),
                   fminf(__uint_as_float(static_cast<uint32_t>(e[i] >> 32)), 15.f * s));
   }
+  uint32_t w[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint64_t q0 = mul2(e[i], r2);
-    u[i] = add2(fma2(fma2(q0, ns2, e[i]), r2, q0), magic2);
+  for (int h = 0; h < 2; ++h) {
+    uint64_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t q0 = mul2(e[4 * h + i], r2);
+      u[i] = add2(fma2(fma2(q0, ns2, e[4 * h + i]), r2, q0), magic2);
+    }
+    // sum of (0x4B400000 + n_i) 16^i modulo 2^32, less the constants'
+    w[h] = static_cast<uint32_t>(u[3] >> 32);
+#pragma unroll
+    for (int i = 6; i >= 0; --i) w[h] = (w[h] << 4) + static_cast<uint32_t>(u[i / 2] >> (32 * (i % 2)));
+    w[h] = ok ? w[h] - (0x4B400000u + 0xB4000000u + 0x40000000u) : 0u;
   }
-  // sum of (0x4B400000 + n_i) 16^i modulo 2^32, less the constants'
-  uint32_t w = static_cast<uint32_t>(u[3] >> 32);
-#pragma unroll
-  for (int i = 6; i >= 0; --i) w = (w << 4) + static_cast<uint32_t>(u[i / 2] >> (32 * (i % 2)));
-  return ok ? w - (0x4B400000u + 0xB4000000u + 0x40000000u) : 0u;
+  return make_uint2(w[0], w[1]);
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads<D>) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads<D>) append_kernel(const AppendArgs a) {
   using L = Layout<D>;
-  constexpr int kLanes = D / 8;  // lanes a row
+  constexpr int kLanes = D / 16;  // lanes a row
   __shared__ uint8_t* sh_block[kBlockTokens];  // each token's block, NULL: it is not stored
   __shared__ int sh_at[kBlockTokens];          // its place there
   __shared__ __half sh_scale[kBlockTokens][L::kGroups][2];
   const int head = blockIdx.x, in_cta = threadIdx.x / kLanes;
   const int tok = (blockIdx.z * gridDim.y + blockIdx.y) * kBlockTokens + in_cta;
   const int l = threadIdx.x % kLanes;
-  const int j = l >> 2, t = l & 3;
+  const int j = l >> 1, p = l & 1;  // channels 32 j + 16 p ..
   const bool there = tok < a.n_tokens;  // tokens behind the last one stay for the shuffles
   const int64_t slot = there ? a.slots[tok] : -1;
   const bool fits = slot >= 0 && slot < a.n_slots;
-  uint4 xk = make_uint4(0, 0, 0, 0), xv = xk;
+  uint4 xk[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)}, xv[2] = {xk[0], xk[0]};
   if (fits) {
-    xk = __ldcs(reinterpret_cast<const uint4*>(a.k + static_cast<int64_t>(tok) * a.k_st + (static_cast<int64_t>(head) * a.k_sh + 8 * l)));
-    xv = __ldcs(reinterpret_cast<const uint4*>(a.v + static_cast<int64_t>(tok) * a.v_st + (static_cast<int64_t>(head) * a.v_sh + 8 * l)));
+    const uint4* k = reinterpret_cast<const uint4*>(a.k + static_cast<int64_t>(tok) * a.k_st +
+                                                    (static_cast<int64_t>(head) * a.k_sh + 16 * l));
+    const uint4* v = reinterpret_cast<const uint4*>(a.v + static_cast<int64_t>(tok) * a.v_st +
+                                                    (static_cast<int64_t>(head) * a.v_sh + 16 * l));
+    xk[0] = __ldcs(k);
+    xk[1] = __ldcs(k + 1);
+    xv[0] = __ldcs(v);
+    xv[1] = __ldcs(v + 1);
   }
   __half2 ks, vs;
-  const uint32_t kw = quantise8(xk, &ks), vw = quantise8(xv, &vs);
-  // A V chunk holds 4 channels of each group: lanes of groups j and j ^ 1 trade halves, so that each
-  // stores one 32-bit word. The even group's lane keeps chunk 2t, the odd one's chunk 2t + 1.
-  const uint32_t other = __shfl_xor_sync(0xffffffffu, vw, 4);
-  const uint32_t vpair = (j & 1) ? __byte_perm(other, vw, 0x7632) : __byte_perm(vw, other, 0x5410);
+  const uint2 kw = quantise16(xk[0], xk[1], &ks), vw = quantise16(xv[0], xv[1], &vs);
+  // A V chunk holds 4 channels of each group, and a lane has four chunks' worth of its own: lanes of groups j and
+  // j ^ 1 trade halves, so that each stores two chunks' 32-bit words. The even group's lane keeps chunks 4 p and
+  // 4 p + 1, the odd one's the two after them.
+  const bool odd = j & 1;
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? vw.x : vw.y, 2);
+  const uint32_t mine = odd ? vw.y : vw.x;
+  const uint32_t va = odd ? other : mine, vb = odd ? mine : other;  // of the even and the odd group
   const int in_block = static_cast<int>(slot) & (kBlockTokens - 1);
   uint8_t* blk = fits ? a.pool + block_offset(slot, head, a.pages, L::kBlockBytes) : nullptr;
-  if (t == 0) {
+  if (p == 0) {
     sh_scale[in_cta][j][0] = __low2half(vs);
     sh_scale[in_cta][j][1] = __high2half(vs);
     if (j == 0) {
@@ -169,24 +192,26 @@ __global__ void __launch_bounds__(kThreads<D>) append_kernel(const AppendArgs a)
     }
   }
   if (fits) {
-    *reinterpret_cast<uint32_t*>(blk + in_block * L::kRowBytes + (t * L::kGroups + j) * 4) = kw;
-    const int g = 2 * t + (j & 1);
-    *reinterpret_cast<uint32_t*>(blk + L::kOffV + in_block * L::kRowBytes + g * (2 * L::kGroups) + (j & ~1) * 2) = vpair;
-    if (t == 0) *reinterpret_cast<__half2*>(blk + L::kOffKScale + in_block * L::kScaleBytes + j * 4) = ks;
+    uint32_t* kc = reinterpret_cast<uint32_t*>(blk + in_block * L::kRowBytes + (2 * p * L::kGroups + j) * 4);
+    kc[0] = kw.x;
+    kc[L::kGroups] = kw.y;
+    uint8_t* vc = blk + L::kOffV + in_block * L::kRowBytes + (4 * p + 2 * odd) * (2 * L::kGroups) + (j & ~1) * 2;
+    *reinterpret_cast<uint32_t*>(vc) = __byte_perm(va, vb, 0x5410);
+    *reinterpret_cast<uint32_t*>(vc + 2 * L::kGroups) = __byte_perm(va, vb, 0x7632);
+    if (p == 0) *reinterpret_cast<__half2*>(blk + L::kOffKScale + in_block * L::kScaleBytes + j * 4) = ks;
   }
   __syncthreads();
   // The V scales, a thread each, in the order in which a block holds them if its tokens follow on from the
   // first one's slot (any other order is as right, only slower).
   const int i = threadIdx.x;
-  if (i < kBlockTokens * L::kGroups * 2) {
-    const int quarter = i & 3, which = (i >> 2) & 1, tt = (i >> 3) & 3, jj = i >> 5;
-    const int first = sh_block[0] == nullptr ? 0 : sh_at[0];
-    const int token = (4 * quarter + tt - first) & (kBlockTokens - 1);
-    uint8_t* to = sh_block[token];
-    if (to != nullptr)
-      *reinterpret_cast<__half*>(to + L::kOffVScale + L::v_scale(jj, sh_at[token]) + 8 * which) =
-          sh_scale[token][jj][which];
-  }
+  static_assert(kAppendThreads<D> == kBlockTokens * L::kGroups * 2, "one V scale or minimum a thread");
+  const int quarter = i & 3, which = (i >> 2) & 1, tt = (i >> 3) & 3, jj = i >> 5;
+  const int first = sh_block[0] == nullptr ? 0 : sh_at[0];
+  const int token = (4 * quarter + tt - first) & (kBlockTokens - 1);
+  uint8_t* to = sh_block[token];
+  if (to != nullptr)
+    *reinterpret_cast<__half*>(to + L::kOffVScale + L::v_scale(jj, sh_at[token]) + 8 * which) =
+        sh_scale[token][jj][which];
 }
 
 struct ReadArgs {
@@ -215,7 +240,7 @@ __device__ __forceinline__ uint4 dequant8(uint32_t w, __half s, __half m) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads<D>) read_kernel(const ReadArgs a) {
+__global__ void __launch_bounds__(kReadThreads<D>) read_kernel(const ReadArgs a) {
   using L = Layout<D>;
   constexpr int kLanes = D / 8;
   const int head = blockIdx.x;
@@ -239,7 +264,7 @@ __global__ void __launch_bounds__(kThreads<D>) read_kernel(const ReadArgs a) {
     vs = v[0];
     vm = v[4];
   }
-  // as in append: the lane holds chunk 2 t (+ 1) of groups j and j ^ 1 and trades one half
+  // the lane holds chunk 2 t (+ 1) of groups j and j ^ 1 and trades one half
   const uint32_t other = __shfl_xor_sync(0xffffffffu, vpair, 4);
   const uint32_t vw = (j & 1) ? __byte_perm(other, vpair, 0x7632) : __byte_perm(vpair, other, 0x5410);
   if (!there) return;
@@ -308,9 +333,9 @@ extern "C" int tm_kv4_append(const void* k, int64_t k_stride_tok, int64_t k_stri
   const int64_t groups = (n_tokens + kBlockTokens - 1) / kBlockTokens;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128)
-    append_kernel<128><<<grid_of(groups, heads), kThreads<128>, 0, st>>>(a);
+    append_kernel<128><<<grid_of(groups, heads), kAppendThreads<128>, 0, st>>>(a);
   else
-    append_kernel<64><<<grid_of(groups, heads), kThreads<64>, 0, st>>>(a);
+    append_kernel<64><<<grid_of(groups, heads), kAppendThreads<64>, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? TM_OK : TM_ERR_LAUNCH;
 }
 
@@ -334,8 +359,8 @@ extern "C" int tm_kv4_read(const void* pool, int64_t num_pages, int heads, int h
   const int64_t groups = (n_tokens + kBlockTokens - 1) / kBlockTokens;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128)
-    read_kernel<128><<<grid_of(groups, heads), kThreads<128>, 0, st>>>(a);
+    read_kernel<128><<<grid_of(groups, heads), kReadThreads<128>, 0, st>>>(a);
   else
-    read_kernel<64><<<grid_of(groups, heads), kThreads<64>, 0, st>>>(a);
+    read_kernel<64><<<grid_of(groups, heads), kReadThreads<64>, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? TM_OK : TM_ERR_LAUNCH;
 }

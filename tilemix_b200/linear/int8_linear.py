@@ -10,7 +10,7 @@
 per-block quantiser of the attention). The integer sums are exact, so a result depends neither on
 the launch's shape nor on the batch a token is in. Rows of codes start on 16 bytes: with
 ``in_features`` not a multiple of 16 they are a view of wider rows, as
-:func:`quantize_per_token_int8` allocates them.
+:func:`quantize_per_token_int8` allocates them. For inference: no gradient passes through.
 """
 from __future__ import annotations
 
@@ -43,7 +43,7 @@ def quantize_per_token_int8(x: Tensor) -> tuple[Tensor, Tensor]:
     codes = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     _launch_quant(x.get_device(), x.data_ptr(), _DTYPES[x.dtype], x.stride(0), rows, cols,
-           codes.data_ptr(), codes.stride(0), scale.data_ptr())
+                  codes.data_ptr(), codes.stride(0), scale.data_ptr())
     return (codes if codes.shape[1] == cols else codes[:, :cols]), scale
 
 
@@ -102,8 +102,8 @@ def int8_matmul(x8: Tensor, x_scale: Tensor, w8: Tensor, w_scale: Tensor, bias: 
     _check_bias(bias, w8.shape[0], out_dtype, x8.get_device())
     out = torch.empty((x8.shape[0], w8.shape[0]), dtype=out_dtype, device=x8.device)
     _launch_matmul(x8.get_device(), x8.data_ptr(), x8.stride(0), x_scale.data_ptr(), w8.data_ptr(), w8.stride(0),
-           w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0),
-           _DTYPES[out_dtype], x8.shape[0], w8.shape[0], x8.shape[1])
+                   w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0),
+                   _DTYPES[out_dtype], x8.shape[0], w8.shape[0], x8.shape[1])
     return out
 
 
@@ -131,8 +131,8 @@ def int8_linear(x: Tensor, w8: Tensor, w_scale: Tensor, bias: Optional[Tensor] =
     scratch = w8.new_empty(m * (wide + 4))
     codes = scratch.data_ptr()
     _launch_linear(index, rows.data_ptr(), _DTYPES[dtype], row_stride, codes, wide, codes + m * wide,
-           w8.data_ptr(), w8.stride(0), w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), n,
-           m, n, k)
+                   w8.data_ptr(), w8.stride(0), w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                   out.data_ptr(), n, m, n, k)
     return out if x.ndim == 2 else out.view(*x.shape[:-1], n)
 
 

@@ -9,7 +9,9 @@
 ``_qwen``) prefills with the routed attention, stores its keys and values in 4 bits and attends
 over the cache itself (``kv4_attention``) in every later step, whatever its length; the prompt's
 first pass uses the unrounded keys and values, except for prompts under 16 tokens. Any other
-attention gets the cached keys and values read back as fp16 from ``update``.
+attention gets the cached keys and values read back as fp16 from ``update``. Of an attention mask
+the steps after the prompt use the keys that its last row allows: a batch's padding, not a pattern
+of its own for each new token.
 """
 from __future__ import annotations
 

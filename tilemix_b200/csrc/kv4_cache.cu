@@ -11,9 +11,10 @@
 // HBM should bound both on a prefill (2 bytes + 5 bits a value); append is bound
 // by the instructions it issues, so a thread has 16 channels of K and of V, two
 // lanes a group: what a token and head cost (slot, addresses, scales) and the
-// shuffles are shared by twice the values. 32768 tokens of 8 heads of 128: XX us
-// (51 with 8 channels a thread) where 27 would carry the bytes. Read back: 8
-// channels a thread, 25 us, at the copy rate.
+// shuffles are shared by twice the values. 32768 tokens of 8 heads of 128: 38 us
+// (51 with 8 channels a thread) where 27 would carry the bytes. Read back: 34 us
+// for the same, 8 channels a thread; 16 took a third fewer instructions and the
+// same time, so it waits for memory, not for its instructions.
 #include <cuda_fp16.h>
 #include <math_constants.h>
 

@@ -184,7 +184,8 @@ static void launch_quant(const void* x, int64_t xs, int64_t rows, int cols, int8
 // (a lane of TMEM is a token); with few, the weights are, and the tokens are the N side, as narrow as they
 // are (a lane is a channel): the tensor core then never works on padding rows and the weights stream through.
 // A split of K is a cluster of CTAs, one part each, whose int32 partial tiles are added through distributed
-// shared memory: exact, so without an effect on the result, and without a workspace.
+// shared memory: exact, so without an effect on the result, and without a workspace. 64 tokens of 18944 -> 3584: 19 us,
+// the weights at 3.5 TB/s from HBM (13.6 us from L2: about 5 us are the start, the first loads and the split's sum).
 constexpr int kBM = 128, kBK = 128;
 constexpr int kGemmThreads = 256;
 constexpr int kMaxSplit = 8;
@@ -626,7 +627,8 @@ __global__ void __launch_bounds__(kGemmThreads) gemm_kernel(const __grid_constan
 // channels' rows, the first one issues the products for both, each keeps its 128 rows of the sum in its own
 // TMEM. A CTA then reads 32 KB for each 128 bytes of K where it read 48 KB for the same number of products: the
 // one-CTA kernel is bound by what L2 delivers. The width is a multiple of 32 from 128 on, chosen so that the last
-// wave of tiles is full.
+// wave of tiles is full. 8192 x 4096 -> 14336: 282 us, 3410 TOP/s, the tensor pipe busy for 92 % of it; 310 us with one
+// CTA a tile.
 struct PairShape {
   static constexpr int kBN = 256;  // widest
   // The ring holds as many stages as there is room for, six of the widest: a stage is on its way for about 3300

@@ -23,6 +23,10 @@
 //     and one FMA with the group's scale and minimum, which rounds it to fp16 once
 //     (the tensor core's operand type); p is rounded to fp16 as the prefill's
 //     kernels do; scores, maxima, sums and the output accumulate in fp32.
+// 64 requests of 512 to 8192 keys (24 query heads, 8 of 128 cached): 84 us, 4.2
+// TB/s, where the bytes alone would take 54; one request of 131,072 keys 45 us (26).
+// What bounds it is the number of instructions, issued in 57 % of the cycles by
+// the three warps a scheduler that the registers leave room for.
 // Rows with no key left give 0. Keys past the length or masked are excluded by
 // selecting, and a V of theirs that is not finite by a zero scale, so infinities
 // and NaN there do not leak.

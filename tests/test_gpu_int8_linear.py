@@ -112,6 +112,46 @@ def test_quantiser_matches_its_definition(cuda_device, m, k, dtype):
     assert (np.abs(scale.double().cpu().numpy() - ref_scale) <= ref_scale * 2.0 ** -24).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,k", [(148, 1), (203, 323), (149, 1024), (301, 1025), (160, 8191), (150, 9001), (150, 3000),
+                                 (150, 8192), (149, 16384), (148, 24576), (150, 24584), (148, 32768)])
+def test_quantiser_of_many_rows(cuda_device, m, k, dtype):
+    """As many rows as SMs and more: other numbers of threads a row, one row of them not finite."""
+    from tilemix_b200.linear.int8_linear import quantize_per_token_int8
+
+    x = _rows(m, k, m + k, dtype).to(cuda_device)
+    if k % 3 == 0:  # a view: rows that start anywhere
+        x = torch.nn.functional.pad(x, (1, 2))[:, 1:k + 1]
+    ref, ref_scale = _codes_of(x)
+    x[5, k // 2] = float("nan")
+    x[6, k - 1] = float("-inf")
+    codes, scale = quantize_per_token_int8(x)
+    ref[5:7] = 0
+    assert np.array_equal(codes.cpu().numpy(), ref)
+    scale = scale.double().cpu().numpy()
+    assert np.isnan(scale[5]) and np.isposinf(scale[6])
+    fine = np.delete(np.arange(m), [5, 6])
+    assert (np.abs(scale - ref_scale)[fine] <= ref_scale[fine] * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(1300, 4663, 323), (777, 93, 843), (100, 511, 2048), (260, 2449, 860), (90, 4097, 512)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_odd_output_rows(cuda_device, m, n, k, dtype):
+    """Output rows that do not start on 16 bytes, and nothing written beside them."""
+    from tilemix_b200._lib import TM_DTYPE_FP16, TM_DTYPE_FP32, launcher
+
+    x8, xs, w8, ws = _operands(cuda_device, m, n, k, seed=m + n)
+    out = torch.full((m + 2, n + 3), 7.0, dtype=dtype, device=cuda_device)
+    inner = out[1:-1, 1:-2]
+    launcher("tm_int8_matmul")(0, x8.data_ptr(), x8.stride(0), xs.data_ptr(), w8.data_ptr(), w8.stride(0), ws.data_ptr(),
+                               0, inner.data_ptr(), inner.stride(0),
+                               TM_DTYPE_FP16 if dtype == torch.float16 else TM_DTYPE_FP32, m, n, k)
+    _check(inner, x8, xs, w8, ws)
+    beside = out.clone()
+    beside[1:-1, 1:-2] = 7
+    assert (beside == 7).all()
+
+
 def test_quantiser_takes_strided_and_unaligned_rows(cuda_device):
     from tilemix_b200.linear.int8_linear import quantize_per_token_int8
 

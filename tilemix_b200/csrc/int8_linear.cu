@@ -137,6 +137,50 @@ __global__ void __launch_bounds__(kThreads) quant_rows_kernel(const T* x, int64_
   if (threadIdx.x == 0) scale[blockIdx.x] = __fdiv_rn(m, 127.f);
 }
 
+// Rows that do not start on 16 bytes, value by value: kWarps warps a row, up to 32 values a thread in registers. One
+// warp (eight rows a CTA) where a row fits it: 3944 rows of 323 take 3.4 us, 19 with 1024 threads a row that read it
+// twice; 4096 rows of 5003 with eight 19, 41 so. Longer rows are read twice (4096 of 18947: 101 us, 131 with 1024
+// threads that hold them).
+template <typename T, int kWarps>
+__global__ void __launch_bounds__(256) quant_odd_kernel(const T* x, int64_t x_stride, unsigned rows, int cols,
+                                                        int8_t* out, int64_t out_stride, float* scale) {
+  static_assert(kWarps == 1 || kWarps == 8, "eight warps a CTA");
+  constexpr int kPer = 32;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product that follows may load its weights
+  constexpr int kRow = 32 * kWarps;
+  const unsigned r = kWarps == 1 ? blockIdx.x * 8 + threadIdx.x / 32 : blockIdx.x;
+  const int t = threadIdx.x % kRow;
+  if (r >= rows) return;  // a whole warp, and only where no one waits for it
+  const T* row = x + r * x_stride + t;
+  int8_t* dst = out + r * out_stride + t;
+  const int n = cols > t ? (cols - t + kRow - 1) / kRow : 0;  // values of this thread
+  T v[kPer];
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (i < n) v[i] = row[i * kRow];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (i < n) m = max_nan(m, fabsf(to_float(v[i])));
+  if constexpr (kWarps == 1) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  } else {
+    m = block_max<kRow>(m);
+  }
+  const RowScale s = row_scale(m);
+#pragma unroll
+  for (int i = 0; i < kPer; i += 2) {
+    if (i >= n) break;
+    const bool two = i + 1 < n;
+    uint32_t c[2];
+    quant_code_pair<kNumericsExact>(to_float(v[i]) * s.k, two ? to_float(v[i + 1]) * s.k : 0.f, s.d, &c[0], &c[1]);
+    dst[i * kRow] = s.ok ? static_cast<int8_t>(c[0] & 0xffu) : int8_t(0);
+    if (two) dst[(i + 1) * kRow] = s.ok ? static_cast<int8_t>(c[1] & 0xffu) : int8_t(0);
+  }
+  if (t == 0) scale[r] = __fdiv_rn(m, 127.f);
+}
+
 template <typename T, int kVec, int kThreads>
 static void run_quant(const T* x, int64_t xs, unsigned rows, int cols, int8_t* out, int64_t os, float* scale,
                       cudaStream_t st) {
@@ -152,8 +196,12 @@ static void launch_quant(const void* x, int64_t xs, int64_t rows, int cols, int8
   const T* p = static_cast<const T*>(x);
   const unsigned g = static_cast<unsigned>(rows);
   const bool vec = cols % 8 == 0 && aligned(x, 16) && xs % 8 == 0 && aligned(out, 8) && os % 8 == 0;
-  if (!vec || cols > 32768)
+  if (cols > 32768 || (!vec && (cols > 8192 || rows < 148)))
     run_quant<T, 0, 1024>(p, xs, g, cols, out, os, scale, st);
+  else if (!vec && cols <= 1024)
+    quant_odd_kernel<T, 1><<<(g + 7) / 8, 256, 0, st>>>(p, xs, g, cols, out, os, scale);
+  else if (!vec)
+    quant_odd_kernel<T, 8><<<g, 256, 0, st>>>(p, xs, g, cols, out, os, scale);
   else if (cols <= 2048)
     run_quant<T, 1, 256>(p, xs, g, cols, out, os, scale, st);
   else if (rows < 148) {
@@ -321,21 +369,35 @@ __device__ __forceinline__ void emit_rows(Load load, uint8_t* piece, const GemmA
   }
   __syncwarp();
   OutT* out = static_cast<OutT*>(g.out);
-  const int chunk = lane % kChunks, b = b0 + chunk * kPer;
+  if (g.vec) {
+    const int chunk = lane % kChunks, b = b0 + chunk * kPer;
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const int row = 32 / kChunks * i + lane / kChunks;
-    if (a0 + row < g.rows_a && b < g.rows_b) {
-      const uint4 w = *reinterpret_cast<const uint4*>(piece + at(row, chunk));
-      OutT* dst = out + static_cast<int64_t>(a0 + row) * g.ldo + b;
-      if (g.vec && b + kPer <= g.rows_b) {
-        *reinterpret_cast<uint4*>(dst) = w;
-      } else {
-        const OutT* e = reinterpret_cast<const OutT*>(&w);
+    for (int i = 0; i < kChunks; ++i) {
+      const int row = 32 / kChunks * i + lane / kChunks;
+      if (a0 + row < g.rows_a && b < g.rows_b) {
+        const uint4 w = *reinterpret_cast<const uint4*>(piece + at(row, chunk));
+        OutT* dst = out + static_cast<int64_t>(a0 + row) * g.ldo + b;
+        if (b + kPer <= g.rows_b) {
+          *reinterpret_cast<uint4*>(dst) = w;
+        } else {
+          const OutT* e = reinterpret_cast<const OutT*>(&w);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k)
-          if (b + k < g.rows_b) dst[k] = e[k];
+          for (int k = 0; k < kPer; ++k)
+            if (b + k < g.rows_b) dst[k] = e[k];
+        }
       }
+    }
+  } else {
+    // Rows that do not start on 16 bytes: a value a lane, side by side (3944 x 323 -> 4663 took 102 us with eight a
+    // lane, 51 so).
+    constexpr int kWide = kCols < 32 ? kCols : 32, kStep = 32 / kWide;
+    const int col = lane % kWide, rows = min(32, g.rows_a - a0);
+#pragma unroll 4
+    for (int row = lane / kWide; row < rows; row += kStep) {
+      OutT* dst = out + static_cast<int64_t>(a0 + row) * g.ldo + b0;
+#pragma unroll
+      for (int c = col; c < kCols; c += kWide)
+        if (b0 + c < g.rows_b) dst[c] = *reinterpret_cast<const OutT*>(piece + at(row, c / kPer) + c % kPer * sizeof(OutT));
     }
   }
   __syncwarp();

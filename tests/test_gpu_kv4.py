@@ -511,3 +511,50 @@ def test_repeated_calls_are_identical(cuda_device):
     first = kv4_attention(q, pool, table, lens, cu, 5)
     for _ in range(5):
         assert torch.equal(kv4_attention(q, pool, table, lens, cu, 5), first)
+
+
+# ---------------------------------------------------------------------------------------------- bounds that do not hold
+def _near(got, ref, bound):
+    """Whether every element is within its bound (a NaN is not)."""
+    return bool((np.abs(got - ref) <= bound).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_queries_beyond_their_bound_do_not_shift_the_others(cuda_device, dim):
+    """The rows of a request that has more than max_seqlen_q see the keys that they see without the bound."""
+    from tilemix_b200.attention.kv4 import kv4_attention
+
+    kv_lens, new, most = [64, 300, 70, 9], [3, 20, 5, 6], 4
+    pool, table, lens, keys, values = _cache(cuda_device, kv_lens, 2, dim, 16, seed=21)
+    q, cu = _queries(cuda_device, new, 4, dim, seed=21)
+    out = torch.full_like(q, 3.0)
+    kv4_attention(q, pool, table, lens, cu, most, out=out)
+    assert _error_code() == 11
+    got, rows = out.double().cpu().numpy(), q.cpu().numpy()
+    ends = cu.tolist()
+    for b, n in enumerate(new):
+        ref, bound = ora.attention(rows[ends[b]:ends[b + 1]], keys[b], values[b], kv_lens[b], dim ** -0.5, True)
+        served = min(n, most)
+        assert _near(got[ends[b]:ends[b] + served], ref[:served], bound[:served]), b
+        assert (got[ends[b] + served:ends[b + 1]] == 3).all(), b
+
+
+@pytest.mark.parametrize("more", [1, 3, 1000])
+def test_keys_beyond_their_bound_do_not_shift_the_others(cuda_device, more):
+    """A request of more keys than max_kv_len (or the table) holds: a row sees the keys up to its own place that are there."""
+    from tilemix_b200.attention.kv4 import kv4_attention
+
+    kv_lens, new = [64, 33], [5, 7]
+    pool, table, lens, keys, values = _cache(cuda_device, kv_lens, 2, 64, 16, seed=22, cols=4)
+    q, cu = _queries(cuda_device, new, 4, 64, seed=22)
+    longer = lens.clone()
+    longer[0] += more
+    out = kv4_attention(q, pool, table, longer, cu, 7, max_kv_len=64)
+    assert _error_code() == 11
+    got, rows = out.double().cpu().numpy(), q.cpu().numpy()
+    for i in range(5):  # row i sees min(64 + more - 5 + i + 1, 64) keys
+        seen = min(64, 64 + more - 5 + i + 1)
+        ref, bound = ora.attention(rows[i:i + 1], keys[0][:seen], values[0][:seen], seen, 64 ** -0.5, True)
+        assert _near(got[i:i + 1], ref, bound), i
+    ref, bound = ora.attention(rows[5:], keys[1], values[1], 33, 64 ** -0.5, True)
+    assert _near(got[5:], ref, bound)

@@ -90,23 +90,26 @@ struct AttnArgs {
 
 // A request's share of the work.
 struct Request {
-  int q0, n_q;   // its query tokens
-  int kv;        // its keys
+  int q0, n_q;   // its query tokens, at most max_q of them
+  int kv;        // its keys, at most max_kv of them
   int tiles;     // row tiles a KV head
   int chunks;    // chunks of kChunkKeys keys of one (KV head, row tile), at least 1
   int cost;      // those and kSetup, times the KV heads and row tiles: its length in the work list
 };
 
+// Query tokens by the offsets as they were given; 0 where these do not follow on from one another.
+__device__ __forceinline__ int given_queries(const AttnArgs& a, int b) {
+  if (a.cu == nullptr) return 1;
+  const int q0 = a.cu[b], q1 = a.cu[b + 1];
+  return q0 >= 0 && q1 > q0 ? q1 - q0 : 0;
+}
+
 template <int NT>
 __device__ __forceinline__ Request request_of(const AttnArgs& a, int b) {
   Request r;
-  r.q0 = b;
-  r.n_q = 1;
-  if (a.cu != nullptr) {
-    r.q0 = a.cu[b];
-    r.n_q = min(a.cu[b + 1] - r.q0, a.max_q);
-  }
-  if (r.q0 < 0 || r.n_q < 0 || r.q0 + static_cast<int64_t>(r.n_q) > a.q_tokens) r.n_q = 0;
+  r.q0 = a.cu != nullptr ? a.cu[b] : b;
+  r.n_q = min(given_queries(a, b), a.max_q);
+  if (r.q0 + static_cast<int64_t>(r.n_q) > a.q_tokens) r.n_q = 0;
   r.kv = static_cast<int>(min(static_cast<int64_t>(max(a.kv_lens[b], 0)), a.max_kv));
   r.tiles = (r.n_q * a.group + 8 * NT - 1) / (8 * NT);
   r.chunks = max(1, (r.kv + kChunkKeys - 1) / kChunkKeys);
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
       const Request r = request_of<NT>(a, b);
       at += r.cost;
       // more keys, or more query tokens, than the call said there may be: those beyond are left out
-      if (r.kv < a.kv_lens[b] || (a.cu != nullptr && a.cu[b + 1] - a.cu[b] > a.max_q)) record_error(a.err, kErrCachePlan);
+      if (r.kv < a.kv_lens[b] || given_queries(a, b) > a.max_q) record_error(a.err, kErrCachePlan);
     }
     if (lane == 0) a.starts[a.batch] = total;
   }
@@ -375,6 +378,10 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
     float cs[NT][2];     // log2 units a score unit of columns 2 t and 2 t + 1
     int lim[NT][2];                 // keys [0, lim) visible to them; padding rows see what the last row sees
     const int n_rows = rq.n_q * a.group;
+    // Keys in front of the request's first query token, by the lengths as they were given: max_q and max_kv leave tokens
+    // and keys out and do not move the others. Query token i sees before + i + 1 keys, which is at most the length.
+    // Looked up anew for each run: held with the request it cost a register of the loop below (64 requests of 512 to 8192 keys: 88 us, 86 so).
+    const int before = max(a.kv_lens[b], 0) - given_queries(a, b);
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
       const int r = row0 + 8 * x + g;
@@ -424,13 +431,13 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
         const int src = (2 * t + c) * 4;
         cs[x][c] = fmaxf(a.scale_log2 * __shfl_sync(0xffffffffu, down, src), 1.17549435e-38f);  // > 0: -inf stays -inf
         const int rc = min(row0 + 8 * x + 2 * t + c, n_rows - 1);
-        lim[x][c] = a.causal ? min(rq.kv, rq.kv - rq.n_q + rc / a.group + 1) : rq.kv;
+        lim[x][c] = a.causal ? min(rq.kv, before + rc / a.group + 1) : rq.kv;
       }
     }
     int lim_lo = rq.kv, lim_hi = rq.kv;
     if (a.causal) {
-      lim_lo = min(rq.kv, rq.kv - rq.n_q + row0 / a.group + 1);
-      lim_hi = min(rq.kv, rq.kv - rq.n_q + (min(row0 + kRows, n_rows) - 1) / a.group + 1);
+      lim_lo = min(rq.kv, before + row0 / a.group + 1);
+      lim_hi = min(rq.kv, before + (min(row0 + kRows, n_rows) - 1) / a.group + 1);
     }
     const uint8_t* mask = a.mask != nullptr ? a.mask + b * a.mask_stride : nullptr;
 

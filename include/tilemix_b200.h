@@ -297,7 +297,7 @@ int tm_rms_norm(const void* x, const void* weight, void* out, int64_t rows, int 
  *
  * What only the device can see is reported through error_flag (optional device
  * int, first writer wins): 11 free pages, table columns, slots, max_kv_len or
- * max_seqlen_q exceeded, or a length negative; 12 a page number outside the pool (its keys are
+ * max_seqlen_q exceeded, a length negative, or offsets that are not rows of q in order; 12 a page number outside the pool (its keys are
  * left out); 13 a slot outside the pool (skipped).
  */
 

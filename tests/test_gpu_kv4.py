@@ -558,3 +558,44 @@ def test_keys_beyond_their_bound_do_not_shift_the_others(cuda_device, more):
         assert _near(got[i:i + 1], ref, bound), i
     ref, bound = ora.attention(rows[5:], keys[1], values[1], 33, 64 ** -0.5, True)
     assert _near(got[5:], ref, bound)
+
+
+@pytest.mark.parametrize("offsets,served", [
+    ([0, 3, 2, 2], [0, 2]),   # the second request's end is in front of its start
+    ([0, 3, 5, 9], [0, 1]),   # the third one's rows run past q
+    ([-1, 1, 3, 5], [1, 2]),  # the first one's begin in front of q
+    ([0, 2, 4, 6], [0, 1, 2]),
+])
+def test_offsets_that_do_not_hold_are_reported(cuda_device, offsets, served):
+    """A request whose rows are not all rows of q is left out, and the error word says so."""
+    from tilemix_b200.attention.kv4 import kv4_attention
+
+    pool, table, lens, keys, values = _cache(cuda_device, [40, 50, 60], 2, 64, 16, seed=23)
+    q, _ = _queries(cuda_device, [6], 4, 64, seed=23)
+    out = torch.full_like(q, 3.0)
+    kv4_attention(q, pool, table, lens, torch.tensor(offsets, dtype=torch.int32, device=cuda_device), 4, out=out)
+    assert _error_code() == (0 if offsets[0] == 0 and offsets[3] == 6 else 11)
+    got, rows = out.double().cpu().numpy(), q.cpu().numpy()
+    free = np.ones(6, dtype=bool)
+    for b in served:
+        at = slice(offsets[b], offsets[b + 1])
+        free[at] = False
+        ref, bound = ora.attention(rows[at], keys[b], values[b], len(keys[b]), 64 ** -0.5, True)
+        assert _near(got[at], ref, bound), b
+    assert (got[free] == 3).all()
+
+
+def test_negative_lengths_are_reported(cuda_device):
+    """A negative length counts as no key: rows of 0, and the error word says 11."""
+    from tilemix_b200.attention.kv4 import kv4_attention
+
+    pool, table, lens, keys, values = _cache(cuda_device, [40, 50], 2, 64, 16, seed=24)
+    q, cu = _queries(cuda_device, [2, 3], 4, 64, seed=24)
+    for wrong in (-1, -2**31):
+        broken = lens.clone()
+        broken[0] = wrong
+        for causal in (True, False):
+            out = kv4_attention(q, pool, table, broken, cu, 3, causal=causal)
+            assert _error_code() == 11 and (out[:2] == 0).all()
+            ref, bound = ora.attention(q[2:].cpu().numpy(), keys[1], values[1], 50, 64 ** -0.5, causal)
+            assert _near(out[2:].double().cpu().numpy(), ref, bound)

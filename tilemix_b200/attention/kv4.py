@@ -218,7 +218,8 @@ def kv4_attention(q: Tensor, pool: Tensor, block_table: Tensor, kv_lens: Tensor,
     [batch, columns], optional) excludes keys for every row of a request; a key behind its last
     column is excluded too. A row that sees no key is 0. ``max_kv_len`` bounds ``kv_lens`` on the
     host (default: the table's capacity). Keys beyond it, or query tokens beyond ``max_seqlen_q``, are
-    left out (``device_error_code`` 11) and move nothing for the others; a small bound makes for a small launch. Rows of ``q`` that belong
+    left out (``device_error_code`` 11) and move nothing for the others; a small bound makes for a small launch.
+    A request whose offsets are not rows of ``q`` in order is left out whole, a negative length counts as 0 (11 too). Rows of ``q`` that belong
     to no request are left as they were in ``out``.
     """
     if not q.is_cuda:

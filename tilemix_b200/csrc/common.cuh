@@ -31,7 +31,7 @@ enum : int {
   kErrTimeoutDrain = 7,     // final drain of in-flight work timed out
   kErrTimeoutQFree = 9,     // Q producer waited too long for the previous work item's last S
   kErrTimeoutOFree = 10,    // MMA warp waited too long for the previous work item's O to be read
-  kErrCachePlan = 11,       // block tables: free pages, table columns or slots run out, or a length is negative
+  kErrCachePlan = 11,       // block tables: free pages, table columns or slots run out; attention: bounds or offsets do not hold; a length is negative
   kErrCachePage = 12,       // a page number outside the pool where a key's page is looked up
   kErrCacheSlot = 13,       // a slot outside the pool
 };

@@ -258,8 +258,10 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
       a.starts[b] = at;
       const Request r = request_of<NT>(a, b);
       at += r.cost;
-      // more keys, or more query tokens, than the call said there may be: those beyond are left out
-      if (r.kv < a.kv_lens[b] || given_queries(a, b) > a.max_q) record_error(a.err, kErrCachePlan);
+      // more keys or query tokens than the call said there may be, offsets that are not rows of q in order, a negative
+      // length: what is beyond is left out
+      if (r.kv != a.kv_lens[b] || r.q0 < 0 || (a.cu != nullptr && a.cu[b + 1] != static_cast<int64_t>(r.q0) + r.n_q))
+        record_error(a.err, kErrCachePlan);
     }
     if (lane == 0) a.starts[a.batch] = total;
   }

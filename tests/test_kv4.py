@@ -266,3 +266,16 @@ def test_the_first_call_cannot_be_captured(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="before the capture"):
         _lib.error_word_ptr(0)
+
+
+def test_token_counts_stay_clear_of_32_bits():
+    """The grid counts 16 tokens a CTA in two of its dimensions, the last rounded up to whole 65,535 CTAs: up to 2^20 tokens
+    more than there are, all of them below 2^31."""
+    from tilemix_b200._lib import lib
+
+    fake = 0x100000
+    for tokens in (2**31 - 17, 2**31 - 2**20):
+        assert lib().tm_kv4_append(fake, 0, 64, fake, 0, 64, tokens, fake, fake, 8, 1, 64, 32, None, None) == -4
+        assert lib().tm_kv4_read(fake, 8, 1, 64, 32, fake, tokens, fake, fake, None, None) == -4
+    groups = (2**31 - 1 - 2**20 + 15) // 16  # of the most tokens that are taken
+    assert -(-groups // 65535) * 65535 * 16 <= 2**31

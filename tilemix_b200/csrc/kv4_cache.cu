@@ -287,11 +287,12 @@ static dim3 grid_of(int64_t groups, int heads) {
   return dim3(static_cast<unsigned>(heads), y, static_cast<unsigned>((groups + y - 1) / y));
 }
 
-// TM_OK and the pool's shape for the kernels, or why not.
+// TM_OK and the pool's shape for the kernels, or why not. The grid's last dimension is rounded up to whole layers of
+// 65,535 CTAs, so a CTA's first token may be up to 2^20 behind the last one and has to stay below 2^31.
 static int pages_of(int64_t n_tokens, int64_t num_pages, int heads, int head_dim, int page_size, Pages* p) {
   const int64_t blocks = page_size / kBlockTokens, bytes = blocks * block_bytes(head_dim);
   if (bytes > 0x7fffffffll || num_pages * blocks > 0x7fffffffll || num_pages * heads > 0x7fffffffll ||
-      (n_tokens + kBlockTokens) * heads > 0x7fffffffll)
+      (n_tokens + kBlockTokens) * heads > 0x7fffffffll || n_tokens > 0x7fffffffll - (1 << 20))
     return TM_ERR_UNSUPPORTED;
   p->heads = static_cast<uint32_t>(heads);
   p->bytes = static_cast<int>(bytes);

@@ -365,7 +365,7 @@ typedef struct tm_kv4_attn_params {
   int batch, heads_q, heads_k, head_dim;
   int max_seqlen_q, max_kv_len; /* host bounds of the query and cache lengths */
   int causal; /* query i of n sees the keys before position kv_len - n + i + 1; else all keys */
-  float sm_scale; /* > 0 */
+  float sm_scale; /* > 0, at most 2^80 */
 } tm_kv4_attn_params;
 
 /* Attention of a few query tokens a request over its cached keys. A row without

@@ -279,3 +279,23 @@ def test_token_counts_stay_clear_of_32_bits():
         assert lib().tm_kv4_read(fake, 8, 1, 64, 32, fake, tokens, fake, fake, None, None) == -4
     groups = (2**31 - 1 - 2**20 + 15) // 16  # of the most tokens that are taken
     assert -(-groups // 65535) * 65535 * 16 <= 2**31
+
+
+def test_scales_whose_scores_leave_fp32_are_refused():
+    """|q . k| is at most 128 * 65504^2 < 2^40: times log2(e) 2^80 every score is finite, times a scale of 2^127 none is."""
+    from tilemix_b200._lib import TmKv4AttnParams, lib
+    from tilemix_b200.attention.kv4 import kv4_attention
+
+    p = TmKv4AttnParams()
+    for name in ("q", "out", "pool", "block_table", "kv_lens"):
+        setattr(p, name, 0x100000)
+    p.q_stride_tok, p.q_stride_head, p.o_stride_tok, p.o_stride_head, p.q_tokens, p.batch = 1024, 128, 1024, 128, 4, 4
+    p.num_pages, p.table_stride, p.cols, p.page_size = 16, 4, 4, 32
+    p.heads_q, p.heads_k, p.head_dim, p.max_seqlen_q, p.max_kv_len = 8, 2, 128, 1, 128
+    need = ctypes.c_int64()
+    for scale, status in ((2.0 ** 80, 0), (2.0 ** 81, -2), (3e38, -2)):
+        p.sm_scale = scale
+        assert lib().tm_kv4_attn_workspace(ctypes.addressof(p), ctypes.byref(need)) == status, scale
+        if status:
+            with pytest.raises(ValueError, match="sm_scale"):
+                kv4_attention(**{name: make() for name, make in ATTN.items()}, out=_Fake((3, 4, 64)), sm_scale=scale)

@@ -33,6 +33,7 @@ __all__ = ["BlockTables", "build_block_tables", "release_pages", "kv4_pool", "kv
            "kv4_attention"]
 
 _HEAD_DIMS = (64, 128)
+_MAX_SCALE = 2.0 ** 80  # every score of fp16 rows stays finite in fp32
 _pack_tables = packer(TmBlockTablesParams)
 _pack_attn = packer(TmKv4AttnParams)
 _launch_tables, _launch_release = launcher("tm_build_block_tables"), launcher("tm_release_pages")
@@ -260,8 +261,8 @@ def kv4_attention(q: Tensor, pool: Tensor, block_table: Tensor, kv_lens: Tensor,
             raise ValueError("out must match q")
         o_tok, o_head, _ = out.stride()
     scale = d ** -0.5 if sm_scale is None else float(sm_scale)
-    if not 0 < scale < float("inf"):
-        raise ValueError("sm_scale must be positive and finite")
+    if not 0 < scale <= _MAX_SCALE:
+        raise ValueError("sm_scale must be positive and at most 2^80")
     capacity = cols * page_size
     bound = capacity if max_kv_len is None else min(max(int(max_kv_len), 0), capacity)
     mask = (0, 0, 0) if key_mask is None else (key_mask.data_ptr(), key_mask.stride(0), key_mask.shape[1])

@@ -877,7 +877,8 @@ static int check(const tm_kv4_attn_params* p) {
   if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->pool, 16)) return TM_ERR_ALIGN;
   if (p->q_stride_tok % 8 || p->q_stride_head % 8 || p->o_stride_tok % 8 || p->o_stride_head % 8) return TM_ERR_ALIGN;
   if (p->key_mask != nullptr && p->mask_cols < 0) return TM_ERR_SHAPE;
-  if (!(p->sm_scale > 0.f) || p->sm_scale > 3.4028235e38f) return TM_ERR_SHAPE;  // maxima are taken before scaling
+  // Positive: maxima are taken before scaling. At most 2^80: |q . k| < 2^40, so a score in log2 units stays finite.
+  if (!(p->sm_scale > 0.f) || p->sm_scale > 1.2089258e24f) return TM_ERR_SHAPE;
   // the chunks of the work list are counted in 32 bits, with room for the last CTA's end
   const double rows = static_cast<double>(p->max_seqlen_q) * p->heads_q;
   if (p->batch * (rows / 8 + p->heads_k) * (p->max_kv_len / kChunkKeys + 1.0 + kSetup) > 2147480000.0)

@@ -79,3 +79,19 @@ def test_qwen_inject_and_map_fixup():
     # every row holding only its highest group widens to all groups
     pm = torch.tensor([0x80, 0x80], dtype=torch.int64).view(torch.uint64)
     assert attn._fixup_precision_map(pm, 512, 64).view(torch.int64).tolist() == [0xFF, 0xFF]
+
+
+@pytest.mark.parametrize("dtype", [torch.bool, torch.int64, torch.float32, torch.float16])
+def test_key_mask_of_the_cache_attention(dtype):
+    """A padding mask [B, keys] keeps a key with 1 in any type; a mask [B, 1, queries, keys] keeps it with True or, as an
+    additive one, with 0, and the last query token's row counts."""
+    from tilemix_b200.models._attention_base import _key_mask
+
+    keep = torch.tensor([[False, True, True], [True, True, True], [False, False, True]])
+    assert _key_mask(None) is None
+    assert torch.equal(_key_mask(keep.to(dtype)), keep)
+    causal = torch.ones(3, 3, dtype=torch.bool).tril()
+    full = (keep[:, None] & causal)[:, None]
+    if dtype.is_floating_point:
+        full = torch.where(full, 0.0, torch.finfo(dtype).min).to(dtype)
+    assert torch.equal(_key_mask(full.to(dtype)), keep)

@@ -203,12 +203,16 @@ class TileMixAttentionMixin:
 
 
 def _key_mask(attention_mask) -> Optional[Tensor]:
-    """Keys that a batch's padding leaves, bool [B, keys], from the mask that HF hands to its attention: that of
-    the last query token, which no causal entry hides a key from."""
+    """Keys that a batch's padding leaves, bool [B, keys], from the mask that HF hands to its attention: a padding mask
+    [B, keys], or the last query token's row of a full one, from which no causal entry hides a key. A full mask of
+    floating type is additive: 0 keeps a key."""
     if attention_mask is None:
         return None
-    mask = attention_mask if attention_mask.ndim == 2 else attention_mask[:, 0, -1]
-    return (mask if mask.dtype == torch.bool else mask == 0 if mask.is_floating_point() else mask != 0).contiguous()
+    full = attention_mask.ndim > 2
+    mask = attention_mask[:, 0, -1] if full else attention_mask
+    if mask.dtype != torch.bool:
+        mask = mask == 0 if full and mask.is_floating_point() else mask != 0
+    return mask.contiguous()
 
 
 def copy_attention_weights(orig, new) -> None:

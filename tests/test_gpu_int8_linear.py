@@ -251,3 +251,16 @@ def test_on_another_stream_and_in_graphs(cuda_device):
                 graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[i]) and torch.equal(outs[1], want[i + 1])
+
+
+@pytest.mark.parametrize("m,n", [(1, 40), (5, 1), (1, 1)])
+@pytest.mark.parametrize("k", [100, 33, 4000])
+def test_single_rows_need_no_padding(cuda_device, m, n, k):
+    """The stride of a single row is never used: a contiguous one of any length is as good as a padded one."""
+    from tilemix_b200.linear.int8_linear import int8_matmul
+
+    x8, xs, w8, ws = _operands(cuda_device, m, n, k, seed=k)
+    a, b = (t if t.shape[0] > 1 else t[0].clone()[None] for t in (x8, w8))
+    assert m > 1 or a.stride(0) == k
+    assert n > 1 or b.stride(0) == k
+    _check(int8_matmul(a, xs, b, ws), x8, xs, w8, ws)

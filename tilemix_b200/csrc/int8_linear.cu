@@ -1076,15 +1076,13 @@ static int matmul(const int8_t* x8, int64_t x_stride, const float* x_scale, cons
   if (tokens == 0) return TM_OK;
   if (!x8 || !x_scale || !w8 || !w_scale || !out) return TM_ERR_NULL;
   const int es = out_dtype == TM_DTYPE_FP32 ? 4 : 2;
+  const int64_t round_k = (static_cast<int64_t>(in_features) + 15) / 16 * 16;
+  if (tokens == 1) x_stride = round_k;  // one row: its stride is never used, but has to suit the tensor map
+  if (out_features == 1) w_stride = round_k;
   if (!aligned(x8, 16) || !aligned(w8, 16) || x_stride % 16 || w_stride % 16) return TM_ERR_ALIGN;
   if (!aligned(out, es) || !aligned(x_scale, 4) || !aligned(w_scale, 4) || (bias && !aligned(bias, es)))
     return TM_ERR_ALIGN;
-  if (x_stride < 0 || w_stride < 0 || (tokens > 1 && x_stride < in_features) ||
-      (out_features > 1 && w_stride < in_features))
-    return TM_ERR_SHAPE;
-  const int64_t round_k = (static_cast<int64_t>(in_features) + 15) / 16 * 16;
-  if (tokens == 1 && x_stride < round_k) x_stride = round_k;  // one row: its stride is never used
-  if (out_features == 1 && w_stride < round_k) w_stride = round_k;
+  if (x_stride < in_features || w_stride < in_features) return TM_ERR_SHAPE;
   const int k_tiles = (in_features + kBK - 1) / kBK;
   const Plan p = plan_of(tokens, out_features, k_tiles);
   GemmArgs g{};

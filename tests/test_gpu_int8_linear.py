@@ -264,3 +264,26 @@ def test_single_rows_need_no_padding(cuda_device, m, n, k):
     assert m > 1 or a.stride(0) == k
     assert n > 1 or b.stride(0) == k
     _check(int8_matmul(a, xs, b, ws), x8, xs, w8, ws)
+
+
+def test_a_layer_keeps_its_scales_through_conversions(cuda_device):
+    """half(), bfloat16() and moves change the type of the activations and of the bias; codes and scales stay as they are."""
+    from tilemix_b200.linear.int8_linear import Int8Linear, int8_linear
+
+    torch.manual_seed(0)
+    layer = Int8Linear(torch.nn.Linear(200, 72).to(cuda_device, torch.float16))
+    codes, scale, bias = layer.codes.clone(), layer.weight_scale.clone(), layer.bias.clone()
+    x = torch.randn((6, 200), generator=torch.Generator().manual_seed(1)).to(cuda_device)
+    for convert, dtype in ((lambda m: m.half(), torch.float16), (lambda m: m.to(torch.bfloat16), torch.bfloat16),
+                           (lambda m: m.cpu().to(cuda_device), torch.bfloat16)):
+        layer = convert(layer)
+        assert torch.equal(layer.codes, codes) and torch.equal(layer.weight_scale, scale)
+        assert layer.dtype == layer.bias.dtype == dtype
+        want = int8_linear(x.to(dtype), codes[:, :200], scale, bias.to(dtype))
+        assert torch.equal(layer(x.to(dtype)), want)
+    with pytest.raises(TypeError):
+        layer(x.half())
+    layer = layer.float()
+    assert torch.equal(layer.weight_scale, scale)
+    with pytest.raises(TypeError):
+        layer(x)

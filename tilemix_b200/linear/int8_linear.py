@@ -138,7 +138,8 @@ def int8_linear(x: Tensor, w8: Tensor, w_scale: Tensor, bias: Optional[Tensor] =
 
 class Int8Linear(nn.Module):
     """``nn.Linear`` for inference with the weight in 8 bits, one scale for each output feature. The
-    codes are laid out once, rows on 16 bytes (buffer ``codes``); ``weight`` is their view."""
+    codes are laid out once, rows on 16 bytes (buffer ``codes``); ``weight`` is their view. ``half()``,
+    ``bfloat16()`` and ``to(dtype)`` change the activations' type and the bias; the scales stay fp32."""
 
     def __init__(self, linear: nn.Linear):
         super().__init__()
@@ -158,9 +159,17 @@ class Int8Linear(nn.Module):
         """The codes, int8 [out_features, in_features]."""
         return self.codes[:, :self.in_features]
 
+    def _apply(self, fn, recurse=True):
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != scale.dtype:
+            self.weight_scale = scale.to(self.weight_scale.device)
+        self.dtype = fn(torch.empty(0, dtype=self.dtype, device=scale.device)).dtype
+        return self
+
     def forward(self, x: Tensor) -> Tensor:
         if x.dtype != self.dtype:
-            raise TypeError(f"the layer was quantised for {self.dtype} activations, got {x.dtype}")
+            raise TypeError(f"the layer takes {self.dtype} activations, got {x.dtype}")
         return int8_linear(x, self.weight, self.weight_scale, self.bias)
 
     def extra_repr(self) -> str:

@@ -287,3 +287,20 @@ def test_a_layer_keeps_its_scales_through_conversions(cuda_device):
     assert torch.equal(layer.weight_scale, scale)
     with pytest.raises(TypeError):
         layer(x)
+
+
+def test_a_layer_made_in_inference_mode(cuda_device):
+    """Its codes are laid out as those of any other layer: rows on 16 bytes, also after a move."""
+    from tilemix_b200.linear.int8_linear import Int8Linear
+
+    torch.manual_seed(0)
+    linear = torch.nn.Linear(200, 72).to(cuda_device, torch.float16)
+    x = torch.randn((3, 200), generator=torch.Generator().manual_seed(1)).half().to(cuda_device)
+    with torch.inference_mode():
+        layer = Int8Linear(linear)
+        assert layer.codes.shape == (72, 208)
+        want = layer(x)
+        assert torch.equal(layer.cpu().to(cuda_device)(x), want)
+    other = Int8Linear(linear)
+    other.load_state_dict(layer.state_dict())
+    assert torch.equal(other(x), want)

@@ -31,6 +31,12 @@ _launch_linear = launcher("tm_int8_linear")
 def quantize_per_token_int8(x: Tensor) -> tuple[Tensor, Tensor]:
     """Codes int8 [rows, cols] and scales fp32 [rows] of fp16 or bf16 ``x`` [rows, cols] (columns
     contiguous). A row of zeros has scale 0; a row with an infinity or a NaN has that scale."""
+    codes, scale = _quantise(x)
+    return (codes if codes.shape[1] == x.shape[1] else codes[:, :x.shape[1]]), scale
+
+
+def _quantise(x: Tensor) -> tuple[Tensor, Tensor]:
+    """:func:`quantize_per_token_int8` with the codes' rows as they are laid out, whole 16 bytes wide."""
     if not x.is_cuda:
         raise RuntimeError("the quantiser is a CUDA kernel")
     if x.ndim != 2 or x.shape[1] == 0:
@@ -44,7 +50,7 @@ def quantize_per_token_int8(x: Tensor) -> tuple[Tensor, Tensor]:
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     _launch_quant(x.get_device(), x.data_ptr(), _DTYPES[x.dtype], x.stride(0), rows, cols,
                   codes.data_ptr(), codes.stride(0), scale.data_ptr())
-    return (codes if codes.shape[1] == cols else codes[:, :cols]), scale
+    return codes, scale
 
 
 def _check_weight(w8: Tensor, w_scale: Tensor, in_features: int, index: int) -> None:
@@ -148,8 +154,8 @@ class Int8Linear(nn.Module):
         self.in_features, self.out_features = linear.in_features, linear.out_features
         self.dtype = linear.weight.dtype
         with torch.no_grad():
-            codes, scale = quantize_per_token_int8(linear.weight.detach().contiguous())
-        self.register_buffer("codes", codes if codes._base is None else codes._base)
+            codes, scale = _quantise(linear.weight.detach().contiguous())
+        self.register_buffer("codes", codes)
         self.register_buffer("weight_scale", scale)
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
         self.train(linear.training)

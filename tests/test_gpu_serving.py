@@ -218,3 +218,15 @@ def test_the_whole_path_together(cuda_device, kind):
                 assert _rel(logits[-1], ref.logits[:, -1]) < 0.3
         outs.append(torch.cat(logits))
     assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("kind", ["llama", "qwen"])
+def test_attention_is_injected_before_the_projections_are_quantised(cuda_device, kind):
+    """The other way round is refused and leaves the model as it was: the weights to copy are no longer there."""
+    from tilemix_b200.models.int8_projections import quantize_projections_int8
+
+    model = quantize_projections_int8(_model(cuda_device, kind))
+    before = [layer.self_attn for layer in model.model.layers]
+    with pytest.raises(ValueError, match="inject TileMix attention before"):
+        _inject(model, kind)
+    assert all(layer.self_attn is a for layer, a in zip(model.model.layers, before))

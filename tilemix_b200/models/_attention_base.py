@@ -18,6 +18,7 @@ from torch import Tensor
 
 from tilemix_b200.attention.precision_maps import BLOCK_PERCENTAGE_PATTERNS, make_precision_bitmask
 from tilemix_b200.attention.tilemix_varlen import tilemix_varlen_attention
+from tilemix_b200.linear.int8_linear import Int8Linear
 from tilemix_b200.models.kv4_cache import Kv4Cache
 
 
@@ -226,6 +227,8 @@ def copy_attention_weights(orig, new) -> None:
 
 def replace_attention(model, make_attention) -> None:
     root = model.model if hasattr(model, "model") else model
+    if any(isinstance(m, Int8Linear) for layer in root.layers for m in layer.self_attn.children()):
+        raise ValueError("inject TileMix attention before the projections are quantised (quantize_projections_int8)")
     for layer in root.layers:
         orig = layer.self_attn
         new_attn = make_attention(orig.config, orig.layer_idx)

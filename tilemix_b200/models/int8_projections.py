@@ -13,8 +13,8 @@ _PROJECTIONS = (("self_attn", ("q_proj", "k_proj", "v_proj", "o_proj")), ("mlp",
 def quantize_projections_int8(model):
     """Replace the seven projections of every decoder layer by :class:`Int8Linear` (weights in 8 bits with
     a scale for each output feature, activations quantised by token), in place. fp16 or bf16 models,
-    plain, TileMix-injected or prepared for prefill (``prepare_llama_prefill`` comes first: it wants
-    fp16 weights); embeddings, norms and the LM head stay as they are. Returns the model."""
+    plain, TileMix-injected or prepared for prefill (injection and ``prepare_llama_prefill`` come first:
+    they want fp16 weights); embeddings, norms and the LM head stay as they are. Returns the model."""
     root = model.model if hasattr(model, "model") else model
     found = []
     for layer in root.layers:

@@ -230,3 +230,17 @@ def test_attention_is_injected_before_the_projections_are_quantised(cuda_device,
     with pytest.raises(ValueError, match="inject TileMix attention before"):
         _inject(model, kind)
     assert all(layer.self_attn is a for layer, a in zip(model.model.layers, before))
+
+
+def test_a_cache_filled_in_inference_mode_is_reset_outside_it(cuda_device):
+    from tilemix_b200.models.kv4_cache import Kv4Cache
+
+    model = _inject(_model(cuda_device))
+    cache, ids = Kv4Cache(64, page_size=16), _ids(cuda_device, 2, 20, seed=3)
+    with torch.inference_mode():
+        first = model(ids, past_key_values=cache, use_cache=True).logits
+        model(ids[:, :2], past_key_values=cache, use_cache=True)
+    cache.reset()
+    with torch.no_grad():
+        again = model(ids, past_key_values=cache, use_cache=True).logits
+    assert torch.equal(first, again)

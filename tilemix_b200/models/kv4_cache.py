@@ -149,6 +149,7 @@ class Kv4Cache(Cache):
             self._free_all()
 
     # -- pages
+    @torch.inference_mode()  # where tensors that were made in it, by a step, may be changed in place
     def _free_all(self) -> None:
         self.table.fill_(-1)
         self.lens.zero_()

@@ -304,3 +304,56 @@ def test_a_layer_made_in_inference_mode(cuda_device):
     other = Int8Linear(linear)
     other.load_state_dict(layer.state_dict())
     assert torch.equal(other(x), want)
+
+
+# Sizes that reach every form of the product: weights on the lanes with 16, 32 and 64 tokens a tile, tokens on the lanes with
+# 64, 128 and 256 channels, pairs of SMs with 128 to 256 channels, K whole and in 2, 4 and 8 parts; many tiles a CTA
+# and more steps than the ring has stages.
+FORMS = [(2, 4162, 2216), (13, 3253, 1974), (5, 2110, 4506), (3, 45001, 1111), (28, 38, 1832), (30, 2054, 4667),
+         (20, 45001, 1111), (49, 11854, 3358), (43, 7067, 11986), (60, 3584, 18944), (42, 1030, 8102), (50, 45001, 1011),
+         (131, 10668, 104), (302, 1435, 3385), (278, 655, 3194), (367, 2498, 9553), (37, 43396, 641), (263, 31780, 132),
+         (1813, 7269, 530), (246, 8453, 13615), (4182, 2147, 1078), (700, 7755, 2841), (4155, 2066, 1100),
+         (1435, 6284, 782), (3935, 2516, 780), (777, 4608, 3584), (3336, 3455, 822)]
+
+
+@pytest.mark.parametrize("m,n,k", FORMS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_every_form_matches_exact_sums(cuda_device, m, n, k, dtype):
+    from tilemix_b200.linear.int8_linear import int8_matmul
+
+    x8, xs, w8, ws = _operands(cuda_device, m, n, k, seed=m + n + k)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(1)).to(cuda_device, dtype)
+    out = int8_matmul(x8, xs, w8, ws, bias, out_dtype=dtype)
+    _check(out, x8, xs, w8, ws, bias)
+    for _ in range(3):
+        assert torch.equal(int8_matmul(x8, xs, w8, ws, bias, out_dtype=dtype), out)
+
+
+@pytest.mark.parametrize("m,n,k", [(3935, 2516, 780), (2000, 3000, 18944)])
+def test_a_token_does_not_depend_on_its_batch_in_the_large_forms(cuda_device, m, n, k):
+    from tilemix_b200.linear.int8_linear import int8_matmul
+
+    x8, xs, w8, ws = _operands(cuda_device, m, n, k, seed=5)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(2)).to(cuda_device, torch.bfloat16)
+    full = int8_matmul(x8, xs, w8, ws, bias, out_dtype=torch.bfloat16)
+    for part in (3, 30, 50, 90, 200, 600, 777, 1500, m - 1):
+        assert torch.equal(int8_matmul(x8[:part], xs[:part], w8, ws, bias, out_dtype=torch.bfloat16), full[:part]), part
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("offset", [0, 3, 8])
+@pytest.mark.parametrize("m,k", [(148, 2056), (160, 4096), (149, 8200), (151, 12288), (148, 16400), (150, 24576)])
+def test_quantiser_of_many_wide_rows(cuda_device, m, k, offset, dtype):
+    """Rows on 16 bytes, and views that start elsewhere."""
+    from tilemix_b200.linear.int8_linear import quantize_per_token_int8
+
+    x = torch.nn.functional.pad(_rows(m, k, m + k, dtype), (offset, 8 - offset)).to(cuda_device)[:, offset:offset + k]
+    ref, ref_scale = _codes_of(x)
+    x[5, k // 2], x[6, k - 1] = float("nan"), float("-inf")
+    ref[5:7] = 0
+    codes, scale = quantize_per_token_int8(x)
+    assert np.array_equal(codes.cpu().numpy(), ref)
+    scale = scale.double().cpu().numpy()
+    assert np.isnan(scale[5]) and np.isposinf(scale[6])
+    fine = np.delete(np.arange(m), [5, 6])
+    assert (np.abs(scale - ref_scale)[fine] <= ref_scale[fine] * 2.0 ** -24).all()

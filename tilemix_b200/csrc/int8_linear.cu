@@ -237,6 +237,7 @@ static void launch_quant(const void* x, int64_t xs, int64_t rows, int cols, int8
 constexpr int kBM = 128, kBK = 128;
 constexpr int kGemmThreads = 256;
 constexpr int kMaxSplit = 8;
+constexpr int kMaxSplitBN = 128;  // widest tile whose K is cut
 constexpr int kSms = 148;
 
 struct GemmArgs {
@@ -304,6 +305,7 @@ struct GemmShape {
   static constexpr int kOffPieces = kOffCols + 2 * 2 * BN * 4;
   static constexpr int smem(bool token_lanes) { return kOffPieces + (token_lanes ? 4 * 4096 : 0) + 1024; }
   static constexpr int kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
+  static constexpr bool kSplits = BN <= kMaxSplitBN;
 };
 
 // y = sum * token scale * channel scale + bias, the token's scale first on either side, so that every launch
@@ -619,7 +621,7 @@ __global__ void __launch_bounds__(kGemmThreads) gemm_kernel(const __grid_constan
       if (!ok) continue;
       tc_fence_after();
       const uint32_t d = tmem + acc * BN + (static_cast<uint32_t>(quad * 32) << 16);
-      if (g.split == 1) {
+      if (!S::kSplits || g.split == 1) {
         if constexpr (kTokenLanes) {
           constexpr int kCols = 128 / sizeof(OutT);
 #pragma unroll 1
@@ -634,7 +636,7 @@ __global__ void __launch_bounds__(kGemmThreads) gemm_kernel(const __grid_constan
             emit<16, kTokenLanes, OutT>(r, g, a, tb * BN + c, row_scale, row_bias, col_scale + c, col_bias + c);
           }
         }
-      } else {
+      } else if constexpr (S::kSplits) {
         // this part's partial tile, column by column (a warp's 32 lanes are 128 consecutive bytes); every
         // copy has landed and every product has read its stage, so the ring is free
         int32_t* red = reinterpret_cast<int32_t*>(smem) + quad * 32 + lane;
@@ -653,29 +655,31 @@ __global__ void __launch_bounds__(kGemmThreads) gemm_kernel(const __grid_constan
     }
   }
 
-  if (g.split > 1) {  // a cluster has one tile; the barriers are reached whatever happened above
-    __syncwarp();
-    cluster_sync();
-    if (warp >= 4 && ok) {
-      int ta, tb;
-      tile_at(first_tile, &ta, &tb);
-      const int row = (warp & 3) * 32 + lane;
-      const uint32_t red = smem_u32(smem) + row * 4;
-      const float* col_scale = reinterpret_cast<const float*>(smem + S::kOffCols);
-      auto reduce = [&](auto parts) {
-        reduce_split<decltype(parts)::value, BN, kTokenLanes, OutT>(
-            red, smem + S::kOffPieces + (warp & 3) * 4096, g, ta * kBM + (warp & 3) * 32, tb * BN, rank, row_scale,
-            row_bias, col_scale, col_scale + BN);
-      };
-      if (g.split == 2)
-        reduce(std::integral_constant<int, 2>{});
-      else if (g.split == 4)
-        reduce(std::integral_constant<int, 4>{});
-      else
-        reduce(std::integral_constant<int, 8>{});
+  if constexpr (S::kSplits) {
+    if (g.split > 1) {  // a cluster has one tile; the barriers are reached whatever happened above
+      __syncwarp();
+      cluster_sync();
+      if (warp >= 4 && ok) {
+        int ta, tb;
+        tile_at(first_tile, &ta, &tb);
+        const int row = (warp & 3) * 32 + lane;
+        const uint32_t red = smem_u32(smem) + row * 4;
+        const float* col_scale = reinterpret_cast<const float*>(smem + S::kOffCols);
+        auto reduce = [&](auto parts) {
+          reduce_split<decltype(parts)::value, BN, kTokenLanes, OutT>(
+              red, smem + S::kOffPieces + (warp & 3) * 4096, g, ta * kBM + (warp & 3) * 32, tb * BN, rank, row_scale,
+              row_bias, col_scale, col_scale + BN);
+        };
+        if (g.split == 2)
+          reduce(std::integral_constant<int, 2>{});
+        else if (g.split == 4)
+          reduce(std::integral_constant<int, 4>{});
+        else
+          reduce(std::integral_constant<int, 8>{});
+      }
+      __syncwarp();
+      cluster_sync();  // nobody leaves while its partial tile is read
     }
-    __syncwarp();
-    cluster_sync();  // nobody leaves while its partial tile is read
   }
   tc_fence_before();
   __syncthreads();
@@ -940,7 +944,8 @@ static Plan plan_of(int64_t m, int n, int k_tiles) {
     for (int split = 1; split <= kMaxSplit; split *= 2) {
       // A part has work, and all clusters are resident at once: a GPC has room for whole ones only, so clusters of
       // four and eight do not reach every SM (36 tiles of 4 parts took two waves, 21 us instead of 11).
-      if (split > 1 && (k_tiles / split < 4 || tiles * split > (split == 2 ? kSms : 128) || bn > 128 || bn < 2 * split))
+      if (split > 1 && (k_tiles / split < 4 || tiles * split > (split == 2 ? kSms : 128) || bn > kMaxSplitBN ||
+                        bn < 2 * split))
         break;
       const double step = most(2 * bn, 2050. / stages, 2 * (kBM + bn) * busy(tiles * split));
       const double out = (!token_lanes ? 60. : split == 1 ? 8. : 20.) * bn / split + (split > 1 ? 2500 : 0);
@@ -953,8 +958,6 @@ static Plan plan_of(int64_t m, int n, int k_tiles) {
     one_cta(false, 32, GemmShape<32>::kStages);
   else if (m <= 64)
     one_cta(false, 64, GemmShape<64>::kStages);
-  else if (m <= 128)
-    one_cta(false, 128, GemmShape<128>::kStages);
   if (m > 32) {
     one_cta(true, 64, GemmShape<64>::kStages);
     one_cta(true, 128, GemmShape<128>::kStages);
@@ -1037,7 +1040,6 @@ static int dispatch(const Plan& p, const CUtensorMap& a, const CUtensorMap& b, c
     if (p.bn == 128) return launch<128, true, OutT>(a, b, g, st);
     return launch<64, true, OutT>(a, b, g, st);
   }
-  if (p.bn == 128) return launch<128, false, OutT>(a, b, g, st);
   if (p.bn == 64) return launch<64, false, OutT>(a, b, g, st);
   if (p.bn == 32) return launch<32, false, OutT>(a, b, g, st);
   return launch<16, false, OutT>(a, b, g, st);

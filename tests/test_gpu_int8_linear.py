@@ -357,3 +357,22 @@ def test_quantiser_of_many_wide_rows(cuda_device, m, k, offset, dtype):
     assert np.isnan(scale[5]) and np.isposinf(scale[6])
     fine = np.delete(np.arange(m), [5, 6])
     assert (np.abs(scale - ref_scale)[fine] <= ref_scale[fine] * 2.0 ** -24).all()
+
+
+def test_more_than_32_bits_of_elements(cuda_device):
+    """Inputs and outputs of over 2^31 elements: the last rows are those of a small call."""
+    from tilemix_b200.linear.int8_linear import int8_matmul, quantize_per_token_int8
+
+    m, n, k = 70001, 40008, 96
+    x8, xs, w8, ws = _operands(cuda_device, m, n, k, seed=3)
+    out = int8_matmul(x8, xs, w8, ws)
+    assert out.numel() > 2**31
+    for rows in (slice(0, 40), slice(2**31 // n - 20, 2**31 // n + 20), slice(m - 40, m)):
+        assert torch.equal(out[rows], int8_matmul(x8[rows], xs[rows], w8, ws))
+    codes, scale = quantize_per_token_int8(out)
+    odd, odd_scale = quantize_per_token_int8(out[:, :8001])
+    for rows in (slice(0, 40), slice(2**31 // n - 20, 2**31 // n + 20), slice(m - 40, m)):
+        few, few_scale = quantize_per_token_int8(out[rows])
+        assert torch.equal(codes[rows], few) and torch.equal(scale[rows], few_scale)
+        few, few_scale = quantize_per_token_int8(out[rows, :8001])
+        assert torch.equal(odd[rows], few) and torch.equal(odd_scale[rows], few_scale)

@@ -205,6 +205,33 @@ def test_attention_of_many_tokens_over_a_filled_cache(cuda_device):
     _check_attention(cuda_device, [2100, 1300], [65, 129], 8, 2, 128, 32, seed=10, masked=True)
 
 
+@pytest.mark.parametrize("heads,dim,page", [(8, 128, 64), (3, 64, 48)])
+def test_a_pool_beyond_32_bits(cuda_device, heads, dim, page):
+    """Slots whose bytes lie more than 2^32 into the pool, and in front of that."""
+    from tilemix_b200.attention.kv4 import kv4_append, kv4_attention, kv4_read
+
+    row = page // 16 * 20 * dim
+    pages = (2**32 + 2**29) // (heads * row)
+    pool = torch.empty((pages, heads, row), dtype=torch.uint8, device=cuda_device)
+    edge = 2**32 // (heads * row)  # the page that holds byte 2^32
+    table = torch.tensor([[pages - 1, 0, edge, edge + 1], [edge - 1, pages - 2, 2**31 // (heads * row), 7]],
+                         dtype=torch.int32, device=cuda_device)
+    n = 4 * page - 5
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    slots = torch.cat([_slots(table[b], torch.arange(n, device=cuda_device), page) for b in range(2)])
+    k, v = (torch.randn((2 * n, heads, dim), generator=g, device=cuda_device).half() for _ in range(2))
+    kv4_append(k, v, pool, slots)
+    got = kv4_read(pool, slots, dim)
+    small = torch.empty((8, heads, row), dtype=torch.uint8, device=cuda_device)
+    few = torch.arange(8, dtype=torch.int32, device=cuda_device).view(2, 4)
+    near = torch.cat([_slots(few[b], torch.arange(n, device=cuda_device), page) for b in range(2)])
+    kv4_append(k, v, small, near)
+    assert all(torch.equal(a, b) for a, b in zip(got, kv4_read(small, near, dim)))
+    q = torch.randn((2, heads * 2, dim), generator=g, device=cuda_device).half()
+    lens = torch.full((2,), n, dtype=torch.int32, device=cuda_device)
+    assert torch.equal(kv4_attention(q, pool, table, lens), kv4_attention(q, small, few, lens))
+
+
 # ---------------------------------------------------------------------------------------------- block tables
 def _tables_case(cached, new, page, seed, extra_pages=5):
     rng = np.random.default_rng(seed)
@@ -297,3 +324,35 @@ def test_tables_into_memory_that_is_not_on_16_bytes(cuda_device):
         got = got.cpu().numpy()
         assert np.array_equal(got[1:-1], want) and got[0] == got[-1] == 77
     assert np.array_equal(after.cpu().numpy(), ref[4]) and np.array_equal(table.cpu().numpy(), ref[5])
+
+
+def test_release_of_many_long_requests(cuda_device):
+    from tilemix_b200.attention.kv4 import release_pages
+
+    page, batch = 16, 700
+    rng = np.random.default_rng(11)
+    lens = rng.integers(0, 5000, batch)
+    lens[5], lens[600] = 131072, 0
+    held = -(-lens // page)
+    free, capacity = 1000, int(held.sum()) + 1000
+    order = rng.permutation(capacity).astype(np.int32)
+    table = np.full((batch, int(held.max()) + 1), -1, dtype=np.int32)
+    at = free
+    for b, n in enumerate(held):
+        table[b, :n] = order[at:at + n]
+        at += n
+    done = rng.random(batch) < 0.5
+    done[5] = True
+    head = 3 * capacity - 500  # the free entries wrap, and so do those that come back
+    ring = np.full(capacity, -7, dtype=np.int32)
+    ring[(head + np.arange(free)) % capacity] = order[:free]
+    to = lambda x, t: torch.tensor(x, dtype=t, device=cuda_device)  # noqa: E731
+    args = [to(lens, torch.int32), to(done, torch.bool), to(table, torch.int32), to(ring, torch.int32),
+            to([head, head + free], torch.int64)]
+    release_pages(*args, page_size=page)
+    back = np.concatenate([table[b, :held[b]] for b in range(batch) if done[b]])
+    ring[(head + free + np.arange(len(back))) % capacity] = back
+    table[done] = -1
+    lens[done] = 0
+    for got, want in zip(args, (lens, done, table, ring, [head, head + free + len(back)])):
+        assert np.array_equal(got.cpu().numpy(), want)

@@ -599,3 +599,32 @@ def test_negative_lengths_are_reported(cuda_device):
             assert _error_code() == 11 and (out[:2] == 0).all()
             ref, bound = ora.attention(q[2:].cpu().numpy(), keys[1], values[1], 50, 64 ** -0.5, causal)
             assert _near(out[2:].double().cpu().numpy(), ref, bound)
+
+
+@pytest.mark.parametrize("heads,dim", [(1, 64), (2, 128)])
+def test_strides_that_are_not_used_may_be_any(cuda_device, heads, dim):
+    """One token, or one head: its row starts on 16 bytes whatever the stride to the next one would be."""
+    from tilemix_b200.attention.kv4 import kv4_append, kv4_attention, kv4_pool, kv4_read
+
+    g = torch.Generator().manual_seed(4)
+    wide = torch.randn((2, 3 * heads * dim + 4), generator=g).half().to(cuda_device)
+    one = wide.as_strided((1, heads, dim), (3 * heads * dim + 4, dim, 1))
+    pool, table = kv4_pool(2, 16, heads, dim, cuda_device), torch.zeros((1, 1), dtype=torch.int32, device=cuda_device)
+    kv4_append(one, one, pool, torch.tensor([0], device=cuda_device))
+    k, v = kv4_read(pool, torch.tensor([0], device=cuda_device), dim)
+    ref = np.zeros(pool.shape, dtype=np.uint8)
+    ora.append(ref, one.cpu().numpy(), one.cpu().numpy(), [0])
+    assert np.array_equal(pool.cpu().numpy(), ref)
+    out = torch.empty_like(wide).as_strided((1, heads, dim), (3 * heads * dim + 4, dim, 1))
+    kv4_attention(one, pool, table, torch.tensor([1], dtype=torch.int32, device=cuda_device), out=out)
+    assert torch.equal(out, v)  # a single key: its value
+    rows = torch.randn((5, dim), generator=g).half().to(cuda_device)
+    single = rows.as_strided((5, 1, dim), (dim, 3, 1))
+    pool = kv4_pool(1, 16, 1, dim, cuda_device)
+    kv4_append(single, single, pool, torch.arange(5, device=cuda_device))
+    k, v = kv4_read(pool, torch.arange(5, device=cuda_device), dim)
+    ref = np.zeros(pool.shape, dtype=np.uint8)
+    ora.append(ref, rows[:, None].cpu().numpy(), rows[:, None].cpu().numpy(), range(5))
+    assert np.array_equal(pool.cpu().numpy(), ref)
+    out = kv4_attention(single, pool, table.expand(5, 1), torch.ones(5, dtype=torch.int32, device=cuda_device))
+    assert torch.equal(out, v[:1].expand(5, 1, dim))

@@ -875,7 +875,9 @@ static int check(const tm_kv4_attn_params* p) {
     return TM_ERR_NULL;
   if (p->cu_seqlens_q == nullptr && (p->max_seqlen_q != 1 || p->q_tokens < p->batch)) return TM_ERR_SHAPE;
   if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->pool, 16)) return TM_ERR_ALIGN;
-  if (p->q_stride_tok % 8 || p->q_stride_head % 8 || p->o_stride_tok % 8 || p->o_stride_head % 8) return TM_ERR_ALIGN;
+  // of one token or head the stride to the next is never used
+  if (p->q_tokens > 1 && (p->q_stride_tok % 8 || p->o_stride_tok % 8)) return TM_ERR_ALIGN;
+  if (p->heads_q > 1 && (p->q_stride_head % 8 || p->o_stride_head % 8)) return TM_ERR_ALIGN;
   if (p->key_mask != nullptr && p->mask_cols < 0) return TM_ERR_SHAPE;
   // Positive: maxima are taken before scaling. At most 2^80: |q . k| < 2^40, so a score in log2 units stays finite.
   if (!(p->sm_scale > 0.f) || p->sm_scale > 1.2089258e24f) return TM_ERR_SHAPE;

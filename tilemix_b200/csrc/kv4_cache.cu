@@ -317,7 +317,10 @@ extern "C" int tm_kv4_append(const void* k, int64_t k_stride_tok, int64_t k_stri
   if (!k || !v || !slots || (num_pages > 0 && !pool)) return TM_ERR_NULL;
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(pool, 16) || !aligned(slots, 8)) return TM_ERR_ALIGN;
   AppendArgs a{};
-  const int64_t strides[4] = {k_stride_tok, k_stride_head, v_stride_tok, v_stride_head};
+  // of one token or head the stride to the next is never used
+  const bool toks = n_tokens > 1, hs = heads > 1;
+  const int64_t strides[4] = {toks ? k_stride_tok : 0, hs ? k_stride_head : 0, toks ? v_stride_tok : 0,
+                              hs ? v_stride_head : 0};
   int* const to[4] = {&a.k_st, &a.k_sh, &a.v_st, &a.v_sh};
   for (int i = 0; i < 4; ++i) {
     if (strides[i] % 8 != 0) return TM_ERR_ALIGN;

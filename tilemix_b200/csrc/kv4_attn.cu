@@ -22,7 +22,7 @@
 //     from its code by OR-ing it into the mantissa of 1024, one exact add (or FMA)
 //     and one FMA with the group's scale and minimum, which rounds it to fp16 once
 //     (the tensor core's operand type); p is rounded to fp16 as the prefill's
-//     kernels do; scores, maxima, sums and the output accumulate in fp32.
+//     kernels do, times 2^15; scores, maxima, sums and the output accumulate in fp32.
 // 64 requests of 512 to 8192 keys (24 query heads, 8 of 128 cached): 84 us, 4.2
 // TB/s, where the bytes alone would take 54; one request of 131,072 keys 45 us (26).
 // What bounds it is a step's instructions, the unpacking of V first among them,
@@ -55,6 +55,12 @@ constexpr int kSms = 148;
 // with several short requests was the last to end: 64 requests of 512 to 8192 keys took 94 us, 82 so (89 with 1, 83
 // with 2).
 constexpr int kSetup = 4;
+
+// The softmax weights and their sums carry a factor of 2^15, which cancels in the end: the largest is 2^15 instead of 1,
+// still exact in fp16, and a weight keeps fp16's 11 bits down to 2^-29 of the largest. Without it those under 2^-14
+// lost bits and those under 2^-25 all of them: behind one key that drew nearly all of a row, 8192 keys of 2^-25.5 of its
+// weight each came out a quarter too small.
+constexpr float kWeightBits = 15.f;
 
 // CTAs an SM of the kernel for head_dim d and nt row tiles, by registers and shared memory.
 constexpr int resident(int d, int nt) { return d == 128 && nt == 2 ? 2 : 3; }
@@ -446,10 +452,10 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
     const uint8_t* mask = a.mask != nullptr ? a.mask + b * a.mask_stride : nullptr;
 
     float o[NT][2 * G][4];
-    // Running maximum in the scores' units and in log2 units (-inf and 0 while there is none), and running sum. The
-    // maximum moves with every larger score: letting it lag by up to 2^8 saved rescales (83 us against 85 for 64
-    // requests of 512 to 8192 keys), but then the heaviest weight is no longer 1, exact in fp16 (error 3.2e-4
-    // against 2.9e-4).
+    // Running maximum in the scores' units, and in log2 units less kWeightBits (-inf and 0 while there is none), and
+    // running sum. The maximum moves with every larger score: letting it lag by up to 2^8 saved rescales (83 us against
+    // 85 for 64 requests of 512 to 8192 keys), but then the heaviest weight is no longer a power of two, exact in fp16
+    // (error 3.2e-4 against 2.9e-4).
     float m[NT][2], mc[NT][2], l[NT][2];
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
@@ -587,7 +593,7 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
             // m = -inf: nothing summed yet, and 0 stays 0
             f[c] = m[x][c] == top ? 1.f : ex2_approx((m[x][c] - top) * cs[x][c]);
             m[x][c] = top;
-            mc[x][c] = top == -CUDART_INF_F ? 0.f : top * cs[x][c];
+            mc[x][c] = top == -CUDART_INF_F ? 0.f : fmaf(top, cs[x][c], -kWeightBits);
             l[x][c] *= f[c];
           }
 #pragma unroll

@@ -310,3 +310,25 @@ def test_tables_of_more_than_2_30_keys(columns):
     args.update(block_table=_i32(3, columns), out=_Fake((3, 4, 64)))
     with pytest.raises(AssertionError, match="went on to allocate"):
         kv4_attention(**args)
+
+
+def test_threads_share_one_error_word(monkeypatch):
+    """Two threads whose first calls overlap: both launch with the word that is read, and that stays allocated."""
+    from tilemix_b200 import _lib
+    from tilemix_b200.attention import tilemix
+
+    monkeypatch.setattr(_lib, "_ERROR_WORD_PTRS", {})
+    monkeypatch.setattr(tilemix, "_ERROR_WORDS", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    others, kept, zeros = [], [], torch.zeros
+
+    def overlapping(*size, dtype, device):
+        if not others:  # the other thread makes its whole call while this one allocates
+            others.append(None)
+            others[0] = _lib.error_word_ptr(0)
+        kept.append(zeros(*size, dtype=dtype))
+        return kept[-1]
+
+    monkeypatch.setattr(torch, "zeros", overlapping)
+    mine = _lib.error_word_ptr(0)
+    assert mine == others[0] == _lib.error_word_ptr(0) == tilemix._ERROR_WORDS[0].data_ptr()

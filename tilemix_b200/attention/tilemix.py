@@ -61,8 +61,8 @@ def _error_word(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     w = _ERROR_WORDS.get(idx)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-        _ERROR_WORDS[idx] = w
+        # threads whose first calls overlap get the same one: its address is kept
+        w = _ERROR_WORDS.setdefault(idx, torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx)))
     return w
 
 

@@ -628,3 +628,21 @@ def test_strides_that_are_not_used_may_be_any(cuda_device, heads, dim):
     assert np.array_equal(pool.cpu().numpy(), ref)
     out = kv4_attention(single, pool, table.expand(5, 1), torch.ones(5, dtype=torch.int32, device=cuda_device))
     assert torch.equal(out, v[:1].expand(5, 1, dim))
+
+
+def test_errors_of_another_stream_are_read(cuda_device):
+    """device_error_code waits for the device, not for the current stream alone."""
+    from tilemix_b200.attention.kv4 import kv4_append, kv4_pool
+
+    x = torch.ones((1, 1, 64), dtype=torch.float16, device=cuda_device)
+    pool, slot = kv4_pool(1, 16, 1, 64, cuda_device), torch.tensor([99], device=cuda_device)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(1000)
+        kv4_append(x, x, pool, slot - 99)  # the kernels are loaded, which waits for the device
+        torch.cuda.synchronize()
+        torch.cuda._sleep(50_000_000)  # some 25 ms
+        kv4_append(x, x, pool, slot)
+    assert _error_code() == 13
+    with torch.cuda.stream(side):
+        assert _error_code() == 0  # cleared for every stream

@@ -75,9 +75,11 @@ def device_error_code(device: Optional[torch.device] = None, reset: bool = True)
     """
     device = device or torch.device("cuda", torch.cuda.current_device())
     w = _error_word(device)
+    torch.cuda.synchronize(w.device)  # the kernels of every stream
     code = int(w.item())
     if reset and code:
         w.zero_()
+        torch.cuda.synchronize(w.device)  # before another stream's next kernel
     return code
 
 

@@ -564,6 +564,7 @@ def test_keys_beyond_their_bound_do_not_shift_the_others(cuda_device, more):
     ([0, 3, 2, 2], [0, 2]),   # the second request's end is in front of its start
     ([0, 3, 5, 9], [0, 1]),   # the third one's rows run past q
     ([-1, 1, 3, 5], [1, 2]),  # the first one's begin in front of q
+    ([0, -2**31, -5, -5], []), ([2**31 - 1, -2**31, 7, 7], []),
     ([0, 2, 4, 6], [0, 1, 2]),
 ])
 def test_offsets_that_do_not_hold_are_reported(cuda_device, offsets, served):

@@ -105,19 +105,18 @@ struct Request {
   int cost;      // those and kSetup, times the KV heads and row tiles: its length in the work list
 };
 
-// Query tokens by the offsets as they were given; 0 where these do not follow on from one another.
-__device__ __forceinline__ int given_queries(const AttnArgs& a, int b) {
-  if (a.cu == nullptr) return 1;
-  const int q0 = a.cu[b], q1 = a.cu[b + 1];
-  return q0 >= 0 && q1 > q0 ? q1 - q0 : 0;
-}
-
 template <int NT>
 __device__ __forceinline__ Request request_of(const AttnArgs& a, int b) {
   Request r;
-  r.q0 = a.cu != nullptr ? a.cu[b] : b;
-  r.n_q = min(given_queries(a, b), a.max_q);
-  if (r.q0 + static_cast<int64_t>(r.n_q) > a.q_tokens) r.n_q = 0;
+  r.q0 = b;
+  int q1 = b + 1;
+  if (a.cu != nullptr) {
+    r.q0 = a.cu[b];
+    q1 = a.cu[b + 1];
+  }
+  // the subtraction may wrap where one of the two is negative, and is not used then
+  r.n_q = min(static_cast<int>(static_cast<uint32_t>(q1) - static_cast<uint32_t>(r.q0)), a.max_q);
+  if (r.q0 < 0 || q1 < r.q0 || r.q0 + static_cast<int64_t>(r.n_q) > a.q_tokens) r.n_q = 0;
   r.kv = static_cast<int>(min(static_cast<int64_t>(max(a.kv_lens[b], 0)), a.max_kv));
   r.tiles = (r.n_q * a.group + 8 * NT - 1) / (8 * NT);
   r.chunks = max(1, (r.kv + kChunkKeys - 1) / kChunkKeys);
@@ -390,8 +389,9 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
     const int n_rows = rq.n_q * a.group;
     // Keys in front of the request's first query token, by the lengths as they were given: max_q and max_kv leave tokens
     // and keys out and do not move the others. Query token i sees before + i + 1 keys, which is at most the length.
-    // Looked up anew for each run: held with the request it cost a register of the loop below (64 requests of 512 to 8192 keys: 88 us, 86 so).
-    const int before = max(a.kv_lens[b], 0) - given_queries(a, b);
+    // Looked up anew for each run: held with the request it cost a register of the loop below (64 requests of 512 to
+    // 8192 keys: 88 us, 86 so).
+    const int before = max(a.kv_lens[b], 0) - (a.cu != nullptr ? a.cu[b + 1] - a.cu[b] : 1);
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
       const int r = row0 + 8 * x + g;

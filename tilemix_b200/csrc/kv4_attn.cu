@@ -590,10 +590,11 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             top = fmaxf(m[x][c], top);
-            // m = -inf: nothing summed yet, and 0 stays 0
-            f[c] = m[x][c] == top ? 1.f : ex2_approx((m[x][c] - top) * cs[x][c]);
+            // By the rounded maxima, which the weights are relative to. m = -inf: nothing summed yet, and 0 stays 0
+            const float now = top == -CUDART_INF_F ? 0.f : fmaf(top, cs[x][c], -kWeightBits);
+            f[c] = m[x][c] == -CUDART_INF_F ? 0.f : ex2_approx(mc[x][c] - now);
             m[x][c] = top;
-            mc[x][c] = top == -CUDART_INF_F ? 0.f : fmaf(top, cs[x][c], -kWeightBits);
+            mc[x][c] = now;
             l[x][c] *= f[c];
           }
 #pragma unroll
@@ -696,7 +697,8 @@ __global__ void __launch_bounds__(kAttnThreads, resident(D, NT)) attn_kernel(con
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) m[x][c] *= cs[x][c];  // log2 units from here on
+      for (int c = 0; c < 2; ++c)  // log2 units from here on, less kWeightBits in all parts
+        m[x][c] = m[x][c] == -CUDART_INF_F ? m[x][c] : mc[x][c];
     // Merge the warps' states, a share of the channel groups each.
 #pragma unroll
     for (int x = 0; x < NT; ++x)
